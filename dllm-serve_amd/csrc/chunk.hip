@@ -1,0 +1,762 @@
+// Attention of a chunk of new tokens over a paged cache (8-bit or bf16 pages) and
+// over itself, bidirectional, causal or causal between blocks.
+//
+// Segment s has n cached rows, in pages or by slot, and L new rows whose K / V are
+// given in bf16.  New row t sees every cached row and the new rows j < vis(t):
+//   vis(t) = L                                  mask_block = 0
+//   vis(t) = min(L, ((n + t) / b + 1) * b - n)  mask_block = b >= 1 (1: causal)
+// so only tiles of new rows ever need a mask that differs from row to row.
+//
+// "M rows" pack the g = Hq / Hkv query heads of a KV head: M row m is token m / g,
+// head hkv * g + m % g; every K / V byte that is read serves all of them.
+//
+//   * chunk_rows_kernel (few M rows: single tokens, blocks): each of a workgroup's
+//     four wavefronts takes 32-key tiles of its own; K goes from memory straight
+//     into MFMA operands, V through the wavefront's own LDS for the transposition.
+//     No wavefront waits for another until the states are merged at the end.
+//   * long caches are split over workgroups; chunk_combine_kernel joins the parts.
+#include "attn_tile.h"
+#include "quant.h"
+
+#include <type_traits>
+
+namespace dllm {
+
+struct ChunkArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* o;
+  const uint8_t* kc;      // cache: records (8-bit) or bf16 rows [slots][Hkv][128]
+  const uint8_t* vc;
+  const int32_t* cu;
+  const int32_t* seg_ids;
+  const int32_t* table;   // page table [n_seg][max_pages], or the slot list
+  const int32_t* lens;    // cached lengths [n_seg], or slot offsets [n_seg + 1]
+  float* ws;
+  int64_t q_stride, k_stride, v_stride, o_stride;
+  int64_t cache_rows;     // rows of the cache (a multiple of 256 with pages)
+  int max_pages, max_q, max_cached;
+  int n_seg, Hkv, g, mtiles, n_split, tiles_per_split;
+  int mask_block;
+  int logical_blocks, xcd_chunk;
+  float scale_log2;
+};
+
+constexpr int kTileKeys = 32;   // keys of a wavefront's tile
+constexpr int kVTile = kTileKeys * 256;
+
+// Segment s: new rows' first row and count, cached rows.
+struct Segment {
+  int row0, len, cached;
+  int64_t slot0;  // slot list: first entry
+};
+template <bool PAGED>
+__device__ __forceinline__ Segment segment(const ChunkArgs& a, int s) {
+  Segment g;
+  const int id = a.seg_ids ? a.seg_ids[s] : s;
+  g.row0 = a.cu[id];
+  g.len = a.cu[id + 1] - g.row0;
+  if (PAGED) {
+    g.cached = a.lens[s];
+    g.slot0 = 0;
+  } else {
+    g.slot0 = a.lens[s];
+    g.cached = a.lens[s + 1] - (int)g.slot0;
+  }
+  // what the launch was sized for
+  g.len = min(max(g.len, 0), a.max_q);
+  g.cached = min(max(g.cached, 0), a.max_cached);
+  return g;
+}
+
+// New rows that new row t sees.
+__device__ __forceinline__ int visible(const Segment& g, int t, int mask_block) {
+  if (mask_block == 0) return g.len;
+  const int64_t end = (((int64_t)g.cached + t) / mask_block + 1) * mask_block - g.cached;
+  return (int)min((int64_t)g.len, end);
+}
+
+// Splits of a segment's cached tiles that hold any (at least one: the new rows
+// belong to the last).
+__device__ __forceinline__ int splits_of(int cached, int tiles_per_split) {
+  const int tiles = (cached + kTileKeys - 1) / kTileKeys;
+  return max(1, (tiles + tiles_per_split - 1) / tiles_per_split);
+}
+
+__device__ __forceinline__ float row_max4(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  x = pair_max32(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
+                                                  false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float row_sum4(float x) {
+  x = pair_sum32(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
+                                                  false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// ---------------------------------------------------------------------------
+// Few M rows.  Per wavefront and 32-key tile, with 16x16x32 MFMAs:
+//   S^T[16 keys x 16 rows] = K . Q^T   two key halves u, four steps of 32 d each
+//   O^T[16 d x 16 rows]   += V^T . P^T eight d blocks, one step of 32 keys
+// Lane (c = l % 16, g4 = l / 16) holds K row 16 u + c and, in the results, M row c:
+// scores of keys 16 u + 4 g4 + i, outputs d = 16 dt + 4 g4 + i.  A contraction does
+// not depend on the order of its index, so the four lanes of a K row each take
+// whole 16-byte pieces of it (FP8: piece c2 covers d = 64 c2 + 16 g4 .. + 15, two
+// steps; bf16: step s covers d = 32 s + 8 g4 .. + 7), Q^T is loaded in the same
+// order, and P^T is fed to the second product as it stands: its index (g4, i) is
+// key 4 g4 + i for i < 4 and 16 + 4 g4 + i - 4 otherwise, which V^T follows.
+//
+// V goes to the wavefront's LDS tile [32 keys][256 B] in bf16, 16-byte chunk p of a
+// row at p ^ 2 (row & 7), and comes back by ds_read_b64_tr_b16: the eight lanes of a
+// write phase and the sixteen (row, chunk) pairs of a read phase fall on different banks.
+template <bool FP8>
+struct TileRegs {
+  static constexpr int N = FP8 ? 2 : 4;  // 16-byte pieces of a lane's row
+  u32x4_t k[2][N];
+  u32x4_t v[2][N];
+  uint32_t kscale[2], vscale[2];  // 8-bit rows: scale bytes (pages: one word holds all four, see unpack)
+  uint32_t bad;                   // keys to leave out
+};
+
+// Floats of a wavefront's parked O (rows of 128 + 4, which spreads them over the
+// banks) and bytes of a workgroup's LDS: V tiles, then the parked O, then m and l.
+constexpr int park_floats(int nb) { return 16 * nb * 132; }
+constexpr int park_off(int nb) { return 4 * (park_floats(nb) > kVTile / 4 ? park_floats(nb) : kVTile / 4); }
+constexpr int rows_lds(int nb) { return (park_off(nb) + 8 * 16 * nb) * 4; }
+
+template <int NB>
+struct RowState {
+  f32x4_t o[NB][8];
+  float m[NB], l[NB];  // reference maximum (log2 domain), this lane's part of the row sum
+};
+
+template <int NB>
+__device__ __forceinline__ void rows_init(RowState<NB>& st) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) st.o[b][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    st.m[b] = -INFINITY;
+    st.l[b] = 0.f;
+  }
+}
+
+// Online softmax of one 32-key tile of one row block; p comes back as the B operand.
+__device__ __forceinline__ bf16x8_t rows_softmax(const f32x4_t (&s)[2], f32x4_t (&o)[8], float& m, float& l, float c) {
+  float mx = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+  mx = row_max4(mx) * c;
+  const bool need = mx > m + kLazy;  // m = -inf: any finite score
+  if (__builtin_amdgcn_ballot_w64(need)) {
+    const float mn = need ? mx : m;
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    l *= alpha;
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[t][i] *= alpha;
+    m = mn;
+  }
+  const float neg = m == -INFINITY ? 0.f : -m;
+  u32x4_t pk;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w >> 1][(2 * w) & 3], c, neg));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w >> 1][(2 * w + 1) & 3], c, neg));
+    pk[w] = cvt_pk_bf16(p0, p1);
+    l = add_bf16x2(pk[w], l);  // the rounded numerators, as the product uses them
+  }
+  return as_bf16x8(pk);
+}
+
+// NaN or infinity among eight bf16 values; the same values with those as zeros.
+__device__ __forceinline__ bool has_nonfinite(u32x4_t x) {
+  bool r = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) r |= (x[w] & 0x7f80u) == 0x7f80u || (x[w] & 0x7f800000u) == 0x7f800000u;
+  return r;
+}
+__device__ __forceinline__ u32x4_t finite_part(u32x4_t x) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if ((x[w] & 0x7f80u) == 0x7f80u) x[w] &= 0xffff0000u;
+    if ((x[w] & 0x7f800000u) == 0x7f800000u) x[w] &= 0xffffu;
+  }
+  return x;
+}
+
+// LDS of one wavefront is read by other lanes than wrote it: nothing may move across.
+__device__ __forceinline__ void wave_lds_fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int NB, bool FP8, bool PAGED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(ChunkArgs a) {
+  constexpr int BM = 16 * NB;
+  constexpr int PARK = park_floats(NB);
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // rows_lds(NB) bytes
+  const int L = xcd_remap(blockIdx.x, a.xcd_chunk);
+  if (L >= a.logical_blocks) return;
+  int r = L;
+  const int mt = r % a.mtiles;
+  r /= a.mtiles;
+  const int split = r % a.n_split;
+  r /= a.n_split;
+  const int hkv = r % a.Hkv;
+  const int s = r / a.Hkv;
+  const Segment sg = segment<PAGED>(a, s);
+  const int g = a.g;
+  const int M = sg.len * g;
+  const int m_base = mt * BM;
+  const int ns = splits_of(sg.cached, a.tiles_per_split);
+  if (m_base >= M || split >= ns) return;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int col = lane & 15, g4 = lane >> 4;
+  uint8_t* const vt = reinterpret_cast<uint8_t*>(lds) + wave * kVTile;
+
+  // ---- Q^T operands and the rows' limits ------------------------------------
+  bf16x8_t qf[NB][4];
+  int lim[NB];  // new rows that M row m_base + 16 b + col sees
+  {
+    const uint32_t qS = (uint32_t)(a.q_stride * 2);
+    const uint32_t qbytes = (uint32_t)sg.len * qS;
+    const __amdgpu_buffer_rsrc_t qrs = make_rsrc(a.q + (int64_t)sg.row0 * a.q_stride, qbytes);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int m = m_base + 16 * b + col;
+      const int tok = m / g;
+      lim[b] = visible(sg, min(tok, sg.len - 1), a.mask_block);
+      const uint32_t base = m < M ? (uint32_t)tok * qS + (uint32_t)((hkv * g + m - tok * g) * HD) * 2u : qbytes;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const uint32_t off = FP8 ? (uint32_t)((st >> 1) * 128 + g4 * 32 + (st & 1) * 16) : (uint32_t)(st * 64 + g4 * 16);
+        qf[b][st] = as_bf16x8(bload(qrs, base == qbytes ? qbytes : base + off, 0u));
+      }
+    }
+  }
+
+  const int tiles = (sg.cached + kTileKeys - 1) / kTileKeys;
+  const int t_begin = split * a.tiles_per_split;
+  const uint32_t n_rows = (uint32_t)min(a.cache_rows, (int64_t)1 << 31);
+  const int t_end = n_rows ? min(tiles, t_begin + a.tiles_per_split) : t_begin;  // no cache: nothing to read
+  const int32_t* const table = PAGED ? a.table + (int64_t)s * a.max_pages : a.table + sg.slot0;
+  const int64_t bf_row = (int64_t)a.Hkv * HD * 2;
+
+  // Loads of cached tile t.  Rows that do not exist (past the cached length, of a
+  // page or slot outside the cache) read row 0 of the cache or nothing, and are in `bad`.
+  auto load_tile = [&](int t, TileRegs<FP8>& x) {
+    const int key0 = t * kTileKeys;
+    const int left = sg.cached - key0;  // >= 1
+    uint32_t bad = left >= 32 ? 0u : ~0u << left;
+    if constexpr (PAGED) {
+      const int pg = key0 >> 8;
+      int pid = pg < a.max_pages ? table[pg] : -1;
+      const bool in = (uint32_t)pid < (n_rows >> 8);
+      pid = in ? pid : 0;
+      if (!in) bad = ~0u;
+      const int row0 = key0 & (kPageRows - 1);
+      const int64_t rec = FP8 ? ((int64_t)pid * a.Hkv + hkv) * kRecord : (int64_t)pid * kPageRows * bf_row + hkv * HD * 2;
+      const uint32_t rowb = FP8 ? kQuantD : (uint32_t)bf_row;
+      // rows past the cached length read as zero through the buffer's bound
+      const uint32_t rows = in ? (uint32_t)min(kPageRows, row0 + left) : 0u;
+      const uint32_t bytes = rows == 0 ? 0u : (rows - 1) * rowb + (FP8 ? kQuantD : HD * 2);
+      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec, bytes), vrs = make_rsrc(a.vc + rec, bytes);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < TileRegs<FP8>::N; ++p) {
+          const uint32_t off = (uint32_t)(row0 + 16 * u + col) * rowb + (uint32_t)(p * 64 + g4 * 16);
+          x.k[u][p] = bload(krs, off, 0u);
+          x.v[u][p] = bload(vrs, off, 0u);
+        }
+      if constexpr (FP8) {
+        // lanes 0..31: the K scales of the tile's rows, 32..63: the V scales
+        const uint8_t* sp = (lane < 32 ? a.kc : a.vc) + (in ? rec : 0) + kScaleOff + row0 + (lane & 31);
+        x.kscale[0] = n_rows && (lane & 31) < left ? *sp : 127u;
+      }
+    } else {
+      u32x4_t zero = {0, 0, 0, 0};
+      uint32_t out = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = 16 * u + col;
+        const uint32_t sl = key < left ? (uint32_t)table[key0 + key] : ~0u;
+        const bool in = sl < n_rows;
+        out |= (uint32_t)(__builtin_amdgcn_ballot_w64(!in) & 0xffffu) << (16 * u);
+#pragma unroll
+        for (int p = 0; p < TileRegs<FP8>::N; ++p) x.k[u][p] = x.v[u][p] = zero;
+        x.kscale[u] = x.vscale[u] = 127u;
+        if (in) {
+          const int64_t rec = FP8 ? record_off(sl, a.Hkv, hkv) : (int64_t)sl * bf_row + hkv * HD * 2;
+          const int64_t row = FP8 ? (int64_t)(sl & (kPageRows - 1)) * kQuantD : 0;
+#pragma unroll
+          for (int p = 0; p < TileRegs<FP8>::N; ++p) {
+            x.k[u][p] = ld128_stream(a.kc + rec + row + p * 64 + g4 * 16);
+            x.v[u][p] = ld128_stream(a.vc + rec + row + p * 64 + g4 * 16);
+          }
+          if constexpr (FP8) {
+            x.kscale[u] = a.kc[rec + kScaleOff + (sl & (kPageRows - 1))];
+            x.vscale[u] = a.vc[rec + kScaleOff + (sl & (kPageRows - 1))];
+          }
+        }
+      }
+      bad = out;
+    }
+    x.bad = bad;
+  };
+
+  RowState<NB> st;
+  rows_init(st);
+  const float c = a.scale_log2;
+  // this lane's transposing-read address: row 4 g4 + col / 4, chunk (col & 3) / 2
+  const int trow = 4 * g4 + (col >> 2);
+  const uint32_t vbase = (uint32_t)(trow * 256 + ((((col & 3) >> 1) ^ (2 * (trow & 7))) * 16) + 8 * (col & 1));
+
+  // K fragments kf[u][step] of the tile, V in LDS: both products and the softmax.
+  auto products = [&](const bf16x8_t (&kf)[2][4], auto&& hide) {
+    bf16x8_t pf[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      f32x4_t sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        sc[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4)
+          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[u][k4], qf[b][k4], sc[u], 0, 0, 0);
+      }
+      hide(sc, b);
+      pf[b] = rows_softmax(sc, st.o[b], st.m[b], st.l[b], c);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      const uint8_t* vp = vt + (vbase ^ (uint32_t)(32 * dt));
+      const u32x2_t lo = ds_read_tr16(vp), hi = ds_read_tr16(vp + 16 * 256);
+      const bf16x8_t af = as_bf16x8(u32x4_t{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        st.o[b][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pf[b], st.o[b][dt], 0, 0, 0);
+    }
+  };
+  auto put_v = [&](int row, int chunk, u32x4_t w) {
+    *reinterpret_cast<u32x4_t*>(vt + row * 256 + ((chunk ^ (2 * (row & 7))) * 16)) = w;
+  };
+
+  auto compute_tile = [&](const TileRegs<FP8>& x) {
+    float ks[2], vs[2];
+    if constexpr (FP8) {
+      if constexpr (PAGED) {
+        // rows of 16 lanes of the word hold K u = 0, K u = 1, V u = 0, V u = 1: each to all lanes
+        const uint32_t w = x.kscale[0] << 23;
+        const auto h = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+        const auto r0 = __builtin_amdgcn_permlane32_swap((uint32_t)h[0], (uint32_t)h[0], false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap((uint32_t)h[1], (uint32_t)h[1], false, false);
+        ks[0] = __uint_as_float((uint32_t)r0[0]);
+        vs[0] = __uint_as_float((uint32_t)r0[1]);
+        ks[1] = __uint_as_float((uint32_t)r1[0]);
+        vs[1] = __uint_as_float((uint32_t)r1[1]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          ks[u] = scale_of(x.kscale[u]);
+          vs[u] = scale_of(x.vscale[u]);
+        }
+      }
+    }
+    wave_lds_fence();  // the reads of the tile before
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int p = 0; p < TileRegs<FP8>::N; ++p) {
+        const int row = 16 * u + col;
+        if constexpr (FP8) {
+          put_v(row, 8 * p + 2 * g4, dequant8(u32x2_t{x.v[u][p][0], x.v[u][p][1]}, vs[u]));
+          put_v(row, 8 * p + 2 * g4 + 1, dequant8(u32x2_t{x.v[u][p][2], x.v[u][p][3]}, vs[u]));
+        } else {
+          put_v(row, 4 * p + g4, x.v[u][p]);
+        }
+      }
+    wave_lds_fence();
+    bf16x8_t kf[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int p = 0; p < TileRegs<FP8>::N; ++p) {
+        if constexpr (FP8) {
+          kf[u][2 * p] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][0], x.k[u][p][1]}, ks[u]));
+          kf[u][2 * p + 1] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][2], x.k[u][p][3]}, ks[u]));
+        } else {
+          kf[u][p] = as_bf16x8(x.k[u][p]);
+        }
+      }
+    const uint32_t bad = x.bad;
+    products(kf, [&](f32x4_t (&sc)[2], int) {
+      if (bad) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((bad >> (16 * u + 4 * g4 + i)) & 1u) sc[u][i] = -INFINITY;
+      }
+    });
+  };
+
+  // ---- cached tiles: this wavefront takes every fourth, the next one in flight ----
+  {
+    TileRegs<FP8> x, y;
+    int t = t_begin + wave;
+    if (t < t_end) load_tile(t, x);
+    for (; t < t_end; t += 8) {
+      if (t + 4 < t_end) load_tile(t + 4, y);
+      compute_tile(x);
+      if (t + 4 < t_end) {
+        if (t + 8 < t_end) load_tile(t + 8, x);
+        compute_tile(y);
+      }
+    }
+  }
+
+  // ---- new rows (the last split's), bf16 from k / v ------------------------------
+  if (split == ns - 1) {
+    const uint32_t kS = (uint32_t)(a.k_stride * 2), vS = (uint32_t)(a.v_stride * 2);
+    const uint32_t kb = (uint32_t)(sg.len - 1) * kS + HD * 2, vb = (uint32_t)(sg.len - 1) * vS + HD * 2;
+    const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.k + (int64_t)sg.row0 * a.k_stride + hkv * HD, kb);
+    const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD, vb);
+    // the furthest new row that any of this workgroup's rows sees
+    const int last = min(m_base + BM, M) - 1;
+    const int see = visible(sg, last / g, a.mask_block);
+    const int new_tiles = (see + kTileKeys - 1) / kTileKeys;
+    const int turn = max(t_end - t_begin, 0);
+    for (int t = (wave - turn) & 3; t < new_tiles; t += 4) {
+      bf16x8_t kf[2][4];
+      u32x4_t vx[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t row = (uint32_t)(t * kTileKeys + 16 * u + col);
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const uint32_t off = FP8 ? (uint32_t)((k4 >> 1) * 128 + g4 * 32 + (k4 & 1) * 16) : (uint32_t)(k4 * 64 + g4 * 16);
+          kf[u][k4] = as_bf16x8(bload(krs, row < (uint32_t)sg.len ? row * kS + off : kb, 0u));
+          vx[u][k4] = bload(vrs, row < (uint32_t)sg.len ? row * vS + (uint32_t)(k4 * 64 + g4 * 16) : vb, 0u);
+        }
+      }
+      // A NaN or infinity in a V row that some M row does not see would reach that row
+      // as 0 * V.  Such elements (rare) are multiplied as zeros and added afterwards
+      // to the rows that see them.
+      bool odd = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) odd |= has_nonfinite(vx[u][p]);
+      const bool fix = __builtin_amdgcn_ballot_w64(odd) != 0;
+      if (fix) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) vx[u][p] = finite_part(vx[u][p]);
+      }
+      wave_lds_fence();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) put_v(16 * u + col, 4 * p + g4, vx[u][p]);
+      wave_lds_fence();
+      products(kf, [&](f32x4_t (&sc)[2], int b) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t * kTileKeys + 16 * u + 4 * g4 + i >= lim[b]) sc[u][i] = -INFINITY;
+      });
+      if (fix) {
+        const int end = min((t + 1) * kTileKeys, sg.len);
+        for (int j = t * kTileKeys; j < end; ++j)
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) {
+            const u32x2_t w = __builtin_bit_cast(
+                u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(vrs, (int)((uint32_t)j * vS + (uint32_t)(32 * dt + 8 * g4)), 0, 0));
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              if (j < lim[b]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+                  if ((h & 0x7f80u) == 0x7f80u) st.o[b][dt][i] += bf16_bits_to_f32(h);
+                }
+              }
+          }
+      }
+    }
+  }
+
+  // ---- merge of the four wavefronts ------------------------------------------------
+  float* const ml = lds + park_off(NB);
+  __syncthreads();  // the V tiles are free
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const float lt = row_sum4(st.l[b]);
+    if (g4 == 0) {
+      ml[(wave * 2) * BM + 16 * b + col] = st.m[b];
+      ml[(wave * 2 + 1) * BM + 16 * b + col] = lt;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt)
+      *reinterpret_cast<f32x4_t*>(lds + wave * PARK + (16 * b + col) * 132 + 16 * dt + 4 * g4) = st.o[b][dt];
+  }
+  __syncthreads();
+  constexpr int TPR = 256 / BM;   // threads of a row
+  constexpr int DPT = HD / TPR;   // d positions of a thread
+  const int row = tid / TPR, d0 = (tid % TPR) * 4;  // d0 + 4 TPR j
+  const int m = m_base + row;
+  if (m >= M) return;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[(w * 2) * BM + row]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  float f[4], lsum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float mw = ml[(w * 2) * BM + row];
+    f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mu);
+    lsum += ml[(w * 2 + 1) * BM + row] * f[w];
+  }
+  const int tok = m / g, head = hkv * g + (m - tok * g);
+  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+  const int64_t rec = ((((int64_t)s * a.Hkv + hkv) * a.mtiles + mt) * a.n_split + split) * BM + row;
+#pragma unroll
+  for (int j = 0; j < DPT / 4; ++j) {
+    const int d = d0 + 4 * TPR * j;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (f[w] == 0.f) continue;  // a wavefront without keys
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(lds + w * PARK + row * 132 + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += x[e] * f[w];
+    }
+    if (ns == 1) {
+      const u32x2_t w2 = {cvt_pk_bf16(acc[0] * inv, acc[1] * inv), cvt_pk_bf16(acc[2] * inv, acc[3] * inv)};
+      *reinterpret_cast<u32x2_t*>(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + head * HD + d) = w2;
+    } else {
+      *reinterpret_cast<f32x4_t*>(a.ws + rec * HD + d) = acc;
+    }
+  }
+  if (ns > 1 && d0 == 0) {
+    float* pml = a.ws + (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * BM * HD + rec * 2;
+    pml[0] = mx;
+    pml[1] = lsum;
+  }
+}
+
+// Joins the parts of every (segment, KV head, M row) whose keys were split: a
+// workgroup holds eight rows, 32 threads of four d each.
+__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, int bm, bool paged) {
+  const int64_t idx = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int d0 = (threadIdx.x & 31) * 4;
+  const int per = a.mtiles * bm;
+  const int pair = (int)(idx / per);  // (segment, KV head)
+  if (pair >= a.n_seg * a.Hkv) return;
+  const int mrow = (int)(idx - (int64_t)pair * per);
+  const int hkv = pair % a.Hkv;
+  const int s = pair / a.Hkv;
+  const Segment sg = paged ? segment<true>(a, s) : segment<false>(a, s);
+  const int ns = splits_of(sg.cached, a.tiles_per_split);
+  if (ns == 1 || mrow >= sg.len * a.g) return;
+  const int64_t recs = (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * bm;
+  const int64_t rec0 = (((int64_t)s * a.Hkv + hkv) * a.mtiles + mrow / bm) * a.n_split * bm + mrow % bm;
+  const float* const ml = a.ws + recs * HD;
+  float mx = -INFINITY;
+#pragma unroll 8
+  for (int p = 0; p < ns; ++p) mx = fmaxf(mx, ml[(rec0 + (int64_t)p * bm) * 2]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int p = 0; p < ns; ++p) {
+    const int64_t rec = rec0 + (int64_t)p * bm;
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.ws + rec * HD + d0);
+    const float mp = ml[rec * 2];
+    const float w = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mu);
+    l += ml[rec * 2 + 1] * w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int tok = mrow / a.g, head = hkv * a.g + (mrow - tok * a.g);
+  const u32x2_t w2 = {cvt_pk_bf16(acc[0] * inv, acc[1] * inv), cvt_pk_bf16(acc[2] * inv, acc[3] * inv)};
+  *reinterpret_cast<u32x2_t*>(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + head * HD + d0) = w2;
+}
+
+// ---- launch plan ---------------------------------------------------------------------
+struct ChunkPlan {
+  int nb;                        // 16-row blocks of a workgroup
+  int mtiles;
+  int n_split, tiles_per_split;  // workgroups along the cached keys
+};
+static ChunkPlan chunk_plan(int n_seg, int max_q, int max_cached, int Hq, int Hkv) {
+  ChunkPlan p = {};
+  const int64_t rows = (int64_t)max_q * (Hq / Hkv);
+  p.nb = rows <= 16 ? 1 : 2;
+  p.mtiles = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
+  const int64_t groups = (int64_t)n_seg * Hkv * p.mtiles;
+  const int tiles = (max_cached + kTileKeys - 1) / kTileKeys;
+  int64_t want = groups > 0 ? 512 / groups : 1;
+  const int most = (tiles + 7) / 8;  // at least two tiles a wavefront
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  int tps = (int)((tiles + want - 1) / want);
+  tps = (tps + 3) / 4 * 4;
+  p.tiles_per_split = tps > 0 ? tps : 4;
+  p.n_split = tiles > 0 ? (tiles + p.tiles_per_split - 1) / p.tiles_per_split : 1;
+  return p;
+}
+static size_t chunk_ws(const ChunkPlan& p, int n_seg, int Hkv) {
+  if (p.n_split <= 1) return 0;
+  return (size_t)n_seg * Hkv * p.mtiles * p.n_split * 16 * p.nb * (HD + 2) * sizeof(float);
+}
+
+}  // namespace dllm
+
+using namespace dllm;
+
+static bool chunk_sizes_ok(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D) {
+  return D == HD && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && n_seg >= 0 && max_q >= 0 && max_cached >= 0 &&
+         max_cached <= 0x7fffffff - 64 && (int64_t)max_q * (Hq / Hkv) <= (1 << 30);
+}
+
+extern "C" size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D) {
+  if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D) || n_seg == 0 || max_q == 0) return 0;
+  return chunk_ws(chunk_plan(n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
+}
+
+extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D, int* rows,
+                                            int* n_split, int* grid) {
+  if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
+    return fail(DLLM_ERR_INVALID_ARG, "dllm_attn_chunk_launch_shape: unsupported sizes");
+  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
+  const bool none = n_seg == 0 || max_q == 0;
+  if (rows) *rows = 16 * p.nb;
+  if (n_split) *n_split = p.n_split;
+  if (grid) {
+    const int64_t logical = (int64_t)n_seg * Hkv * p.mtiles * p.n_split;
+    const int64_t grain = 8 * (int64_t)(p.mtiles < 16 ? p.mtiles : 16);
+    *grid = none ? 0 : (int)((logical + grain - 1) / grain * grain);
+  }
+  return DLLM_OK;
+}
+
+static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
+                     const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached, const void* k_cache,
+                     const void* v_cache, int cache_type, int64_t cache_rows, const int32_t* table, int max_pages,
+                     const int32_t* lens, int mask_block, int Hq, int Hkv, int D, int64_t q_stride, int64_t k_stride,
+                     int64_t v_stride, int64_t o_stride, float softmax_scale, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  set_error("");
+  int rc = common_checks(name, q, k, v, o, Hq, Hkv, D, q_stride, k_stride, v_stride, o_stride);
+  if (rc) return rc;
+  if (n_seg < 0 || max_q < 0 || max_cached < 0 || mask_block < 0 || max_pages < 0 || cache_rows < 0)
+    return fail(DLLM_ERR_INVALID_ARG, "%s: negative size", name);
+  if (cache_type != DLLM_CACHE_BF16 && cache_type != DLLM_CACHE_FP8)
+    return fail(DLLM_ERR_INVALID_ARG, "%s: cache type %d", name, cache_type);
+  if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY))
+    return fail(DLLM_ERR_INVALID_ARG, "%s: softmax_scale must be positive and finite", name);
+  if (n_seg == 0 || max_q == 0) return DLLM_OK;
+  if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
+    return fail(DLLM_ERR_UNSUPPORTED, "%s: %d new rows of %d query heads per KV head, %d cached", name, max_q, Hq / Hkv,
+                max_cached);
+  if (!cu || !lens) return fail(DLLM_ERR_INVALID_ARG, "%s: null cu / lengths", name);
+  const int64_t kvs = k_stride > v_stride ? k_stride : v_stride;
+  if ((int64_t)max_q * (q_stride > kvs ? q_stride : kvs) * 2 + 4096 >= ((int64_t)1 << 32))
+    return fail(DLLM_ERR_UNSUPPORTED, "%s: a segment spans more than 4 GiB of q / k / v", name);
+  if (cache_type == DLLM_CACHE_BF16 && (int64_t)Hkv * HD * 2 * kPageRows >= ((int64_t)1 << 31))
+    return fail(DLLM_ERR_UNSUPPORTED, "%s: %d KV heads", name, Hkv);
+  if (cache_rows > ((int64_t)1 << 31)) return fail(DLLM_ERR_UNSUPPORTED, "%s: more than 2^31 cache rows", name);
+  if (cache_rows % kPageRows && (paged || cache_type == DLLM_CACHE_FP8))
+    return fail(DLLM_ERR_INVALID_ARG, "%s: the cache must be whole 256-row pages", name);
+  if (max_cached > 0 && cache_rows > 0) {
+    if (!k_cache || !v_cache || !table || (paged && max_pages == 0))
+      return fail(DLLM_ERR_INVALID_ARG, "%s: null cache / %s", name, paged ? "page table" : "slots");
+    if (!aligned16(k_cache) || !aligned16(v_cache))
+      return fail(DLLM_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", name);
+  }
+  if ((int64_t)n_seg * max_pages >= ((int64_t)1 << 31)) return fail(DLLM_ERR_INVALID_ARG, "%s: page table too large", name);
+  ChunkArgs a = {};
+  a.q = q; a.k = k; a.v = v; a.o = o;
+  a.kc = reinterpret_cast<const uint8_t*>(k_cache);
+  a.vc = reinterpret_cast<const uint8_t*>(v_cache);
+  a.cu = cu; a.seg_ids = seg_ids; a.table = table; a.lens = lens;
+  a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.o_stride = o_stride;
+  a.cache_rows = cache_rows;
+  a.max_pages = max_pages; a.max_q = max_q; a.max_cached = max_cached;
+  a.n_seg = n_seg; a.Hkv = Hkv; a.g = Hq / Hkv;
+  a.mask_block = mask_block;
+  a.scale_log2 = softmax_scale * kLog2e;
+  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
+  a.mtiles = p.mtiles; a.n_split = p.n_split; a.tiles_per_split = p.tiles_per_split;
+  const size_t need = chunk_ws(p, n_seg, Hkv);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(DLLM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", name, need,
+                  workspace ? workspace_bytes : (size_t)0);
+    if (!aligned16(workspace)) return fail(DLLM_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
+    a.ws = reinterpret_cast<float*>(workspace);
+  }
+  const int64_t logical = (int64_t)n_seg * Hkv * p.mtiles * p.n_split;
+  if (logical > (int64_t)1 << 28) return fail(DLLM_ERR_INVALID_ARG, "%s: problem too large", name);
+  a.logical_blocks = (int)logical;
+  // the row blocks of a (segment, KV head) read the same keys: next to each other on one XCD
+  a.xcd_chunk = p.mtiles < 16 ? p.mtiles : 16;
+  const int64_t grain = 8 * (int64_t)a.xcd_chunk;
+  const unsigned grid = (unsigned)((logical + grain - 1) / grain * grain);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto pick = [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    return cache_type == DLLM_CACHE_FP8 ? (paged ? chunk_rows_kernel<NB, true, true> : chunk_rows_kernel<NB, true, false>)
+                                        : (paged ? chunk_rows_kernel<NB, false, true> : chunk_rows_kernel<NB, false, false>);
+  };
+  auto kern = p.nb == 1 ? pick(std::integral_constant<int, 1>()) : pick(std::integral_constant<int, 2>());
+  if ((rc = set_lds(kern, rows_lds(p.nb), name))) return rc;
+  kern<<<dim3(grid), dim3(256), rows_lds(p.nb), st>>>(a);
+  if ((rc = check_launch(name))) return rc;
+  if (p.n_split > 1) {
+    const int64_t rows = (int64_t)n_seg * Hkv * p.mtiles * 16 * p.nb;
+    chunk_combine_kernel<<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a, 16 * p.nb, paged);
+    rc = check_launch(name);
+  }
+  return rc;
+}
+
+extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
+                                         const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
+                                         const void* k_cache, const void* v_cache, int cache_type, int num_pages,
+                                         const int32_t* page_table, int max_pages, const int32_t* cached_len,
+                                         int mask_block, int Hq, int Hkv, int D, int64_t q_stride_tok,
+                                         int64_t k_stride_tok, int64_t v_stride_tok, int64_t o_stride_tok,
+                                         float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "dllm_attn_chunk_paged_fwd";
+  if (num_pages < 0 || num_pages > (1 << 23)) return fail(DLLM_ERR_INVALID_ARG, "%s: %d pages", name, num_pages);
+  return chunk_fwd(name, true, q, k, v, o, cu, seg_ids, n_seg, max_q, max_cached, k_cache, v_cache, cache_type,
+                   (int64_t)num_pages * kPageRows, page_table, max_pages, cached_len, mask_block, Hq, Hkv, D,
+                   q_stride_tok, k_stride_tok, v_stride_tok, o_stride_tok, softmax_scale, workspace, workspace_bytes,
+                   stream);
+}
+
+extern "C" int dllm_attn_chunk_slots_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
+                                         const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
+                                         const void* k_cache, const void* v_cache, int cache_type, int64_t cache_slots,
+                                         const int32_t* slots, const int32_t* slot_off, int mask_block, int Hq, int Hkv,
+                                         int D, int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
+                                         int64_t o_stride_tok, float softmax_scale, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  return chunk_fwd("dllm_attn_chunk_slots_fwd", false, q, k, v, o, cu, seg_ids, n_seg, max_q, max_cached, k_cache,
+                   v_cache, cache_type, cache_slots, slots, 0, slot_off, mask_block, Hq, Hkv, D, q_stride_tok,
+                   k_stride_tok, v_stride_tok, o_stride_tok, softmax_scale, workspace, workspace_bytes, stream);
+}

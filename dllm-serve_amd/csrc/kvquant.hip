@@ -1,0 +1,176 @@
+// Quantising KV-cache scatter and its read-back (the 8-bit counterpart of
+// kvcache.hip; row format in quant.h).
+//
+// Sixteen lanes carry one (token, KV head) row of K and of V, eight elements each:
+// one 16-byte load, the row's maximum by four cross-lane steps, one 8-byte store
+// (the sixteen lanes write a whole 128-byte line), and one lane's scale byte.  The
+// reverse reads 8 bytes and the scale and writes 16.  Both are bound by memory: 516
+// bytes read and written per row and matrix pair for 258 on the other side.
+#include "quant.h"
+
+namespace dllm {
+
+struct QuantArgs {
+  uint16_t* k;  // token rows (read by the store, written by the load)
+  uint16_t* v;
+  uint8_t* kp;  // pages
+  uint8_t* vp;
+  const int32_t* slot;
+  int64_t k_stride, v_stride;  // elements
+  int64_t n_slots;
+  int rows, Hkv;               // rows = n_tok * Hkv
+  int chunk;                   // consecutive workgroups of an XCD
+};
+
+template <bool VEC>
+__device__ __forceinline__ u32x4_t ld_row8(const uint16_t* p) {
+  if constexpr (VEC) return ld128_stream(p);
+  u32x4_t r;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) r[w] = (uint32_t)p[2 * w] | ((uint32_t)p[2 * w + 1] << 16);
+  return r;
+}
+template <bool VEC>
+__device__ __forceinline__ void st_row8(uint16_t* p, u32x4_t x) {
+  if constexpr (VEC) {
+    st128(p, x);
+  } else {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      p[2 * w] = (uint16_t)x[w];
+      p[2 * w + 1] = (uint16_t)(x[w] >> 16);
+    }
+  }
+}
+
+// U rows of sixteen lanes in flight; a workgroup takes 16 U consecutive (token,
+// head) rows.
+template <bool VEC, int U>
+__global__ __launch_bounds__(256) void kv_quant_store(QuantArgs a) {
+  const int L = (int)(blockIdx.x & 7) * a.chunk + (int)(blockIdx.x >> 3);
+  const int lane16 = threadIdx.x & 15;
+  const int row0 = L * 16 * U + (threadIdx.x >> 4);
+  u32x4_t kx[U], vx[U];
+  int64_t slot[U];
+  int head[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int row = row0 + 16 * u;
+    slot[u] = -1;
+    head[u] = 0;
+    kx[u] = vx[u] = u32x4_t{0, 0, 0, 0};
+    if (row < a.rows) {
+      const int tok = (int)((uint32_t)row / (uint32_t)a.Hkv);
+      head[u] = row - tok * a.Hkv;
+      const int64_t e = (int64_t)head[u] * kQuantD + lane16 * 8;
+      slot[u] = a.slot[tok];
+      kx[u] = ld_row8<VEC>(a.k + (int64_t)tok * a.k_stride + e);
+      vx[u] = ld_row8<VEC>(a.v + (int64_t)tok * a.v_stride + e);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint32_t kb, vb;
+    const u32x2_t kc = quant_row16(kx[u], kb);
+    const u32x2_t vc = quant_row16(vx[u], vb);
+    if (slot[u] < 0 || slot[u] >= a.n_slots) continue;
+    const int64_t rec = record_off((uint32_t)slot[u], a.Hkv, head[u]);
+    const int r = (int)(slot[u] & (kPageRows - 1));
+    *reinterpret_cast<u32x2_t*>(a.kp + rec + r * kQuantD + lane16 * 8) = kc;
+    *reinterpret_cast<u32x2_t*>(a.vp + rec + r * kQuantD + lane16 * 8) = vc;
+    if (lane16 == 0) {
+      a.kp[rec + kScaleOff + r] = (uint8_t)kb;
+      a.vp[rec + kScaleOff + r] = (uint8_t)vb;
+    }
+  }
+}
+
+template <bool VEC, int U>
+__global__ __launch_bounds__(256) void kv_quant_load(QuantArgs a) {
+  const int L = (int)(blockIdx.x & 7) * a.chunk + (int)(blockIdx.x >> 3);
+  const int lane16 = threadIdx.x & 15;
+  const int row0 = L * 16 * U + (threadIdx.x >> 4);
+  u32x2_t kc[U], vc[U];
+  uint32_t kb[U], vb[U];
+  uint16_t *ko[U], *vo[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int row = row0 + 16 * u;
+    ko[u] = nullptr;
+    if (row < a.rows) {
+      const int tok = (int)((uint32_t)row / (uint32_t)a.Hkv);
+      const int head = row - tok * a.Hkv;
+      const int64_t slot = a.slot[tok];
+      if (slot >= 0 && slot < a.n_slots) {
+        const int64_t e = (int64_t)head * kQuantD + lane16 * 8;
+        const int64_t rec = record_off((uint32_t)slot, a.Hkv, head);
+        const int r = (int)(slot & (kPageRows - 1));
+        ko[u] = a.k + (int64_t)tok * a.k_stride + e;
+        vo[u] = a.v + (int64_t)tok * a.v_stride + e;
+        kc[u] = *reinterpret_cast<const u32x2_t*>(a.kp + rec + r * kQuantD + lane16 * 8);
+        vc[u] = *reinterpret_cast<const u32x2_t*>(a.vp + rec + r * kQuantD + lane16 * 8);
+        kb[u] = a.kp[rec + kScaleOff + r];
+        vb[u] = a.vp[rec + kScaleOff + r];
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (ko[u]) {
+      st_row8<VEC>(ko[u], dequant8(kc[u], scale_of(kb[u])));
+      st_row8<VEC>(vo[u], dequant8(vc[u], scale_of(vb[u])));
+    }
+}
+
+template <bool STORE>
+static int kv_quant(const char* name, uint16_t* k, int64_t ks, uint16_t* v, int64_t vs, uint8_t* kp, uint8_t* vp,
+                    int64_t num_pages, const int32_t* slot, int n_tok, int Hkv, int D, void* stream) {
+  set_error("");
+  if (D != kQuantD) return fail(DLLM_ERR_UNSUPPORTED, "%s: head_dim %d not supported (the kernels handle 128)", name, D);
+  if (n_tok < 0 || Hkv <= 0 || num_pages < 0 || num_pages > ((int64_t)1 << 23))
+    return fail(DLLM_ERR_INVALID_ARG, "%s: bad sizes n_tok=%d Hkv=%d num_pages=%lld (at most 2^23 pages)", name, n_tok,
+                Hkv, (long long)num_pages);
+  if (n_tok == 0 || num_pages == 0) return DLLM_OK;  // without pages every slot is outside the cache
+  if (!k || !v || !kp || !vp || !slot) return fail(DLLM_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (ks < (int64_t)Hkv * D || vs < (int64_t)Hkv * D)
+    return fail(DLLM_ERR_INVALID_ARG, "%s: token stride (%lld, %lld) smaller than a token row of %lld", name,
+                (long long)ks, (long long)vs, (long long)Hkv * D);
+  if (!aligned16(kp) || !aligned16(vp)) return fail(DLLM_ERR_INVALID_ARG, "%s: pages must be 16-byte aligned", name);
+  if ((int64_t)n_tok * Hkv > ((int64_t)1 << 30))
+    return fail(DLLM_ERR_UNSUPPORTED, "%s: %d tokens of %d KV heads in one call", name, n_tok, Hkv);
+  const bool vec = ks % 8 == 0 && vs % 8 == 0 && aligned16(k) && aligned16(v);
+  QuantArgs a = {};
+  a.k = k; a.v = v; a.kp = kp; a.vp = vp; a.slot = slot;
+  a.k_stride = ks; a.v_stride = vs;
+  a.n_slots = num_pages * kPageRows;
+  a.rows = n_tok * Hkv;
+  a.Hkv = Hkv;
+  const int U = 1;
+  const int64_t blocks = ((int64_t)a.rows + 16 * U - 1) / (16 * U);
+  // consecutive workgroups on one XCD: the scale bytes of a page's rows share lines
+  a.chunk = (int)((blocks + 7) / 8);
+  auto kern = STORE ? (vec ? kv_quant_store<true, U> : kv_quant_store<false, U>)
+                    : (vec ? kv_quant_load<true, U> : kv_quant_load<false, U>);
+  kern<<<dim3((unsigned)a.chunk * 8), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+  return check_launch(name);
+}
+
+}  // namespace dllm
+
+extern "C" size_t dllm_quant_page_bytes(int D) { return D == dllm::kQuantD ? dllm::kRecord : 0; }
+
+extern "C" int dllm_store_kvcache_fp8(const dllm_bf16* key, int64_t key_stride_tok, const dllm_bf16* value,
+                                      int64_t value_stride_tok, uint8_t* k_pages, uint8_t* v_pages, int64_t num_pages,
+                                      const int32_t* slot_mapping, int n_tok, int Hkv, int D, void* stream) {
+  return dllm::kv_quant<true>("dllm_store_kvcache_fp8", const_cast<dllm_bf16*>(key), key_stride_tok,
+                              const_cast<dllm_bf16*>(value), value_stride_tok, k_pages, v_pages, num_pages,
+                              slot_mapping, n_tok, Hkv, D, stream);
+}
+
+extern "C" int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* value, int64_t value_stride_tok,
+                                     const uint8_t* k_pages, const uint8_t* v_pages, int64_t num_pages,
+                                     const int32_t* slot_mapping, int n_tok, int Hkv, int D, void* stream) {
+  return dllm::kv_quant<false>("dllm_load_kvcache_fp8", key, key_stride_tok, value, value_stride_tok,
+                               const_cast<uint8_t*>(k_pages), const_cast<uint8_t*>(v_pages), num_pages, slot_mapping,
+                               n_tok, Hkv, D, stream);
+}

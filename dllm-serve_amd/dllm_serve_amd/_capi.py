@@ -26,6 +26,11 @@ DLLM_ERR_UNSUPPORTED = -2
 DLLM_ERR_WORKSPACE = -3
 DLLM_ERR_HIP = -4
 
+CACHE_BF16 = 0
+CACHE_FP8 = 1
+PAGE_ROWS = 256
+PAGE_BYTES = PAGE_ROWS * 128 + PAGE_ROWS  # one 8-bit page of one KV head: codes, then scale bytes
+
 # name -> (restype, argtypes); must match include/dllm_attn.h
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -59,6 +64,21 @@ SIGNATURES = {
         _I,
         [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I64, _P, _P, _I, _I, _I,
          _I64, _I64, _I64, _I64, _F, _P],
+    ),
+    "dllm_quant_page_bytes": (_SZ, [_I]),
+    "dllm_store_kvcache_fp8": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I, _I, _I, _P]),
+    "dllm_load_kvcache_fp8": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I, _I, _I, _P]),
+    "dllm_attn_chunk_workspace_size": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "dllm_attn_chunk_launch_shape": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "dllm_attn_chunk_paged_fwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I,
+         _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
+    ),
+    "dllm_attn_chunk_slots_fwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I64, _P, _P, _I, _I, _I, _I,
+         _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
     ),
     "dllm_select_kv_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
     "dllm_select_kv_store": (
@@ -315,6 +335,53 @@ def attn_block_cached_fwd_noalloc(q, k, v, o, cu, seg_ids, n_seg, max_q, max_key
         q.shape[1], Hkv, D,
         q.stride(0), k.stride(0), v.stride(0), o.stride(0), float(scale), _stream(q.device))
     _check(rc, "dllm_attn_block_cached_fwd_noalloc")
+
+
+def store_kvcache_fp8(key, value, k_pages, v_pages, slot_mapping, n_tok, Hkv, D):
+    """K1 into 8-bit pages: rows quantised as they are written (see include/dllm_attn.h)."""
+    _require_gpu(key, value, k_pages, v_pages, slot_mapping)
+    rc = _lib_now().dllm_store_kvcache_fp8(
+        key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+        min(k_pages.numel(), v_pages.numel()) // (Hkv * PAGE_BYTES), slot_mapping.data_ptr(), n_tok, Hkv, D,
+        _stream(key.device))
+    _check(rc, "dllm_store_kvcache_fp8")
+
+
+def load_kvcache_fp8(key, value, k_pages, v_pages, slot_mapping, n_tok, Hkv, D):
+    """K2 from 8-bit pages: what the rows stand for, in bf16."""
+    _require_gpu(key, value, k_pages, v_pages, slot_mapping)
+    rc = _lib_now().dllm_load_kvcache_fp8(
+        key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+        min(k_pages.numel(), v_pages.numel()) // (Hkv * PAGE_BYTES), slot_mapping.data_ptr(), n_tok, Hkv, D,
+        _stream(key.device))
+    _check(rc, "dllm_load_kvcache_fp8")
+
+
+def chunk_workspace_size(n_seg, max_q, max_cached, Hq, Hkv, D) -> int:
+    return int(_lib_now().dllm_attn_chunk_workspace_size(n_seg, max_q, max_cached, Hq, Hkv, D))
+
+
+def chunk_launch_shape(n_seg, max_q, max_cached, Hq, Hkv, D) -> dict:
+    """Launch shape of the chunk attention for these sizes (no launch): M rows
+    per workgroup, workgroups along the keys, grid."""
+    vals = [ctypes.c_int(0) for _ in range(3)]
+    _check(load().dllm_attn_chunk_launch_shape(n_seg, max_q, max_cached, Hq, Hkv, D, *[ctypes.byref(x) for x in vals]),
+           "dllm_attn_chunk_launch_shape")
+    return dict(rows=vals[0].value, n_split=vals[1].value, grid=vals[2].value)
+
+
+def attn_chunk_paged_fwd_raw(*args) -> None:
+    """dllm_attn_chunk_paged_fwd over device addresses the caller has already checked."""
+    rc = _lib_now().dllm_attn_chunk_paged_fwd(*args)
+    if rc != DLLM_OK:
+        _check(rc, "dllm_attn_chunk_paged_fwd")
+
+
+def attn_chunk_slots_fwd_raw(*args) -> None:
+    """dllm_attn_chunk_slots_fwd over device addresses the caller has already checked."""
+    rc = _lib_now().dllm_attn_chunk_slots_fwd(*args)
+    if rc != DLLM_OK:
+        _check(rc, "dllm_attn_chunk_slots_fwd")
 
 
 JOB_COLS = 8  # row0, n_tok, blk_start, blk_len, n_keep, slot_off, head_select, pool_k

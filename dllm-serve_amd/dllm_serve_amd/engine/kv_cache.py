@@ -19,7 +19,18 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from .. import _capi
+
 BLOCK_SIZE = 256
+
+
+def quantized_pages(num_pages: int, num_kv_heads: int, head_dim: int = 128, device=None) -> torch.Tensor:
+    """An empty 8-bit cache of K or of V: uint8 [num_pages, num_kv_heads, 33024]
+    (per page and KV head 256 rows of e4m3 codes, then the rows' scale bytes;
+    an unwritten row reads as zeros)."""
+    if head_dim != 128:
+        raise ValueError(f"8-bit pages hold rows of 128, not of {head_dim}")
+    return torch.zeros(num_pages, num_kv_heads, _capi.PAGE_BYTES, dtype=torch.uint8, device=device)
 
 
 def block_bytes(num_layers: int, num_kv_heads: int, head_dim: int, world_size: int = 1,

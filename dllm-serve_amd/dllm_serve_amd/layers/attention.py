@@ -22,6 +22,7 @@ current HIP stream; nothing falls back to the CPU.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 import struct
 import weakref
@@ -65,7 +66,11 @@ def _slot_tensor(slot_mapping, device) -> torch.Tensor:
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   slot_mapping: torch.Tensor) -> None:
-    """k_cache.flat[slot_mapping[i], :] = key[i], same for value (attention.py:33-50)."""
+    """k_cache.flat[slot_mapping[i], :] = key[i], same for value (attention.py:33-50).
+    With 8-bit pages (quantized_pages) the rows are quantised as they are written."""
+    if k_cache.dtype == torch.uint8 or v_cache.dtype == torch.uint8:
+        _quant_copy(_capi.store_kvcache_fp8, key, value, k_cache, v_cache, slot_mapping)
+        return
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     assert key.stride(-1) == 1 and value.stride(-1) == 1
@@ -82,7 +87,11 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 
 def load_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  slot_mapping: torch.Tensor) -> None:
-    """key[i] = k_cache.flat[slot_mapping[i], :], same for value (attention.py:77-92)."""
+    """key[i] = k_cache.flat[slot_mapping[i], :], same for value (attention.py:77-92).
+    From 8-bit pages the rows come back as the bf16 values they stand for."""
+    if k_cache.dtype == torch.uint8 or v_cache.dtype == torch.uint8:
+        _quant_copy(_capi.load_kvcache_fp8, key, value, k_cache, v_cache, slot_mapping)
+        return
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     assert key.stride(-1) == 1 and value.stride(-1) == 1
@@ -93,6 +102,141 @@ def load_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, 
     assert key.dtype == value.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16, "bf16 tensors expected"
     slot = _slot_tensor(slot_mapping, key.device)
     _capi.load_kvcache(key, value, k_cache, v_cache, slot, N, D)
+
+
+def _check_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, device) -> int:
+    """Check a pair of 8-bit caches and return their KV heads."""
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if (t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != _capi.PAGE_BYTES or not t.is_contiguous()
+                or t.device != device or t.shape[1] != k_cache.shape[1]):
+            raise ValueError(f"{n} must be contiguous 8-bit pages, uint8 [num_pages, KV heads, {_capi.PAGE_BYTES}] on "
+                             f"{device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return k_cache.shape[1]
+
+
+def _on_device(device: torch.device):
+    """Makes `device` current where it is not: a launch on another device's stream fails."""
+    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _quant_copy(copy, key, value, k_cache, v_cache, slot_mapping) -> None:
+    N, num_heads, head_dim = key.shape
+    assert value.shape == key.shape and value.device == key.device
+    assert key.stride(-1) == 1 and value.stride(-1) == 1
+    assert key.stride(1) == head_dim and value.stride(1) == head_dim
+    assert slot_mapping.numel() == N
+    assert key.dtype == value.dtype == torch.bfloat16, "bf16 tensors expected"
+    if _check_pages(k_cache, v_cache, key.device) != num_heads:
+        raise ValueError(f"rows of {num_heads} KV heads, pages of {k_cache.shape[1]}")
+    slot = _slot_tensor(slot_mapping, key.device)
+    with _on_device(key.device):
+        copy(key, value, k_cache, v_cache, slot, N, num_heads, head_dim)
+
+
+class ChunkPlan:
+    """Launch tables of one step's chunk attention, shared by its layers.
+
+    Sequence b feeds ``seqlens[b]`` new rows behind ``cached_lens[b]`` rows in the
+    256-row cache pages ``block_tables[b]`` (host integers; more pages than
+    needed are fine).  ``mask_block`` 0: the new rows see each other; b >= 1:
+    a row sees the rows up to the end of its own block of b positions
+    (1: causal), positions counted from the first cached row.  The tables are
+    uploaded with one asynchronous copy; nothing synchronises."""
+
+    def __init__(self, seqlens, cached_lens, block_tables, device, mask_block: int = 0):
+        seqlens, cached = [int(n) for n in seqlens], [int(n) for n in cached_lens]
+        tables = [[int(p) for p in t] for t in block_tables]
+        if not (len(seqlens) == len(cached) == len(tables)):
+            raise ValueError(f"{len(seqlens)} sequences, {len(cached)} cached lengths, {len(tables)} block tables")
+        if any(n < 0 for n in seqlens + cached) or mask_block < 0:
+            raise ValueError("lengths and mask_block must not be negative")
+        need = [-(-n // _capi.PAGE_ROWS) for n in cached]
+        for b, (t, n) in enumerate(zip(tables, need)):
+            if len(t) < n or any(p < 0 for p in t[:n]):
+                raise ValueError(f"sequence {b}: {cached[b]} cached rows need {n} pages, block table {t[:n]}")
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.n_seg = B = len(seqlens)
+        self.total_rows = sum(seqlens)
+        self.max_q, self.max_cached = max(seqlens, default=0), max(cached, default=0)
+        self.max_pages = W = max(need, default=0)
+        self.max_page = max((p for t, n in zip(tables, need) for p in t[:n]), default=-1)
+        self.mask_block = int(mask_block)
+        flat = np.full(2 * B + 1 + B * W, -1, dtype=np.int64)
+        flat[0] = 0
+        flat[1:B + 1] = np.cumsum(seqlens)
+        flat[B + 1:2 * B + 1] = cached
+        for b, (t, n) in enumerate(zip(tables, need)):
+            flat[2 * B + 1 + b * W:2 * B + 1 + b * W + n] = t[:n]
+        if flat.max() >= 2**31:
+            raise ValueError("chunk tables exceed int32")
+        host = torch.from_numpy(flat.astype(np.int32))
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        dev = host.to(self.device, non_blocking=True)
+        self.cu, self.cached_lens, self.block_tables = dev[:B + 1], dev[B + 1:2 * B + 1], dev[2 * B + 1:]
+        self._args = (self.cu.data_ptr(), self.cached_lens.data_ptr(), self.block_tables.data_ptr())
+
+
+def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    plan: ChunkPlan, softmax_scale: float) -> torch.Tensor:
+    """Attention of every sequence's new rows over its cached rows and over
+    each other (see ChunkPlan), [rows, Hq * 128].
+
+    q / k / v are the new rows of all sequences, packed, as
+    [rows, heads * 128] or [rows, heads, 128] with contiguous heads, bf16.  The
+    caches are 8-bit pages (quantized_pages) or bf16 [num_pages, 256, Hkv,
+    128]; the new rows are read from k / v, so they may be stored before or after."""
+    D = 128
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"bf16 {n} expected, got {t.dtype}")
+        if t.dim() not in (2, 3) or t.numel() != t.shape[0] * (t.shape[1] if t.dim() == 2 else t.shape[1] * D) \
+                or t.dim() == 2 and t.shape[1] % D:
+            raise ValueError(f"{n} must be [rows, heads * 128] or [rows, heads, 128]; got {tuple(t.shape)}")
+    heads = [t.shape[1] // D if t.dim() == 2 else t.shape[1] for t in (q, k, v)]
+    Hq, Hkv = heads[0], heads[1]
+    if heads[2] != Hkv or Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"{heads[0]} / {heads[1]} / {heads[2]} heads of q / k / v")
+    q, nq, q_st = _token_rows(q, Hq, D, "q")
+    k, nk, k_st = _token_rows(k, Hkv, D, "k")
+    v, nv, v_st = _token_rows(v, Hkv, D, "v")
+    dev = q.device
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise RuntimeError("chunk_attention runs on the GPU only (no CPU fallback)")
+    if k.device != dev or v.device != dev or plan.device != dev:
+        raise ValueError(f"q / k / v and the plan are on {q.device} / {k.device} / {v.device} / {plan.device}")
+    if not (nq == nk == nv == plan.total_rows):
+        raise ValueError(f"q / k / v have {nq} / {nk} / {nv} rows, the plan's sequences feed {plan.total_rows}")
+    if k_cache.dtype == torch.uint8:
+        if _check_pages(k_cache, v_cache, dev) != Hkv:
+            raise ValueError(f"k / v of {Hkv} KV heads, pages of {k_cache.shape[1]}")
+        kind, pages = _capi.CACHE_FP8, min(k_cache.shape[0], v_cache.shape[0])
+    else:
+        for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            if (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != dev or t.dim() != 4
+                    or tuple(t.shape[1:]) != (_capi.PAGE_ROWS, Hkv, D)):
+                raise ValueError(f"{n} must be contiguous bf16 [num_pages, {_capi.PAGE_ROWS}, {Hkv}, {D}] or 8-bit pages "
+                                 f"on {dev}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+        kind, pages = _capi.CACHE_BF16, min(k_cache.shape[0], v_cache.shape[0])
+    if plan.max_page >= pages:
+        raise ValueError(f"a block table names page {plan.max_page} of a cache of {pages}")
+    with _on_device(dev):
+        o = torch.empty(nq, Hq * D, dtype=torch.bfloat16, device=dev)
+        need = _capi.chunk_workspace_size(plan.n_seg, plan.max_q, plan.max_cached, Hq, Hkv, D)
+        # from the allocator at every call: a plan may be used on several streams and in several graphs
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        if nq:
+            cu, lens, tables = plan._args
+            _capi.attn_chunk_paged_fwd_raw(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, None, plan.n_seg, plan.max_q,
+                plan.max_cached, k_cache.data_ptr(), v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens,
+                plan.mask_block, Hq, Hkv, D, q_st, k_st, v_st, o.stride(0), float(softmax_scale),
+                None if ws is None else ws.data_ptr(), need, _capi._stream(dev))
+    return o
 
 
 class StepLayout:

@@ -196,6 +196,86 @@ int dllm_attn_block_cached_fwd_noalloc(const dllm_bf16* q, const dllm_bf16* k, c
                                        int64_t o_stride_tok, float softmax_scale, void* stream);
 
 /*
+ * 8-bit KV cache.  No counterpart in the reference, whose cache is in the model's type.
+ *
+ * A page of one KV head is a record of dllm_quant_page_bytes(D) bytes (33024 for D =
+ * 128, 0 for other D): 256 rows of D e4m3 codes, then the 256 rows' scale bytes.  A
+ * cache is [num_pages][Hkv] records, one for K and one for V, 16-byte aligned; slot =
+ * page * 256 + row as in the bf16 cache.  A row x of one (token, KV head) is kept as
+ *   e = max(E - 8 + (m > 1.75), -117),  max |x_i| = m * 2^E, 1 <= m < 2, over finite x_i
+ *   code_i = e4m3(x_i * 2^-e) (round to nearest even),  scale byte = e + 127
+ * and read back as code_i * 2^e, which is exact in bf16 (a value of at least 1.9375 *
+ * 2^127 rounds to 2^128 and reads back as infinity).  NaN and infinities are kept
+ * as NaN.
+ *
+ * dllm_store_kvcache_fp8 is dllm_store_kvcache into such pages, dllm_load_kvcache_fp8
+ * dllm_load_kvcache from them: key / value are [n_tok][Hkv][D] with the given token
+ * strides; a slot outside the cache is skipped, or leaves its row untouched.  The
+ * slots of one store must differ: a row written twice by one call holds parts of
+ * both.
+ */
+size_t dllm_quant_page_bytes(int D);
+int dllm_store_kvcache_fp8(const dllm_bf16* key, int64_t key_stride_tok, const dllm_bf16* value,
+                           int64_t value_stride_tok, uint8_t* k_pages, uint8_t* v_pages, int64_t num_pages,
+                           const int32_t* slot_mapping, int n_tok, int Hkv, int D, void* stream);
+int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* value, int64_t value_stride_tok,
+                          const uint8_t* k_pages, const uint8_t* v_pages, int64_t num_pages,
+                          const int32_t* slot_mapping, int n_tok, int Hkv, int D, void* stream);
+
+/*
+ * Attention of a chunk of new tokens over a paged cache and over itself.  The
+ * reference's counterpart for state 2 is K3b above; this form takes chunks of any
+ * length (one token, a block, a piece of a prompt), 8-bit or bf16 caches
+ * (cache_type: DLLM_CACHE_FP8 as above, or DLLM_CACHE_BF16, [rows][Hkv][D] as
+ * dllm_store_kvcache writes it), and masks among the new tokens.
+ *
+ * Segment s (id = seg_ids ? seg_ids[s] : s) has new rows [cu[id], cu[id+1]) of q, k, v
+ * (L of them) and n cached rows.  Its new row t stands at position n + t and sees
+ * every cached row and the new rows j < vis(t):
+ *   mask_block = 0      vis(t) = L                               (bidirectional)
+ *   mask_block = b > 0  vis(t) = min(L, ((n + t) / b + 1) * b - n)  (causal between
+ *                       blocks of b positions; b = 1: causal)
+ *   o[t, h] = sum_u softmax_u(scale * q[t, h] . k[u, h / (Hq/Hkv)]) v[u, h / (Hq/Hkv)]
+ * over the rows it sees; f32 accumulation, probabilities rounded to bf16 for the
+ * product with V, bf16 output.  The new rows' K / V are read from k and v, not from
+ * the cache: whether they have been stored there does not matter.  A row whose
+ * scores are all -infinity is written as zeros; NaN and infinities in K / V rows
+ * that a row does not see do not reach it.  Rows of o outside the segments are not
+ * written.
+ *
+ * _paged_fwd: cached row r of segment s is row r % 256 of page page_table[s *
+ * max_pages + r / 256], n = cached_len[s].  _slots_fwd: it is cache slot
+ * slots[slot_off[s] + r], n = slot_off[s+1] - slot_off[s].  A row whose page or slot is
+ * outside the cache (or whose page index is >= max_pages) is left out of the softmax.
+ * max_q and max_cached must bound L and n of every segment: longer segments are
+ * cut there.  D must be 128, Hq a multiple of Hkv, softmax_scale positive; pointers are
+ * 16-byte aligned, token strides multiples of 8 elements, and a segment's new rows span
+ * at most 4 GiB of q, k or v.  workspace: dllm_attn_chunk_workspace_size(...) bytes
+ * (0 where one workgroup takes all keys of a row), any contents; calls that may
+ * overlap need workspaces of their own.
+ */
+#define DLLM_CACHE_BF16 0
+#define DLLM_CACHE_FP8 1
+size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D);
+/* Launch shape for these sizes, without launching: M rows (tokens x Hq / Hkv) of a
+ * workgroup, workgroups along the keys, grid.  Any output pointer may be null. */
+int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D, int* rows,
+                                 int* n_split, int* grid);
+int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
+                              const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
+                              const void* k_cache, const void* v_cache, int cache_type, int num_pages,
+                              const int32_t* page_table, int max_pages, const int32_t* cached_len, int mask_block,
+                              int Hq, int Hkv, int D, int64_t q_stride_tok, int64_t k_stride_tok,
+                              int64_t v_stride_tok, int64_t o_stride_tok, float softmax_scale, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int dllm_attn_chunk_slots_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
+                              const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
+                              const void* k_cache, const void* v_cache, int cache_type, int64_t cache_slots,
+                              const int32_t* slots, const int32_t* slot_off, int mask_block, int Hq, int Hkv, int D,
+                              int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok, int64_t o_stride_tok,
+                              float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * K5 / K6 -- sparse KV selection fused with the KV-cache scatter (mode 1 /
  * "compute cache").  Replaces _select_important_head_kv (head_select != 0,
  * dllmserve/layers/attention.py:344-413), _select_important_kv (head_select

@@ -13,6 +13,8 @@ Modules
   select     head / token KV selection with the explicit rounding and
              tie-break rule the GPU kernels implement
   kvcache    store_kvcache / load_kvcache by slot
+  quant      the 8-bit rows of the quantised KV cache, store and load by slot
+  chunk      attention of a chunk of new rows over cached rows and itself
   rope       NeoX rotary embedding (input preparation; expected results of the K7 kernel)
   sampler    low-confidence remasking: softmax-max of logit rows (with the
              Gumbel transform at temperature > 0) and the unmasking step
@@ -26,6 +28,9 @@ Parity pins (what checks each function; see tests/test_oracle_*.py):
   select     exact rational arithmetic + full sort on small inputs, torch.topk
              on tie-free inputs, torch bf16 einsum agreement, special cases
   kvcache    brute-force loops, round trips, untouched-slot sentinels
+  quant      torch's own float8_e4m3fn conversions over every code and over random
+             rows, the scale rule's defining inequality
+  chunk      torch softmax on the causal and bidirectional masks, one row at a time
   rope       norm preservation, relative-position invariance, position 0,
              quarter-turn / half-turn tables (exact swaps and negations),
              agreement with the torch f32 expression

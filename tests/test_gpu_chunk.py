@@ -1,0 +1,337 @@
+"""chunk_attention against the formula in 64 bits, at the lengths, masks and layouts
+where it can go wrong.
+
+The bound of an output, from the roundings the kernels make: the result in bf16 (2^-8
+of it), every probability in bf16 (2^-8, in the numerator and in the row sum alike:
+2^-8 * sum p |v - o|), the scores in f32 (relative change of a probability at most
+twice the error of its score, which is 140 roundings of 2^-23 of sum |q k| and the
+exponential's 2^-20), and the f32 sums over the keys."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import chunk, quant
+from dllm_serve_amd import _capi
+from dllm_serve_amd.engine.kv_cache import quantized_pages
+from dllm_serve_amd.layers.attention import ChunkPlan, chunk_attention, load_kvcache, store_kvcache
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+SCALE = 128 ** -0.5
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def check(out, ref, spread, reach, keys, what=""):
+    o = _np(out).reshape(ref.shape)
+    assert np.array_equal(np.isnan(o), np.isnan(ref)), what
+    ok = np.isfinite(ref)
+    assert np.array_equal(o[~ok & ~np.isnan(ref)], ref[~ok & ~np.isnan(ref)]), what
+    with np.errstate(invalid="ignore"):
+        p = 2.0 ** -8 + 2 * (140 * 2.0 ** -23 * reach[..., None] + 2.0 ** -20)
+        tol = 2.0 ** -8 * np.abs(ref) + 1.05 * p * (spread + np.abs(ref)) + (keys / 16 + 40) * 2.0 ** -23 * spread + 1e-30
+        bad = np.abs(o - ref) > tol
+    assert not (bad & ok).any(), f"{what}: worst {np.nanmax(np.where(ok, np.abs(o - ref) / tol, 0)):.2f} of the bound"
+
+
+class Batch:
+    """New rows, a paged cache of the wanted kind and the cached rows as float64."""
+
+    def __init__(self, dev, lens, cached, Hq, Hkv, bits, seed=0, spare=2, kv_scale=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.dev, self.lens, self.cached, self.Hkv, self.bits = dev, lens, cached, Hkv, bits
+        n = sum(lens)
+
+        def normal(*s):
+            return (kv_scale * torch.randn(*s, generator=g)).to(BF16)
+
+        self.q, self.k, self.v = normal(n, Hq, 128), normal(n, Hkv, 128), normal(n, Hkv, 128)
+        need = [-(-c // 256) for c in cached]
+        self.pages = sum(need) + spare
+        perm = torch.randperm(self.pages, generator=g).tolist()
+        self.tables = [perm[sum(need[:b]):sum(need[:b + 1])] for b in range(len(lens))]
+        rows = self.pages * 256
+        if bits == 8:
+            self.kc, self.vc = quantized_pages(self.pages, Hkv, device=dev), quantized_pages(self.pages, Hkv, device=dev)
+            slots = torch.arange(rows, dtype=torch.int32, device=dev)
+            store_kvcache(normal(rows, Hkv, 128).to(dev), normal(rows, Hkv, 128).to(dev), self.kc, self.vc, slots)
+        else:
+            self.kc = normal(self.pages, 256, Hkv, 128).to(dev)
+            self.vc = normal(self.pages, 256, Hkv, 128).to(dev)
+
+    def slots(self, b):
+        r = np.arange(self.cached[b])
+        return np.array(self.tables[b] or [0])[r // 256] * 256 + r % 256
+
+    def cache_rows(self, pages, b):
+        s = self.slots(b)
+        if self.bits == 8:
+            return quant.load(pages.cpu().numpy(), s)
+        return _np(pages.view(-1, self.Hkv, 128))[s]
+
+    def run(self, mask_block=0, scale=SCALE):
+        plan = ChunkPlan(self.lens, self.cached, self.tables, self.dev, mask_block=mask_block)
+        d = self.dev
+        return chunk_attention(self.q.to(d), self.k.to(d), self.v.to(d), self.kc, self.vc, plan, scale)
+
+    def verify(self, out, mask_block=0, scale=SCALE, keep=None):
+        r0 = 0
+        for b, L in enumerate(self.lens):
+            x = [_np(t[r0:r0 + L]) for t in (self.q, self.k, self.v)]
+            kc, vc = self.cache_rows(self.kc, b), self.cache_rows(self.vc, b)
+            ref, spread, reach = chunk.attend(*x, kc, vc, scale, mask_block, None if keep is None else keep[b])
+            check(out[r0:r0 + L], ref, spread, reach, L + self.cached[b], f"sequence {b}")
+            r0 += L
+
+
+SHAPES = [
+    # lens, cached, Hq, Hkv, mask_block
+    ([1], [0], 2, 2, 1),
+    ([1], [1], 2, 2, 1),
+    ([1, 1, 1], [31, 32, 33], 4, 2, 1),
+    ([1, 1], [255, 257], 7, 1, 0),
+    ([1], [1500], 7, 1, 1),
+    ([2, 3], [64, 700], 2, 1, 1),
+    ([16, 17], [5, 300], 2, 2, 0),
+    ([32, 5, 33], [129, 0, 256], 4, 2, 4),
+    ([0, 7, 0, 40], [300, 13, 0, 100], 4, 4, 1),
+    ([65], [90], 7, 1, 32),
+    ([130, 9], [40, 512], 2, 1, 1),
+    ([300], [0], 2, 2, 1),
+    ([129], [77], 3, 1, 33),
+    ([260, 70], [511, 0], 4, 4, 0),
+]
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("lens,cached,Hq,Hkv,mask_block", SHAPES)
+def test_against_the_formula(dev, lens, cached, Hq, Hkv, mask_block, bits):
+    b = Batch(dev, lens, cached, Hq, Hkv, bits, seed=len(lens) + sum(lens) + sum(cached))
+    b.verify(b.run(mask_block), mask_block)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_one_token_of_a_long_cache_is_split(dev, bits):
+    shape = _capi.chunk_launch_shape(1, 1, 9000, 7, 1, 128)
+    assert shape["n_split"] > 8
+    b = Batch(dev, [1], [9000], 7, 1, bits, seed=3)
+    b.verify(b.run(1), 1)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_ragged_batch_whose_short_sequences_leave_splits_empty(dev, bits):
+    b = Batch(dev, [1, 1, 2], [3000, 0, 40], 4, 2, bits, seed=4)
+    b.verify(b.run(1), 1)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_large_scores(dev, bits):
+    """Scores of hundreds: the maximum moves, most probabilities vanish."""
+    b = Batch(dev, [40, 1], [300, 600], 2, 1, bits, seed=5, kv_scale=4.0)
+    b.verify(b.run(1, scale=0.5), 1, scale=0.5)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("L", [5, 40, 140])
+def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L):
+    b = Batch(dev, [L], [70], 2, 2, bits, seed=6)
+    b.v[L - 1, 0, 3] = float("nan")
+    b.v[L - 2, 1, 9] = float("inf")
+    b.k[L - 1, 1, 0] = float("nan")
+    b.k[L - 2, 0, :] = float("inf")
+    out = b.run(1)
+    ref_rows = slice(0, L - 2)
+    assert torch.isfinite(out[ref_rows]).all()
+    x = [_np(t) for t in (b.q, b.k, b.v)]
+    ref, spread, reach = chunk.attend(*x, b.cache_rows(b.kc, 0), b.cache_rows(b.vc, 0), SCALE, 1)
+    check(out[ref_rows], ref[ref_rows], spread[ref_rows], reach[ref_rows], L + 70)
+    o = _np(out).reshape(ref.shape)
+    assert np.isnan(o[L - 1]).all(axis=-1)[1]          # a NaN score
+    assert o[L - 2, 1, 9] == np.inf and np.isnan(o[L - 1, 1, 9])
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_stale_rows_behind_the_cached_length(dev, bits):
+    """The rest of the last page holds NaN: it takes no part."""
+    b = Batch(dev, [1, 20], [40, 300], 2, 2, bits, seed=7)
+    want = [b.run(m) for m in (0, 1)]
+    for s, c in enumerate(b.cached):
+        page, row = b.tables[s][-1], c % 256
+        for t in (b.kc, b.vc):
+            if bits == 8:
+                t[page, :, row * 128:256 * 128] = 0x7F
+                t[page, :, 256 * 128 + row:] = 255
+            else:
+                t[page, row:] = float("nan")
+    assert all(torch.equal(b.run(m), w) for m, w in zip((0, 1), want))
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_pages_outside_the_cache_are_left_out(dev, bits):
+    b = Batch(dev, [3, 1], [600, 520], 2, 1, bits, seed=8)
+    plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
+    # a table that lost a page after the plan was made, as a runner's bug would
+    t = plan.block_tables.view(2, plan.max_pages)
+    t[0, 1] = -1
+    t[1, 0] = b.pages
+    t[1, 2] = 2**31 - 1
+    out = chunk_attention(b.q.to(dev), b.k.to(dev), b.v.to(dev), b.kc, b.vc, plan, SCALE)
+    keep = [np.ones(600, bool), np.zeros(520, bool)]
+    keep[0][256:512] = False
+    keep[1][256:512] = True
+    b.verify(out, 1, keep=keep)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_empty_cache_and_no_sequences(dev, bits):
+    b = Batch(dev, [5, 33], [0, 0], 2, 2, bits, seed=9, spare=0)
+    assert b.kc.shape[0] == 0
+    b.verify(b.run(1), 1)
+    b = Batch(dev, [], [], 2, 2, bits, seed=9)
+    assert b.run(1).shape == (0, 256)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_layouts(dev, bits):
+    """Column slices of one fused projection, two- and three-dimensional."""
+    b = Batch(dev, [9, 50], [100, 3], 4, 2, bits, seed=10)
+    want = b.run(1)
+    fused = torch.cat([b.q.flatten(1), b.k.flatten(1), b.v.flatten(1), torch.zeros(59, 8, dtype=BF16)], 1).to(dev)
+    q, k, v = fused[:, :512], fused[:, 512:768], fused[:, 768:1024]
+    plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
+    assert torch.equal(chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE), want)
+    assert torch.equal(chunk_attention(q.view(59, 4, 128), k.view(59, 2, 128), v, b.kc, b.vc, plan, SCALE), want)
+
+
+def test_rows_outside_the_segments_stay(dev):
+    """The C entry point writes the segments' rows only."""
+    b = Batch(dev, [3, 4], [10, 300], 2, 2, 8, seed=11)
+    plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
+    o = torch.full((9, 256), 3.0, dtype=BF16, device=dev)
+    ws = torch.empty(max(1, _capi.chunk_workspace_size(2, 4, 300, 2, 2, 128)), dtype=torch.uint8, device=dev)
+    q, k, v = (torch.cat([t, t[:2]]).to(dev) for t in (b.q, b.k, b.v))
+    cu, lens, tables = plan._args
+    _capi.attn_chunk_paged_fwd_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, None, 2, 4, 300,
+                                   b.kc.data_ptr(), b.vc.data_ptr(), _capi.CACHE_FP8, b.pages, tables, plan.max_pages,
+                                   lens, 1, 2, 2, 128, 256, 256, 256, 256, SCALE, ws.data_ptr(), ws.numel(),
+                                   _capi._stream(dev))
+    assert (o[7:] == 3).all()
+    b.verify(o[:7], 1)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("lens,cached", [([1, 1], [700, 40]), ([32, 8], [300, 0]), ([150], [600])])
+def test_slot_lists(dev, bits, lens, cached):
+    """The slot-list form over rows in any order, some of them outside the cache, and a
+    subset of a packed batch by segment ids."""
+    b = Batch(dev, lens, cached, 4, 2, bits, seed=12)
+    g = torch.Generator().manual_seed(1)
+    rows = b.pages * 256
+    ids = list(range(len(lens)))[::-1]
+    lists = {}
+    for i in ids:
+        s = torch.randperm(rows, generator=g)[:cached[i]].to(torch.int64)
+        if cached[i] > 20:
+            s[7], s[cached[i] - 1] = -1, rows
+        lists[i] = s
+    off = np.concatenate([[0], np.cumsum([cached[i] for i in ids])])
+    slots = torch.cat([lists[i] for i in ids] + [torch.zeros(1, dtype=torch.int64)]).to(torch.int32).to(dev)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device=dev)
+    seg, offs = torch.tensor(ids, dtype=torch.int32, device=dev), torch.tensor(off, dtype=torch.int32, device=dev)
+    q, k, v = b.q.to(dev), b.k.to(dev), b.v.to(dev)
+    o = torch.empty_like(q)
+    max_q, max_c = max(lens), max(cached)
+    ws = torch.empty(max(16, _capi.chunk_workspace_size(len(ids), max_q, max_c, 4, 2, 128)), dtype=torch.uint8, device=dev)
+    kind = _capi.CACHE_FP8 if bits == 8 else _capi.CACHE_BF16
+    _capi.attn_chunk_slots_fwd_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu.data_ptr(), seg.data_ptr(),
+                                   len(ids), max_q, max_c, b.kc.data_ptr(), b.vc.data_ptr(), kind, rows,
+                                   slots.data_ptr(), offs.data_ptr(), 0, 4, 2, 128, 512, 256, 256, 512, SCALE,
+                                   ws.data_ptr(), ws.numel(), _capi._stream(dev))
+    r0 = 0
+    for i, L in enumerate(lens):
+        s = lists[i].numpy()
+        s = s[(s >= 0) & (s < rows)]
+        if bits == 8:
+            kc, vc = quant.load(b.kc.cpu().numpy(), s), quant.load(b.vc.cpu().numpy(), s)
+        else:
+            kc, vc = _np(b.kc.view(-1, 2, 128))[s], _np(b.vc.view(-1, 2, 128))[s]
+        x = [_np(t[r0:r0 + L]) for t in (b.q, b.k, b.v)]
+        check(o[r0:r0 + L], *chunk.attend(*x, kc, vc, SCALE), L + cached[i], f"sequence {i}")
+        r0 += L
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_captured_graph_replays(dev, bits):
+    """Captured and replayed, with eager calls of the same plan between the replays."""
+    b = Batch(dev, [1, 1], [2500, 900], 7, 1, bits, seed=13)
+    plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
+    q, k, v = b.q.to(dev), b.k.to(dev), b.v.to(dev)
+    want = chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE))
+        graphs.append(gr)
+    for i in range(4):
+        outs[i % 2].zero_()
+        graphs[i % 2].replay()
+        assert torch.equal(chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE), want)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i % 2], want)
+    q2 = torch.flip(q, [0]).contiguous()
+    q.copy_(q2)
+    graphs[0].replay()
+    assert torch.equal(outs[0], chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE))
+
+
+def test_two_streams_at_once(dev):
+    b = Batch(dev, [1], [6000], 7, 1, 8, seed=14)
+    plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
+    q, k, v = b.q.to(dev), b.k.to(dev), b.v.to(dev)
+    want = chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for s, o in zip(streams, outs):
+            with torch.cuda.stream(s):
+                o.append(chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for o in outs for x in o)
+
+
+def test_same_inputs_same_bits(dev):
+    b = Batch(dev, [1, 30, 200], [4000, 600, 90], 4, 2, 8, seed=15)
+    first = b.run(1)
+    assert all(torch.equal(b.run(1), first) for _ in range(3))
+
+
+@pytest.mark.parametrize("mask_block", [1, 8])
+def test_a_prompt_in_chunks_is_the_prompt_at_once(dev, mask_block):
+    """Prefill in chunks, each stored (8-bit) and attended over the pages, then single tokens:
+    every step against the formula over the rows as the cache holds them."""
+    Hq, Hkv, D, total = 4, 2, 128, 330
+    g = torch.Generator().manual_seed(16)
+    q, k, v = (torch.randn(total, h, D, generator=g).to(BF16) for h in (Hq, Hkv, Hkv))
+    kc, vc = quantized_pages(3, Hkv, device=dev), quantized_pages(3, Hkv, device=dev)
+    table, at = [2, 0], 0
+    for L in (96, 120, 104, 1, 8, 1):
+        x = [t[at:at + L].to(dev) for t in (q, k, v)]
+        plan = ChunkPlan([L], [at], [table], dev, mask_block=mask_block)
+        pos = torch.arange(at, at + L)
+        slots = (torch.tensor(table)[pos // 256] * 256 + pos % 256).to(torch.int32).to(dev)
+        store_kvcache(x[1], x[2], kc, vc, slots)
+        out = chunk_attention(*x, kc, vc, plan, SCALE)
+        held = [_np(t[:at]) for t in (k, v)]
+        held = [quant.dequantise(*quant.quantise(t)) if at else t for t in held]
+        ref = chunk.attend(*[_np(t[at:at + L]) for t in (q, k, v)], *held, SCALE, mask_block)
+        check(out, *ref, at + L, f"chunk at {at}")
+        at += L
+    ko, vo = torch.empty(at, Hkv, D, dtype=BF16, device=dev), torch.empty(at, Hkv, D, dtype=BF16, device=dev)
+    pos = torch.arange(at)
+    load_kvcache(ko, vo, kc, vc, (torch.tensor(table)[pos // 256] * 256 + pos % 256).to(torch.int32).to(dev))
+    assert np.array_equal(_np(ko), quant.dequantise(*quant.quantise(_np(k[:at]))))
+    assert np.array_equal(_np(vo), quant.dequantise(*quant.quantise(_np(v[:at]))))
