@@ -14,7 +14,10 @@
 //     four wavefronts takes 32-key tiles of its own; K goes from memory straight
 //     into MFMA operands, V through the wavefront's own LDS for the transposition.
 //     No wavefront waits for another until the states are merged at the end.
-//   * long caches are split over workgroups; chunk_combine_kernel joins the parts.
+//   * chunk_tile_kernel (many M rows: pieces of prompts): 64-key tiles of K and V in LDS,
+//     in bf16, shared by the workgroup's wavefronts of 32 M rows each; 8-bit rows are
+//     converted once, on their way into LDS.
+//   * long key ranges are split over workgroups; chunk_combine_kernel joins the parts.
 #include "attn_tile.h"
 #include "quant.h"
 
@@ -39,6 +42,8 @@ struct ChunkArgs {
   int max_pages, max_q, max_cached;
   int n_seg, Hkv, g, mtiles, n_split, tiles_per_split;
   int mask_block;
+  int bm;                 // M rows of a workgroup
+  int tile_form;          // chunk_tile_kernel (else chunk_rows_kernel)
   int logical_blocks, xcd_chunk;
   float scale_log2;
 };
@@ -77,11 +82,20 @@ __device__ __forceinline__ int visible(const Segment& g, int t, int mask_block) 
   return (int)min((int64_t)g.len, end);
 }
 
-// Splits of a segment's cached tiles that hold any (at least one: the new rows
-// belong to the last).
-__device__ __forceinline__ int splits_of(int cached, int tiles_per_split) {
-  const int tiles = (cached + kTileKeys - 1) / kTileKeys;
-  return max(1, (tiles + tiles_per_split - 1) / tiles_per_split);
+constexpr int kBigTile = 64;    // keys of chunk_tile_kernel's tiles
+
+// Splits that hold keys of M tile mt (at least one).  chunk_rows_kernel deals the
+// cached tiles alone, the new rows belonging to the last split; chunk_tile_kernel
+// the cached tiles and those of the new rows that the M tile sees.
+__device__ __forceinline__ int splits_of(const ChunkArgs& a, const Segment& g, int mt) {
+  int tiles;
+  if (a.tile_form) {
+    const int last = min((mt + 1) * a.bm, g.len * a.g) - 1;
+    tiles = (g.cached + kBigTile - 1) / kBigTile + (visible(g, last / a.g, a.mask_block) + kBigTile - 1) / kBigTile;
+  } else {
+    tiles = (g.cached + kTileKeys - 1) / kTileKeys;
+  }
+  return max(1, (tiles + a.tiles_per_split - 1) / a.tiles_per_split);
 }
 
 __device__ __forceinline__ float row_max4(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -214,8 +228,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int g = a.g;
   const int M = sg.len * g;
   const int m_base = mt * BM;
-  const int ns = splits_of(sg.cached, a.tiles_per_split);
-  if (m_base >= M || split >= ns) return;
+  if (m_base >= M) return;
+  const int ns = splits_of(a, sg, mt);
+  if (split >= ns) return;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
@@ -556,9 +571,295 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many M rows: NW wavefronts of 32 M rows share 64-key tiles of K and V in LDS
+// (bf16, the swizzled layout of attn_tile.h), two stages.  The tile sequence is the
+// cached rows' tiles, then those of the new rows.  While tile t is computed, tile t + 1
+// is on its way: bf16 rows by DMA into the other stage; 8-bit rows into registers
+// (16 bytes a thread and matrix with eight wavefronts), converted and written to the
+// other stage after the products -- once per workgroup, not once per wavefront.
+template <int NW, bool FP8>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_tile_kernel(ChunkArgs a) {
+  constexpr int TK = kBigTile;
+  constexpr int STAGE = 2 * TK * 256;
+  constexpr int BM = 32 * NW;
+  constexpr int DMA = TK * 256 / 1024 / NW;  // DMA instructions of one matrix, tile and wavefront
+  constexpr int PER = TK * 8 / (64 * NW);    // 8-bit rows: 16-byte pieces of one matrix and thread
+  extern __shared__ __attribute__((aligned(16))) float lds_f[];
+  uint8_t* const lds = reinterpret_cast<uint8_t*>(lds_f);
+  const int L = xcd_remap(blockIdx.x, a.xcd_chunk);
+  if (L >= a.logical_blocks) return;
+  int r = L;
+  // the last M tiles first: with a causal mask they see the most keys
+  const int mt = a.mtiles - 1 - r % a.mtiles;
+  r /= a.mtiles;
+  const int split = r % a.n_split;
+  r /= a.n_split;
+  const int hkv = r % a.Hkv;
+  const int s = r / a.Hkv;
+  const Segment sg = segment<true>(a, s);
+  const int g = a.g;
+  const int M = sg.len * g;
+  const int m_base = mt * BM;
+  if (m_base >= M) return;
+  const int ns = splits_of(a, sg, mt);
+  if (split >= ns) return;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int lrow = lane & 31, hl = lane >> 5;
+  const int rl = lane >> 4, P = lane & 15;
+
+  const int t_cached = (sg.cached + TK - 1) / TK;
+  const int see_last = visible(sg, (min(m_base + BM, M) - 1) / g, a.mask_block);
+  const int see_first = visible(sg, m_base / g, a.mask_block);
+  const int t_all = t_cached + (see_last + TK - 1) / TK;
+  const int t0 = split * a.tiles_per_split, t1 = min(t_all, t0 + a.tiles_per_split);
+  const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
+  const int32_t* const table = a.table + (int64_t)s * a.max_pages;
+  const uint32_t bf_row = (uint32_t)(a.Hkv * HD * 2);
+  const uint32_t kS = (uint32_t)(a.k_stride * 2), vS = (uint32_t)(a.v_stride * 2);
+  const uint16_t* const knew = a.k + (int64_t)sg.row0 * a.k_stride + hkv * HD;
+  const uint16_t* const vnew = a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD;
+
+  // page of cached tile t, or -1 (then its rows are left out)
+  auto page_of = [&](int t) -> int {
+    const int pg = t * TK / kPageRows;
+    if (n_pages == 0 || pg >= a.max_pages) return -1;
+    const int pid = table[pg];
+    return (uint32_t)pid < n_pages ? pid : -1;
+  };
+  // `rows` rows (none: zeros) of kb / vb with strides kr / vr to a stage
+  auto dma_rows = [&](uint8_t* stage, const void* kb, const void* vb, int rows, uint32_t kr, uint32_t vr) {
+    const __amdgpu_buffer_rsrc_t krs = make_rsrc(kb, rows > 0 ? (uint32_t)(rows - 1) * kr + HD * 2 : 0u);
+    const __amdgpu_buffer_rsrc_t vrs = make_rsrc(vb, rows > 0 ? (uint32_t)(rows - 1) * vr + HD * 2 : 0u);
+#pragma unroll
+    for (int j = 0; j < DMA; ++j) {
+      const int q = DMA * wave + j;
+      const uint32_t row = (uint32_t)(4 * q + rl);
+      dma16(krs, stage + q * 1024, row * kr + (uint32_t)((P ^ ((4 * q + rl) & 15)) * 16));
+      dma16(vrs, stage + TK * 256 + q * 1024, row * vr + (uint32_t)((P ^ (4 * rl)) * 16));
+    }
+  };
+  u32x4_t kx[PER], vx[PER];
+  uint32_t ksc[PER], vsc[PER];
+  // Tile t on its way to `stage`; true where it goes through registers.
+  auto issue = [&](uint8_t* stage, int t) -> bool {
+    if (t >= t_cached) {
+      const int j0 = (t - t_cached) * TK;
+      dma_rows(stage, knew + (int64_t)j0 * a.k_stride, vnew + (int64_t)j0 * a.v_stride, sg.len - j0, kS, vS);
+      return false;
+    }
+    const int pid = page_of(t);
+    const int row0 = t * TK & (kPageRows - 1);
+    const int rows = pid < 0 ? 0 : min(sg.cached - t * TK, TK);
+    if constexpr (FP8) {
+      const int64_t rec = ((int64_t)max(pid, 0) * a.Hkv + hkv) * kRecord;
+      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
+      const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.vc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int piece = i * 64 * NW + tid, row = piece >> 3;
+        kx[i] = bload(krs, (uint32_t)piece * 16u, 0u);
+        vx[i] = bload(vrs, (uint32_t)piece * 16u, 0u);
+        ksc[i] = vsc[i] = 127u;
+        if (row < rows) {
+          ksc[i] = a.kc[rec + kScaleOff + row0 + row];
+          vsc[i] = a.vc[rec + kScaleOff + row0 + row];
+        }
+      }
+      return true;
+    } else {
+      const int64_t off = ((int64_t)max(pid, 0) * kPageRows + row0) * bf_row + hkv * HD * 2;
+      dma_rows(stage, a.kc + off, a.vc + off, rows, bf_row, bf_row);
+      return false;
+    }
+  };
+  auto put = [&](uint8_t* stage) {
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int piece = i * 64 * NW + tid, row = piece >> 3, ch = (piece & 7) * 2;
+        const float ks = scale_of(ksc[i]), vs = scale_of(vsc[i]);
+        uint8_t* const kr = stage + row * 256;
+        uint8_t* const vr = stage + TK * 256 + row * 256;
+        st128(kr + ((ch ^ (row & 15)) * 16), dequant8(u32x2_t{kx[i][0], kx[i][1]}, ks));
+        st128(kr + (((ch + 1) ^ (row & 15)) * 16), dequant8(u32x2_t{kx[i][2], kx[i][3]}, ks));
+        st128(vr + ((ch ^ (4 * (row & 3))) * 16), dequant8(u32x2_t{vx[i][0], vx[i][1]}, vs));
+        st128(vr + (((ch + 1) ^ (4 * (row & 3))) * 16), dequant8(u32x2_t{vx[i][2], vx[i][3]}, vs));
+      }
+    }
+  };
+
+  bf16x8_t qf[1][8];
+  const int m_lane = m_base + wave * 32 + lrow;
+  const int lim = visible(sg, min(m_lane / g, sg.len - 1), a.mask_block);
+  {
+    const uint32_t qS = (uint32_t)(a.q_stride * 2);
+    const uint32_t qbytes = (uint32_t)sg.len * qS;
+    const __amdgpu_buffer_rsrc_t qrs = make_rsrc(a.q + (int64_t)sg.row0 * a.q_stride, qbytes);
+    const int tok = m_lane / g;
+    const bool ok = m_lane < M;
+    const uint32_t qoff = (uint32_t)tok * qS + (uint32_t)((hkv * g + m_lane - tok * g) * HD + hl * 8) * 2u;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) qf[0][kk] = as_bf16x8(bload(qrs, ok ? qoff + (uint32_t)kk * 32u : qbytes, 0u));
+  }
+  // of this wavefront's rows: the least and the most that any sees
+  const int lim_lo = __builtin_amdgcn_readfirstlane(visible(sg, min((m_base + wave * 32) / g, sg.len - 1), a.mask_block));
+  const int lim_hi =
+      __builtin_amdgcn_readfirstlane(visible(sg, (min(m_base + wave * 32 + 32, M) - 1) / g, a.mask_block));
+  const bool live = m_base + wave * 32 < M;
+
+  DenseAddr ad;
+  dense_addr(ad, lane, 0u, 0u);
+  DenseState<1> st;
+  dense_state_init(st);
+  const float c = a.scale_log2;
+
+  if (t0 < t1) {
+    if (issue(lds, t0)) put(lds);
+    vm_wait<0>();
+    __syncthreads();
+  }
+  for (int t = t0; t < t1; ++t) {
+    uint8_t* const cur = lds + ((t - t0) & 1) * STAGE;
+    uint8_t* const nxt = lds + ((t - t0 + 1) & 1) * STAGE;
+    const bool more = t + 1 < t1;
+    const bool regs = more && issue(nxt, t + 1);
+    // keys of the tile that this lane's row sees, the least of the wavefront's rows, and the most
+    int valid, lo, hi;
+    bool fix = false;
+    if (t < t_cached) {
+      valid = lo = hi = page_of(t) < 0 ? 0 : min(sg.cached - t * TK, TK);
+    } else {
+      const int j0 = (t - t_cached) * TK;
+      valid = lim - j0;
+      lo = lim_lo - j0;
+      hi = lim_hi - j0;
+      if (see_first - j0 < TK && see_first < sg.len) {
+        // Some M row of the workgroup does not see all of the tile: a NaN or infinity in V
+        // would reach it as 0 * V.  Every wavefront looks through the whole tile, so all agree;
+        // such elements are multiplied as zeros and added below to the rows that see them.
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < TK * 256 / 1024; ++i)
+          odd |= has_nonfinite(*reinterpret_cast<const u32x4_t*>(cur + TK * 256 + i * 1024 + lane * 16));
+        fix = __builtin_amdgcn_ballot_w64(odd) != 0;
+        if (fix) {
+          __syncthreads();
+#pragma unroll 1
+          for (int i = wave; i < TK * 256 / 1024; i += NW) {
+            u32x4_t* const p = reinterpret_cast<u32x4_t*>(cur + TK * 256 + i * 1024 + lane * 16);
+            *p = finite_part(*p);
+          }
+          __syncthreads();
+        }
+      }
+    }
+    if (live && hi > 0) {
+      f32x16_t sacc[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[b][i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const bf16x8_t af =
+              as_bf16x8(*reinterpret_cast<const u32x4_t*>(cur + b * 32 * 256 + (ad.kbase ^ (uint32_t)(32 * kk))));
+          sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, qf[0][kk], sacc[b], 0, 0, 0);
+        }
+      if (lo < TK) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (b * 32 + 8 * (i >> 2) + 4 * hl + (i & 3) >= valid) sacc[b][i] = -INFINITY;
+      }
+      bf16x8_t pf[4];
+      dense_softmax<2, false>(sacc, st.oacc[0], st.m_run[0], st.l_run[0], st.thr[0], st.neg_m[0], pf, c, TK, 0, hl);
+#pragma unroll
+      for (int cch = 0; cch < 4; ++cch)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          const uint8_t* vp = cur + TK * 256 + (ad.vbase ^ (uint32_t)(64 * db)) + cch * 16 * 256;
+          const u32x2_t x0 = ds_read_tr16(vp), x1 = ds_read_tr16(vp + 8 * 256);
+          st.oacc[0][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(u32x4_t{x0[0], x0[1], x1[0], x1[1]}),
+                                                                   pf[cch], st.oacc[0][db], 0, 0, 0);
+        }
+      if (fix) {
+        const int j0 = (t - t_cached) * TK, end = min(j0 + TK, sg.len);
+#pragma unroll 1
+        for (int j = j0; j < end; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * hl;
+            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vnew + (int64_t)j * a.v_stride + d);
+            if (j < lim) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+                if ((h & 0x7f80u) == 0x7f80u) st.oacc[0][i >> 2][4 * (i & 3) + e] += bf16_bits_to_f32(h);
+              }
+            }
+          }
+      }
+    }
+    if (regs) put(nxt);
+    if (more) {
+      vm_wait<0>();
+      __syncthreads();
+    }
+  }
+
+  const float l_tot = pair_sum32(st.l_run[0]);
+  if (ns > 1) {
+    if (m_lane < M) {
+      const int64_t rec = ((((int64_t)s * a.Hkv + hkv) * a.mtiles + mt) * a.n_split + split) * BM + wave * 32 + lrow;
+      float* const po = a.ws + rec * HD;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * hl;
+        *reinterpret_cast<f32x4_t*>(po + d) =
+            f32x4_t{st.oacc[0][i >> 2][4 * (i & 3)], st.oacc[0][i >> 2][4 * (i & 3) + 1],
+                    st.oacc[0][i >> 2][4 * (i & 3) + 2], st.oacc[0][i >> 2][4 * (i & 3) + 3]};
+      }
+      if (hl == 0) {
+        float* const pml = a.ws + (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * BM * HD + rec * 2;
+        pml[0] = st.m_run[0];
+        pml[1] = l_tot;
+      }
+    }
+    return;
+  }
+  const float inv = l_tot != 0.f ? 1.f / l_tot : 0.f;
+  __syncthreads();  // every wavefront is done with the stages
+  uint8_t* const ot = lds + wave * 8192;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      const u32x2_t w = {cvt_pk_bf16(st.oacc[0][db][4 * rq] * inv, st.oacc[0][db][4 * rq + 1] * inv),
+                         cvt_pk_bf16(st.oacc[0][db][4 * rq + 2] * inv, st.oacc[0][db][4 * rq + 3] * inv)};
+      *reinterpret_cast<u32x2_t*>(ot + lrow * 256 + (((4 * db + rq) ^ (lrow & 15)) * 16) + 8 * hl) = w;
+    }
+  wave_lds_fence();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int row = 4 * j + rl, m = m_base + wave * 32 + row;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(ot + row * 256 + ((P ^ (row & 15)) * 16));
+    if (m < M) {
+      const int tok = m / g;
+      st128(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + (hkv * g + m - tok * g) * HD + P * 8, v);
+    }
+  }
+}
+
 // Joins the parts of every (segment, KV head, M row) whose keys were split: a
 // workgroup holds eight rows, 32 threads of four d each.
-__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, int bm, bool paged) {
+__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, bool paged) {
+  const int bm = a.bm;
   const int64_t idx = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int d0 = (threadIdx.x & 31) * 4;
   const int per = a.mtiles * bm;
@@ -568,8 +869,9 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, int bm,
   const int hkv = pair % a.Hkv;
   const int s = pair / a.Hkv;
   const Segment sg = paged ? segment<true>(a, s) : segment<false>(a, s);
-  const int ns = splits_of(sg.cached, a.tiles_per_split);
-  if (ns == 1 || mrow >= sg.len * a.g) return;
+  if (mrow >= sg.len * a.g) return;
+  const int ns = splits_of(a, sg, mrow / bm);
+  if (ns == 1) return;
   const int64_t recs = (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * bm;
   const int64_t rec0 = (((int64_t)s * a.Hkv + hkv) * a.mtiles + mrow / bm) * a.n_split * bm + mrow % bm;
   const float* const ml = a.ws + recs * HD;
@@ -597,30 +899,41 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, int bm,
 
 // ---- launch plan ---------------------------------------------------------------------
 struct ChunkPlan {
-  int nb;                        // 16-row blocks of a workgroup
-  int mtiles;
-  int n_split, tiles_per_split;  // workgroups along the cached keys
+  bool tile_form;
+  int nw;                        // chunk_tile_kernel: wavefronts
+  int nb;                        // chunk_rows_kernel: 16-row blocks
+  int bm, mtiles;                // M rows of a workgroup, M tiles
+  int n_split, tiles_per_split;  // workgroups along the keys
 };
-static ChunkPlan chunk_plan(int n_seg, int max_q, int max_cached, int Hq, int Hkv) {
+static ChunkPlan chunk_plan(bool paged, int n_seg, int max_q, int max_cached, int Hq, int Hkv) {
   ChunkPlan p = {};
   const int64_t rows = (int64_t)max_q * (Hq / Hkv);
-  p.nb = rows <= 16 ? 1 : 2;
-  p.mtiles = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
-  const int64_t groups = (int64_t)n_seg * Hkv * p.mtiles;
-  const int tiles = (max_cached + kTileKeys - 1) / kTileKeys;
+  const int64_t pairs = (int64_t)n_seg * Hkv;
+  p.tile_form = paged && rows > 64;
+  if (p.tile_form) {
+    p.nw = pairs * ((rows + 255) / 256) >= 256 ? 8 : 4;
+    p.bm = 32 * p.nw;
+  } else {
+    p.nb = rows <= 16 ? 1 : 2;
+    p.bm = 16 * p.nb;
+  }
+  p.mtiles = (int)((rows + p.bm - 1) / p.bm);
+  const int64_t groups = pairs * p.mtiles;
+  const int64_t key = p.tile_form ? kBigTile : kTileKeys;
+  const int64_t tiles = (max_cached + key - 1) / key + (p.tile_form ? (max_q + key - 1) / key : 0);
+  const int64_t least = 8;  // tiles of a split
   int64_t want = groups > 0 ? 512 / groups : 1;
-  const int most = (tiles + 7) / 8;  // at least two tiles a wavefront
-  if (want > most) want = most;
+  if (want > (tiles + least - 1) / least) want = (tiles + least - 1) / least;
   if (want < 1) want = 1;
-  int tps = (int)((tiles + want - 1) / want);
-  tps = (tps + 3) / 4 * 4;
-  p.tiles_per_split = tps > 0 ? tps : 4;
-  p.n_split = tiles > 0 ? (tiles + p.tiles_per_split - 1) / p.tiles_per_split : 1;
+  int64_t tps = (tiles + want - 1) / want;
+  if (!p.tile_form) tps = (tps + 3) / 4 * 4;
+  p.tiles_per_split = tps > 0 ? (int)tps : 4;
+  p.n_split = tiles > 0 ? (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
   return p;
 }
 static size_t chunk_ws(const ChunkPlan& p, int n_seg, int Hkv) {
   if (p.n_split <= 1) return 0;
-  return (size_t)n_seg * Hkv * p.mtiles * p.n_split * 16 * p.nb * (HD + 2) * sizeof(float);
+  return (size_t)n_seg * Hkv * p.mtiles * p.n_split * p.bm * (HD + 2) * sizeof(float);
 }
 
 }  // namespace dllm
@@ -634,16 +947,19 @@ static bool chunk_sizes_ok(int n_seg, int max_q, int max_cached, int Hq, int Hkv
 
 extern "C" size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D) {
   if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D) || n_seg == 0 || max_q == 0) return 0;
-  return chunk_ws(chunk_plan(n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
+  // the larger of the two entry points' needs
+  const size_t paged = chunk_ws(chunk_plan(true, n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
+  const size_t slots = chunk_ws(chunk_plan(false, n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
+  return paged > slots ? paged : slots;
 }
 
 extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D, int* rows,
                                             int* n_split, int* grid) {
   if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
     return fail(DLLM_ERR_INVALID_ARG, "dllm_attn_chunk_launch_shape: unsupported sizes");
-  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
+  const ChunkPlan p = chunk_plan(true, n_seg, max_q, max_cached, Hq, Hkv);
   const bool none = n_seg == 0 || max_q == 0;
-  if (rows) *rows = 16 * p.nb;
+  if (rows) *rows = p.bm;
   if (n_split) *n_split = p.n_split;
   if (grid) {
     const int64_t logical = (int64_t)n_seg * Hkv * p.mtiles * p.n_split;
@@ -699,7 +1015,8 @@ static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dll
   a.n_seg = n_seg; a.Hkv = Hkv; a.g = Hq / Hkv;
   a.mask_block = mask_block;
   a.scale_log2 = softmax_scale * kLog2e;
-  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
+  const ChunkPlan p = chunk_plan(paged, n_seg, max_q, max_cached, Hq, Hkv);
+  a.bm = p.bm; a.tile_form = p.tile_form;
   a.mtiles = p.mtiles; a.n_split = p.n_split; a.tiles_per_split = p.tiles_per_split;
   const size_t need = chunk_ws(p, n_seg, Hkv);
   if (need) {
@@ -717,18 +1034,31 @@ static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dll
   const int64_t grain = 8 * (int64_t)a.xcd_chunk;
   const unsigned grid = (unsigned)((logical + grain - 1) / grain * grain);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  auto pick = [&](auto nb) {
-    constexpr int NB = decltype(nb)::value;
-    return cache_type == DLLM_CACHE_FP8 ? (paged ? chunk_rows_kernel<NB, true, true> : chunk_rows_kernel<NB, true, false>)
-                                        : (paged ? chunk_rows_kernel<NB, false, true> : chunk_rows_kernel<NB, false, false>);
+  const bool fp8 = cache_type == DLLM_CACHE_FP8;
+  auto launch = [&](auto kern, int threads, int lds_bytes) -> int {
+    int e = set_lds(kern, lds_bytes, name);
+    if (e) return e;
+    kern<<<dim3(grid), dim3(threads), lds_bytes, st>>>(a);
+    return check_launch(name);
   };
-  auto kern = p.nb == 1 ? pick(std::integral_constant<int, 1>()) : pick(std::integral_constant<int, 2>());
-  if ((rc = set_lds(kern, rows_lds(p.nb), name))) return rc;
-  kern<<<dim3(grid), dim3(256), rows_lds(p.nb), st>>>(a);
-  if ((rc = check_launch(name))) return rc;
+  auto rows_form = [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    return fp8 ? (paged ? chunk_rows_kernel<NB, true, true> : chunk_rows_kernel<NB, true, false>)
+               : (paged ? chunk_rows_kernel<NB, false, true> : chunk_rows_kernel<NB, false, false>);
+  };
+  constexpr int kTileLds = 2 * 2 * kBigTile * 256;
+  if (p.tile_form && p.nw == 8)
+    rc = launch(fp8 ? chunk_tile_kernel<8, true> : chunk_tile_kernel<8, false>, 512, kTileLds);
+  else if (p.tile_form)
+    rc = launch(fp8 ? chunk_tile_kernel<4, true> : chunk_tile_kernel<4, false>, 256, kTileLds);
+  else if (p.nb == 1)
+    rc = launch(rows_form(std::integral_constant<int, 1>()), 256, rows_lds(1));
+  else
+    rc = launch(rows_form(std::integral_constant<int, 2>()), 256, rows_lds(2));
+  if (rc) return rc;
   if (p.n_split > 1) {
-    const int64_t rows = (int64_t)n_seg * Hkv * p.mtiles * 16 * p.nb;
-    chunk_combine_kernel<<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a, 16 * p.nb, paged);
+    const int64_t rows = (int64_t)n_seg * Hkv * p.mtiles * p.bm;
+    chunk_combine_kernel<<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a, paged);
     rc = check_launch(name);
   }
   return rc;

@@ -102,6 +102,8 @@ SHAPES = [
     ([300], [0], 2, 2, 1),
     ([129], [77], 3, 1, 33),
     ([260, 70], [511, 0], 4, 4, 0),
+    ([100, 20], [1500, 0], 2, 1, 1),   # many rows, keys split, a short sequence beside a long one
+    ([520], [700], 2, 1, 16),          # the new rows' own tiles are split as well
 ]
 
 
