@@ -50,6 +50,7 @@ struct ChunkArgs {
 
 constexpr int kTileKeys = 32;   // keys of a wavefront's tile
 constexpr int kVTile = kTileKeys * 256;
+constexpr int kMaxSplitTiles = 62 * kPageRows / kTileKeys;  // chunk_rows_kernel: at most 63 pages, one a lane
 
 // Segment s: new rows' first row and count, cached rows.
 struct Segment {
@@ -264,6 +265,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int t_end = n_rows ? min(tiles, t_begin + a.tiles_per_split) : t_begin;  // no cache: nothing to read
   const int32_t* const table = PAGED ? a.table + (int64_t)s * a.max_pages : a.table + sg.slot0;
   const int64_t bf_row = (int64_t)a.Hkv * HD * 2;
+  // Page ids of the split, one a lane (a split spans at most 63): a tile's
+  // loads then wait for no load of their own.
+  const int pg0 = t_begin * kTileKeys / kPageRows;
+  const int page_reg = PAGED && t_begin < t_end ? table[min(pg0 + lane, a.max_pages - 1)] : -1;
 
   // Loads of cached tile t.  Rows that do not exist (past the cached length, of a
   // page or slot outside the cache) read row 0 of the cache or nothing, and are in `bad`.
@@ -273,7 +278,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     uint32_t bad = left >= 32 ? 0u : ~0u << left;
     if constexpr (PAGED) {
       const int pg = key0 >> 8;
-      int pid = pg < a.max_pages ? table[pg] : -1;
+      int pid = pg < a.max_pages ? __builtin_amdgcn_readlane(page_reg, (pg - pg0) & 63) : -1;
       const bool in = (uint32_t)pid < (n_rows >> 8);
       pid = in ? pid : 0;
       if (!in) bad = ~0u;
@@ -335,21 +340,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int trow = 4 * g4 + (col >> 2);
   const uint32_t vbase = (uint32_t)(trow * 256 + ((((col & 3) >> 1) ^ (2 * (trow & 7))) * 16) + 8 * (col & 1));
 
-  // K fragments kf[u][step] of the tile, V in LDS: both products and the softmax.
-  auto products = [&](const bf16x8_t (&kf)[2][4], auto&& hide) {
+  // K fragments of key half u from keys(u, .), V in LDS: both products and the softmax.
+  auto products = [&](auto&& keys, auto&& hide) {
+    f32x4_t sc[NB][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      bf16x8_t kf[4];
+      keys(u, kf);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        sc[b][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4)
+          sc[b][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k4], qf[b][k4], sc[b][u], 0, 0, 0);
+      }
+    }
     bf16x8_t pf[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      f32x4_t sc[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        sc[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4)
-          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[u][k4], qf[b][k4], sc[u], 0, 0, 0);
-      }
-      hide(sc, b);
-      pf[b] = rows_softmax(sc, st.o[b], st.m[b], st.l[b], c);
+      hide(sc[b], b);
+      pf[b] = rows_softmax(sc[b], st.o[b], st.m[b], st.l[b], c);
     }
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
@@ -400,20 +410,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
       }
     wave_lds_fence();
-    bf16x8_t kf[2][4];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
+    const uint32_t bad = x.bad;
+    auto keys = [&](int u, bf16x8_t (&kf)[4]) {
 #pragma unroll
       for (int p = 0; p < TileRegs<FP8>::N; ++p) {
         if constexpr (FP8) {
-          kf[u][2 * p] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][0], x.k[u][p][1]}, ks[u]));
-          kf[u][2 * p + 1] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][2], x.k[u][p][3]}, ks[u]));
+          kf[2 * p] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][0], x.k[u][p][1]}, ks[u]));
+          kf[2 * p + 1] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][2], x.k[u][p][3]}, ks[u]));
         } else {
-          kf[u][p] = as_bf16x8(x.k[u][p]);
+          kf[p] = as_bf16x8(x.k[u][p]);
         }
       }
-    const uint32_t bad = x.bad;
-    products(kf, [&](f32x4_t (&sc)[2], int) {
+    };
+    products(keys, [&](f32x4_t (&sc)[2], int) {
       if (bad) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -451,7 +460,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int new_tiles = (see + kTileKeys - 1) / kTileKeys;
     const int turn = max(t_end - t_begin, 0);
     for (int t = (wave - turn) & 3; t < new_tiles; t += 4) {
-      bf16x8_t kf[2][4];
+      bf16x8_t kx[2][4];
       u32x4_t vx[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -459,7 +468,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
           const uint32_t off = FP8 ? (uint32_t)((k4 >> 1) * 128 + g4 * 32 + (k4 & 1) * 16) : (uint32_t)(k4 * 64 + g4 * 16);
-          kf[u][k4] = as_bf16x8(bload(krs, row < (uint32_t)sg.len ? row * kS + off : kb, 0u));
+          kx[u][k4] = as_bf16x8(bload(krs, row < (uint32_t)sg.len ? row * kS + off : kb, 0u));
           vx[u][k4] = bload(vrs, row < (uint32_t)sg.len ? row * vS + (uint32_t)(k4 * 64 + g4 * 16) : vb, 0u);
         }
       }
@@ -484,7 +493,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int p = 0; p < 4; ++p) put_v(16 * u + col, 4 * p + g4, vx[u][p]);
       wave_lds_fence();
-      products(kf, [&](f32x4_t (&sc)[2], int b) {
+      auto keys = [&](int u, bf16x8_t (&kf)[4]) {
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) kf[k4] = kx[u][k4];
+      };
+      products(keys, [&](f32x4_t (&sc)[2], int b) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -856,11 +869,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   }
 }
 
-// Joins the parts of every (segment, KV head, M row) whose keys were split: a
-// workgroup holds eight rows, 32 threads of four d each.
+// Joins the parts of every (segment, KV head, M row) whose keys were split.  G groups of
+// 32 threads (four d each) share a row's parts, each taking every G-th, so that a row
+// of many parts is one round of loads rather than a long chain (28 rows of 128 parts:
+// 39 us with one group, see the launch).
+template <int G>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, bool paged) {
+  constexpr int ROWS = 8 / G;
+  __shared__ f32x4_t part[G > 1 ? 256 : 1];
+  __shared__ float part_ml[G > 1 ? 16 : 1];
   const int bm = a.bm;
-  const int64_t idx = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int grp = threadIdx.x >> 5;
+  const int64_t idx = (int64_t)blockIdx.x * ROWS + grp / G;
+  const int sub = grp % G;
   const int d0 = (threadIdx.x & 31) * 4;
   const int per = a.mtiles * bm;
   const int pair = (int)(idx / per);  // (segment, KV head)
@@ -877,12 +898,12 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, bool pa
   const float* const ml = a.ws + recs * HD;
   float mx = -INFINITY;
 #pragma unroll 8
-  for (int p = 0; p < ns; ++p) mx = fmaxf(mx, ml[(rec0 + (int64_t)p * bm) * 2]);
+  for (int p = sub; p < ns; p += G) mx = fmaxf(mx, ml[(rec0 + (int64_t)p * bm) * 2]);
   const float mu = mx == -INFINITY ? 0.f : mx;
   float l = 0.f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int p = 0; p < ns; ++p) {
+  for (int p = sub; p < ns; p += G) {
     const int64_t rec = rec0 + (int64_t)p * bm;
     const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.ws + rec * HD + d0);
     const float mp = ml[rec * 2];
@@ -890,6 +911,29 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, bool pa
     l += ml[rec * 2 + 1] * w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
+  }
+  if constexpr (G > 1) {  // G = 8: the workgroup holds one row
+    part[threadIdx.x] = acc;
+    if ((threadIdx.x & 31) == 0) {
+      part_ml[2 * sub] = mx;
+      part_ml[2 * sub + 1] = l;
+    }
+    __syncthreads();
+    if (sub) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < G; ++i) top = fmaxf(top, part_ml[2 * i]);
+    const float tu = top == -INFINITY ? 0.f : top;
+    l = 0.f;
+    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float w = part_ml[2 * i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(part_ml[2 * i] - tu);
+      l += part_ml[2 * i + 1] * w;
+      const f32x4_t x = part[32 * i + (threadIdx.x & 31)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
+    }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int tok = mrow / a.g, head = hkv * a.g + (mrow - tok * a.g);
@@ -926,7 +970,7 @@ static ChunkPlan chunk_plan(bool paged, int n_seg, int max_q, int max_cached, in
   if (want > (tiles + least - 1) / least) want = (tiles + least - 1) / least;
   if (want < 1) want = 1;
   int64_t tps = (tiles + want - 1) / want;
-  if (!p.tile_form) tps = (tps + 3) / 4 * 4;
+  if (!p.tile_form) tps = (tps + 3) / 4 * 4 < kMaxSplitTiles ? (tps + 3) / 4 * 4 : kMaxSplitTiles;
   p.tiles_per_split = tps > 0 ? (int)tps : 4;
   p.n_split = tiles > 0 ? (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
   return p;
@@ -1058,7 +1102,10 @@ static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dll
   if (rc) return rc;
   if (p.n_split > 1) {
     const int64_t rows = (int64_t)n_seg * Hkv * p.mtiles * p.bm;
-    chunk_combine_kernel<<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a, paged);
+    if (p.n_split > 8)
+      chunk_combine_kernel<8><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a, paged);
+    else
+      chunk_combine_kernel<1><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a, paged);
     rc = check_launch(name);
   }
   return rc;
