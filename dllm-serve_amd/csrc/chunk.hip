@@ -1,7 +1,7 @@
 // Attention of a chunk of new tokens over a paged cache (8-bit or bf16 pages) and
 // over itself, bidirectional, causal or causal between blocks.
 //
-// Segment s has n cached rows, in pages or by slot, and L new rows whose K / V are
+// Segment s has n cached rows in pages and L new rows whose K / V are
 // given in bf16.  New row t sees every cached row and the new rows j < vis(t):
 //   vis(t) = L                                  mask_block = 0
 //   vis(t) = min(L, ((n + t) / b + 1) * b - n)  mask_block = b >= 1 (1: causal)
@@ -11,9 +11,8 @@
 // head hkv * g + m % g; every K / V byte that is read serves all of them.
 //
 //   * chunk_rows_kernel (few M rows: single tokens, blocks): each of a workgroup's
-//     four wavefronts takes 32-key tiles of its own; K goes from memory straight
-//     into MFMA operands, V through the wavefront's own LDS for the transposition.
-//     No wavefront waits for another until the states are merged at the end.
+//     four wavefronts takes 32-key tiles of its own, by DMA into its own LDS.  No
+//     wavefront waits for another until the states are merged at the end.
 //   * chunk_tile_kernel (many M rows: pieces of prompts): 64-key tiles of K and V in LDS,
 //     in bf16, shared by the workgroup's wavefronts of 32 M rows each; 8-bit rows are
 //     converted once, on their way into LDS.
@@ -30,15 +29,15 @@ struct ChunkArgs {
   const uint16_t* k;
   const uint16_t* v;
   uint16_t* o;
-  const uint8_t* kc;      // cache: records (8-bit) or bf16 rows [slots][Hkv][128]
+  const uint8_t* kc;      // cache: records (8-bit) or bf16 rows [pages * 256][Hkv][128]
   const uint8_t* vc;
   const int32_t* cu;
   const int32_t* seg_ids;
-  const int32_t* table;   // page table [n_seg][max_pages], or the slot list
-  const int32_t* lens;    // cached lengths [n_seg], or slot offsets [n_seg + 1]
+  const int32_t* table;   // page table [n_seg][max_pages]
+  const int32_t* lens;    // cached lengths [n_seg]
   float* ws;
   int64_t q_stride, k_stride, v_stride, o_stride;
-  int64_t cache_rows;     // rows of the cache (a multiple of 256 with pages)
+  int64_t cache_rows;     // rows of the cache, whole pages
   int max_pages, max_q, max_cached;
   int n_seg, Hkv, g, mtiles, n_split, tiles_per_split;
   int mask_block;
@@ -49,27 +48,18 @@ struct ChunkArgs {
 };
 
 constexpr int kTileKeys = 32;   // keys of a wavefront's tile
-constexpr int kVTile = kTileKeys * 256;
 constexpr int kMaxSplitTiles = 62 * kPageRows / kTileKeys;  // chunk_rows_kernel: at most 63 pages, one a lane
 
 // Segment s: new rows' first row and count, cached rows.
 struct Segment {
   int row0, len, cached;
-  int64_t slot0;  // slot list: first entry
 };
-template <bool PAGED>
 __device__ __forceinline__ Segment segment(const ChunkArgs& a, int s) {
   Segment g;
   const int id = a.seg_ids ? a.seg_ids[s] : s;
   g.row0 = a.cu[id];
   g.len = a.cu[id + 1] - g.row0;
-  if (PAGED) {
-    g.cached = a.lens[s];
-    g.slot0 = 0;
-  } else {
-    g.slot0 = a.lens[s];
-    g.cached = a.lens[s + 1] - (int)g.slot0;
-  }
+  g.cached = a.lens[s];
   // what the launch was sized for
   g.len = min(max(g.len, 0), a.max_q);
   g.cached = min(max(g.cached, 0), a.max_cached);
@@ -119,28 +109,43 @@ __device__ __forceinline__ float row_sum4(float x) {
 // Lane (c = l % 16, g4 = l / 16) holds K row 16 u + c and, in the results, M row c:
 // scores of keys 16 u + 4 g4 + i, outputs d = 16 dt + 4 g4 + i.  A contraction does
 // not depend on the order of its index, so the four lanes of a K row each take
-// whole 16-byte pieces of it (FP8: piece c2 covers d = 64 c2 + 16 g4 .. + 15, two
+// whole 16-byte pieces of it (8-bit: piece p covers d = 64 p + 16 g4 .. + 15, two
 // steps; bf16: step s covers d = 32 s + 8 g4 .. + 7), Q^T is loaded in the same
 // order, and P^T is fed to the second product as it stands: its index (g4, i) is
 // key 4 g4 + i for i < 4 and 16 + 4 g4 + i - 4 otherwise, which V^T follows.
 //
-// V goes to the wavefront's LDS tile [32 keys][256 B] in bf16, 16-byte chunk p of a
-// row at p ^ 2 (row & 7), and comes back by ds_read_b64_tr_b16: the eight lanes of a
-// write phase and the sixteen (row, chunk) pairs of a read phase fall on different banks.
+// K and V come by DMA into two stages of the wavefront's own LDS, as they are (8-bit
+// rows with their scale bytes), so that two tiles -- 16 KiB in 8 bits -- are in flight
+// without registers, and no wavefront waits for another.  8-bit codes become bf16
+// on their way from LDS into the operands: K with its row's scale, which is part of
+// the conversion; V^T, whose operand holds eight keys of one d
+// (ds_read_b64_tr_b8: in a group of 16 lanes lane 2k + h supplies bytes 8 h .. 8 h + 7
+// of row k of an 8 x 16 block and lane n receives column n), without: the powers of two
+// are multiplied onto P instead, which commutes with its rounding.
+//
+// Chunks of 16 bytes are XOR-swizzled inside a row, so that the lanes of a read phase
+// fall on different banks:
+//   8-bit K, V [32][128 B]  chunk ^ (row / 2 & 7) ^ 4 (row / 16)
+//   bf16 K [32][256 B]      chunk ^ (row & 15)
+//   bf16 V [32][256 B]      chunk ^ 2 (row & 7)
 template <bool FP8>
-struct TileRegs {
-  static constexpr int N = FP8 ? 2 : 4;  // 16-byte pieces of a lane's row
-  u32x4_t k[2][N];
-  u32x4_t v[2][N];
-  uint32_t kscale[2], vscale[2];  // 8-bit rows: scale bytes (pages: one word holds all four, see unpack)
-  uint32_t bad;                   // keys to leave out
+struct RowsTile {
+  static constexpr int kRow = FP8 ? kQuantD : 2 * HD;
+  static constexpr int kV = kTileKeys * kRow;      // offset of V in a stage
+  static constexpr int kScales = 2 * kV;           // K's 32 scale bytes, then V's
+  static constexpr int kStage = FP8 ? kScales + 256 : kScales;
+  static constexpr int kDma = kV / 1024;           // instructions of one matrix
+  static constexpr int kOps = 2 * kDma + (FP8 ? 1 : 0);
 };
 
 // Floats of a wavefront's parked O (rows of 128 + 4, which spreads them over the
-// banks) and bytes of a workgroup's LDS: V tiles, then the parked O, then m and l.
+// banks), and bytes of a workgroup's LDS: the stages, later the parked O, m and l.
 constexpr int park_floats(int nb) { return 16 * nb * 132; }
-constexpr int park_off(int nb) { return 4 * (park_floats(nb) > kVTile / 4 ? park_floats(nb) : kVTile / 4); }
-constexpr int rows_lds(int nb) { return (park_off(nb) + 8 * 16 * nb) * 4; }
+template <int NB, bool FP8>
+constexpr int rows_lds() {
+  constexpr int stages = 4 * 2 * RowsTile<FP8>::kStage, park = (4 * park_floats(NB) + 8 * 16 * NB) * 4;
+  return stages > park ? stages : park;
+}
 
 template <int NB>
 struct RowState {
@@ -159,8 +164,11 @@ __device__ __forceinline__ void rows_init(RowState<NB>& st) {
   }
 }
 
-// Online softmax of one 32-key tile of one row block; p comes back as the B operand.
-__device__ __forceinline__ bf16x8_t rows_softmax(const f32x4_t (&s)[2], f32x4_t (&o)[8], float& m, float& l, float c) {
+// Online softmax of one 32-key tile of one row block; p, times the keys' V scales
+// where SCALED, comes back as the B operand.
+template <bool SCALED>
+__device__ __forceinline__ bf16x8_t rows_softmax(const f32x4_t (&s)[2], f32x4_t (&o)[8], float& m, float& l, float c,
+                                                 const float (&vs)[8]) {
   float mx = s[0][0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
@@ -182,8 +190,9 @@ __device__ __forceinline__ bf16x8_t rows_softmax(const f32x4_t (&s)[2], f32x4_t 
   for (int w = 0; w < 4; ++w) {
     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w >> 1][(2 * w) & 3], c, neg));
     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w >> 1][(2 * w + 1) & 3], c, neg));
-    pk[w] = cvt_pk_bf16(p0, p1);
-    l = add_bf16x2(pk[w], l);  // the rounded numerators, as the product uses them
+    const uint32_t r = cvt_pk_bf16(p0, p1);
+    l = add_bf16x2(r, l);  // the rounded numerators, as the product uses them
+    pk[w] = SCALED ? cvt_pk_bf16(p0 * vs[2 * w], p1 * vs[2 * w + 1]) : r;
   }
   return as_bf16x8(pk);
 }
@@ -211,11 +220,58 @@ __device__ __forceinline__ void wave_lds_fence() {
   asm volatile("" ::: "memory");
 }
 
-template <int NB, bool FP8, bool PAGED>
+// The V^T codes of a tile, eight d blocks (one asm block with its own wait: the
+// builtin would wait for the DMA of the next tiles as well).  vb: this lane's address
+// for block 0; block dt is at vb ^ 16 dt.
+__device__ __forceinline__ void v_codes(const uint8_t* vb_ptr, u32x2_t (&r)[8]) {
+  const uint32_t vb = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)vb_ptr;
+  asm volatile(
+      "ds_read_b64_tr_b8 %0, %8\n"
+      "ds_read_b64_tr_b8 %1, %9\n"
+      "ds_read_b64_tr_b8 %2, %10\n"
+      "ds_read_b64_tr_b8 %3, %11\n"
+      "ds_read_b64_tr_b8 %4, %12\n"
+      "ds_read_b64_tr_b8 %5, %13\n"
+      "ds_read_b64_tr_b8 %6, %14\n"
+      "ds_read_b64_tr_b8 %7, %15\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+      : "v"(vb), "v"(vb ^ 16u), "v"(vb ^ 32u), "v"(vb ^ 48u), "v"(vb ^ 64u), "v"(vb ^ 80u), "v"(vb ^ 96u), "v"(vb ^ 112u)
+      : "memory");
+}
+// The same for bf16 rows: blocks at vb ^ 32 dt, keys 16 .. 31 4 KiB further; output 2 dt + half.
+__device__ __forceinline__ void v_rows(const uint8_t* vb_ptr, u32x2_t (&r)[16]) {
+  const uint32_t vb = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)vb_ptr;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16\n"
+      "ds_read_b64_tr_b16 %1, %16 offset:4096\n"
+      "ds_read_b64_tr_b16 %2, %17\n"
+      "ds_read_b64_tr_b16 %3, %17 offset:4096\n"
+      "ds_read_b64_tr_b16 %4, %18\n"
+      "ds_read_b64_tr_b16 %5, %18 offset:4096\n"
+      "ds_read_b64_tr_b16 %6, %19\n"
+      "ds_read_b64_tr_b16 %7, %19 offset:4096\n"
+      "ds_read_b64_tr_b16 %8, %20\n"
+      "ds_read_b64_tr_b16 %9, %20 offset:4096\n"
+      "ds_read_b64_tr_b16 %10, %21\n"
+      "ds_read_b64_tr_b16 %11, %21 offset:4096\n"
+      "ds_read_b64_tr_b16 %12, %22\n"
+      "ds_read_b64_tr_b16 %13, %22 offset:4096\n"
+      "ds_read_b64_tr_b16 %14, %23\n"
+      "ds_read_b64_tr_b16 %15, %23 offset:4096\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+        "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+      : "v"(vb), "v"(vb ^ 32u), "v"(vb ^ 64u), "v"(vb ^ 96u), "v"(vb ^ 128u), "v"(vb ^ 160u), "v"(vb ^ 192u), "v"(vb ^ 224u)
+      : "memory");
+}
+
+template <int NB, bool FP8>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(ChunkArgs a) {
+  using T = RowsTile<FP8>;
   constexpr int BM = 16 * NB;
   constexpr int PARK = park_floats(NB);
-  extern __shared__ __attribute__((aligned(16))) float lds[];  // rows_lds(NB) bytes
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // rows_lds() bytes
   const int L = xcd_remap(blockIdx.x, a.xcd_chunk);
   if (L >= a.logical_blocks) return;
   int r = L;
@@ -225,7 +281,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   r /= a.n_split;
   const int hkv = r % a.Hkv;
   const int s = r / a.Hkv;
-  const Segment sg = segment<PAGED>(a, s);
+  const Segment sg = segment(a, s);
   const int g = a.g;
   const int M = sg.len * g;
   const int m_base = mt * BM;
@@ -236,7 +292,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int col = lane & 15, g4 = lane >> 4;
-  uint8_t* const vt = reinterpret_cast<uint8_t*>(lds) + wave * kVTile;
+  uint8_t* const my = reinterpret_cast<uint8_t*>(lds) + wave * 2 * T::kStage;
+
+  const int tiles = (sg.cached + kTileKeys - 1) / kTileKeys;
+  const int t_begin = split * a.tiles_per_split;
+  const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
+  const int t_end = n_pages ? min(tiles, t_begin + a.tiles_per_split) : t_begin;  // no cache: nothing to read
+  const uint32_t bf_row = (uint32_t)(a.Hkv * HD * 2);
+  // Page ids of the split, one a lane (a split spans at most 63): a tile's loads
+  // then wait for no load of their own.
+  const int pg0 = t_begin * kTileKeys / kPageRows;
+  const int page_reg = t_begin < t_end ? a.table[(int64_t)s * a.max_pages + min(pg0 + lane, a.max_pages - 1)] : -1;
 
   // ---- Q^T operands and the rows' limits ------------------------------------
   bf16x8_t qf[NB][4];
@@ -259,89 +325,58 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   }
 
-  const int tiles = (sg.cached + kTileKeys - 1) / kTileKeys;
-  const int t_begin = split * a.tiles_per_split;
-  const uint32_t n_rows = (uint32_t)min(a.cache_rows, (int64_t)1 << 31);
-  const int t_end = n_rows ? min(tiles, t_begin + a.tiles_per_split) : t_begin;  // no cache: nothing to read
-  const int32_t* const table = PAGED ? a.table + (int64_t)s * a.max_pages : a.table + sg.slot0;
-  const int64_t bf_row = (int64_t)a.Hkv * HD * 2;
-  // Page ids of the split, one a lane (a split spans at most 63): a tile's
-  // loads then wait for no load of their own.
-  const int pg0 = t_begin * kTileKeys / kPageRows;
-  const int page_reg = PAGED && t_begin < t_end ? table[min(pg0 + lane, a.max_pages - 1)] : -1;
-
-  // Loads of cached tile t.  Rows that do not exist (past the cached length, of a
-  // page or slot outside the cache) read row 0 of the cache or nothing, and are in `bad`.
-  auto load_tile = [&](int t, TileRegs<FP8>& x) {
-    const int key0 = t * kTileKeys;
-    const int left = sg.cached - key0;  // >= 1
-    uint32_t bad = left >= 32 ? 0u : ~0u << left;
-    if constexpr (PAGED) {
-      const int pg = key0 >> 8;
-      int pid = pg < a.max_pages ? __builtin_amdgcn_readlane(page_reg, (pg - pg0) & 63) : -1;
-      const bool in = (uint32_t)pid < (n_rows >> 8);
-      pid = in ? pid : 0;
-      if (!in) bad = ~0u;
-      const int row0 = key0 & (kPageRows - 1);
-      const int64_t rec = FP8 ? ((int64_t)pid * a.Hkv + hkv) * kRecord : (int64_t)pid * kPageRows * bf_row + hkv * HD * 2;
-      const uint32_t rowb = FP8 ? kQuantD : (uint32_t)bf_row;
-      // rows past the cached length read as zero through the buffer's bound
-      const uint32_t rows = in ? (uint32_t)min(kPageRows, row0 + left) : 0u;
-      const uint32_t bytes = rows == 0 ? 0u : (rows - 1) * rowb + (FP8 ? kQuantD : HD * 2);
-      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec, bytes), vrs = make_rsrc(a.vc + rec, bytes);
+  // page of tile t, or -1: outside the cache, its rows are left out
+  auto page_of = [&](int t) -> int {
+    const int pg = t * kTileKeys / kPageRows;
+    const int pid = __builtin_amdgcn_readlane(page_reg, (pg - pg0) & 63);
+    return pg < a.max_pages && (uint32_t)pid < n_pages ? pid : -1;
+  };
+  // DMA of cached tile t into a stage; rows past the cached length, and all rows of a
+  // page outside the cache, arrive as zeros through the buffer's bound.
+  auto issue = [&](uint8_t* stage, int t) {
+    const int pid = page_of(t);
+    const int row0 = t * kTileKeys & (kPageRows - 1);
+    const int rows = pid < 0 ? 0 : min(sg.cached - t * kTileKeys, kTileKeys);
+    if constexpr (FP8) {
+      const int64_t rec = ((int64_t)max(pid, 0) * a.Hkv + hkv) * kRecord;
+      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
+      const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.vc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
+      // lane l of instruction j: row 8 j + l / 8, physical chunk l % 8
+      const uint32_t row = (uint32_t)((lane >> 3) * kQuantD), ch = (uint32_t)((lane & 7) ^ (lane >> 4)) * 16;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int p = 0; p < TileRegs<FP8>::N; ++p) {
-          const uint32_t off = (uint32_t)(row0 + 16 * u + col) * rowb + (uint32_t)(p * 64 + g4 * 16);
-          x.k[u][p] = bload(krs, off, 0u);
-          x.v[u][p] = bload(vrs, off, 0u);
-        }
-      if constexpr (FP8) {
-        // lanes 0..31: the K scales of the tile's rows, 32..63: the V scales
-        const uint8_t* sp = (lane < 32 ? a.kc : a.vc) + (in ? rec : 0) + kScaleOff + row0 + (lane & 31);
-        x.kscale[0] = n_rows && (lane & 31) < left ? *sp : 127u;
+      for (int j = 0; j < T::kDma; ++j) {
+        const uint32_t off = (uint32_t)(j * 1024) + row + (ch ^ (uint32_t)(j == 1 || j == 2 ? 64 : 0));
+        dma16<kStreamAux>(krs, stage + j * 1024, off);
+        dma16<kStreamAux>(vrs, stage + T::kV + j * 1024, off);
       }
+      // lanes 0 .. 7: K's scale bytes, 8 .. 15: V's (the others repeat them)
+      const uint8_t* sp = (lane & 8 ? a.vc : a.kc) + rec + kScaleOff + row0 + (lane & 7) * 4;
+      __builtin_amdgcn_global_load_lds(sp, (__attribute__((address_space(3))) void*)(stage + T::kScales), 4, 0, 0);
     } else {
-      u32x4_t zero = {0, 0, 0, 0};
-      uint32_t out = 0;
+      const int64_t off0 = ((int64_t)max(pid, 0) * kPageRows + row0) * bf_row + hkv * HD * 2;
+      const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * bf_row + HD * 2 : 0u;
+      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + off0, bytes), vrs = make_rsrc(a.vc + off0, bytes);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = 16 * u + col;
-        const uint32_t sl = key < left ? (uint32_t)table[key0 + key] : ~0u;
-        const bool in = sl < n_rows;
-        out |= (uint32_t)(__builtin_amdgcn_ballot_w64(!in) & 0xffffu) << (16 * u);
-#pragma unroll
-        for (int p = 0; p < TileRegs<FP8>::N; ++p) x.k[u][p] = x.v[u][p] = zero;
-        x.kscale[u] = x.vscale[u] = 127u;
-        if (in) {
-          const int64_t rec = FP8 ? record_off(sl, a.Hkv, hkv) : (int64_t)sl * bf_row + hkv * HD * 2;
-          const int64_t row = FP8 ? (int64_t)(sl & (kPageRows - 1)) * kQuantD : 0;
-#pragma unroll
-          for (int p = 0; p < TileRegs<FP8>::N; ++p) {
-            x.k[u][p] = ld128_stream(a.kc + rec + row + p * 64 + g4 * 16);
-            x.v[u][p] = ld128_stream(a.vc + rec + row + p * 64 + g4 * 16);
-          }
-          if constexpr (FP8) {
-            x.kscale[u] = a.kc[rec + kScaleOff + (sl & (kPageRows - 1))];
-            x.vscale[u] = a.vc[rec + kScaleOff + (sl & (kPageRows - 1))];
-          }
-        }
+      for (int j = 0; j < T::kDma; ++j) {  // lane l: row 4 j + l / 16, physical chunk l % 16
+        const int row = 4 * j + g4;
+        dma16<kStreamAux>(krs, stage + j * 1024, (uint32_t)row * bf_row + (uint32_t)((col ^ (row & 15)) * 16));
+        dma16<kStreamAux>(vrs, stage + T::kV + j * 1024, (uint32_t)row * bf_row + (uint32_t)((col ^ (2 * (row & 7))) * 16));
       }
-      bad = out;
     }
-    x.bad = bad;
   };
 
   RowState<NB> st;
   rows_init(st);
   const float c = a.scale_log2;
-  // this lane's transposing-read address: row 4 g4 + col / 4, chunk (col & 3) / 2
-  const int trow = 4 * g4 + (col >> 2);
-  const uint32_t vbase = (uint32_t)(trow * 256 + ((((col & 3) >> 1) ^ (2 * (trow & 7))) * 16) + 8 * (col & 1));
+  // this lane's transposing reads: bf16 rows, row 4 g4 + col / 4, chunk (col & 3) / 2 of a
+  // 32-byte block; 8-bit rows, row 4 g4 + k or 16 + 4 g4 + k - 4 with k = col / 2, half col & 1
+  const int row16 = 4 * g4 + (col >> 2);
+  const uint32_t vb16 = (uint32_t)(row16 * 256 + ((((col & 3) >> 1) ^ (2 * (row16 & 7))) * 16) + 8 * (col & 1));
+  const int k8 = col >> 1, row8 = k8 < 4 ? 4 * g4 + k8 : 12 + 4 * g4 + k8;
+  const uint32_t vb8 = (uint32_t)(row8 * 128 + ((((row8 >> 1) & 7) ^ (4 * (row8 >> 4))) * 16) + 8 * (col & 1));
 
-  // K fragments of key half u from keys(u, .), V in LDS: both products and the softmax.
-  auto products = [&](auto&& keys, auto&& hide) {
+  // S^T of a tile whose K fragments of half u are keys(u, .), hide() its keys, softmax.
+  auto scores = [&](auto&& keys, auto&& hide, const float (&vs)[8], auto scaled, bf16x8_t (&pf)[NB]) {
     f32x4_t sc[NB][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -355,96 +390,112 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           sc[b][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k4], qf[b][k4], sc[b][u], 0, 0, 0);
       }
     }
-    bf16x8_t pf[NB];
+    hide(sc);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      hide(sc[b], b);
-      pf[b] = rows_softmax(sc[b], st.o[b], st.m[b], st.l[b], c);
-    }
+    for (int b = 0; b < NB; ++b)
+      pf[b] = rows_softmax<decltype(scaled)::value>(sc[b], st.o[b], st.m[b], st.l[b], c, vs);
+  };
+  auto add_bf16_rows = [&](const uint8_t* vtile, const bf16x8_t (&pf)[NB]) {
+    u32x2_t x[16];
+    v_rows(vtile + vb16, x);
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-      const uint8_t* vp = vt + (vbase ^ (uint32_t)(32 * dt));
-      const u32x2_t lo = ds_read_tr16(vp), hi = ds_read_tr16(vp + 16 * 256);
-      const bf16x8_t af = as_bf16x8(u32x4_t{lo[0], lo[1], hi[0], hi[1]});
+    for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        st.o[b][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pf[b], st.o[b][dt], 0, 0, 0);
-    }
-  };
-  auto put_v = [&](int row, int chunk, u32x4_t w) {
-    *reinterpret_cast<u32x4_t*>(vt + row * 256 + ((chunk ^ (2 * (row & 7))) * 16)) = w;
+        st.o[b][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            as_bf16x8(u32x4_t{x[2 * dt][0], x[2 * dt][1], x[2 * dt + 1][0], x[2 * dt + 1][1]}), pf[b], st.o[b][dt], 0, 0, 0);
   };
 
-  auto compute_tile = [&](const TileRegs<FP8>& x) {
-    float ks[2], vs[2];
-    if constexpr (FP8) {
-      if constexpr (PAGED) {
-        // rows of 16 lanes of the word hold K u = 0, K u = 1, V u = 0, V u = 1: each to all lanes
-        const uint32_t w = x.kscale[0] << 23;
-        const auto h = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-        const auto r0 = __builtin_amdgcn_permlane32_swap((uint32_t)h[0], (uint32_t)h[0], false, false);
-        const auto r1 = __builtin_amdgcn_permlane32_swap((uint32_t)h[1], (uint32_t)h[1], false, false);
-        ks[0] = __uint_as_float((uint32_t)r0[0]);
-        vs[0] = __uint_as_float((uint32_t)r0[1]);
-        ks[1] = __uint_as_float((uint32_t)r1[0]);
-        vs[1] = __uint_as_float((uint32_t)r1[1]);
+  auto compute_tile = [&](const uint8_t* stage, int t) {
+    const int left = page_of(t) < 0 ? 0 : sg.cached - t * kTileKeys;
+    const uint32_t bad = left >= kTileKeys ? 0u : ~0u << left;  // keys to leave out
+    u32x4_t kx[2][FP8 ? 2 : 4];
+    float ks[2] = {0.f, 0.f}, vs[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (FP8) {
+        const uint32_t sw = (uint32_t)(((col >> 1) & 7) ^ (4 * u));
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          kx[u][p] = *reinterpret_cast<const u32x4_t*>(stage + (16 * u + col) * 128 + (((4 * p + g4) ^ sw) * 16));
+        ks[u] = scale_of(stage[T::kScales + 16 * u + col]);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(stage + T::kScales + 32 + 16 * u + 4 * g4);
+        vs[4 * u] = __uint_as_float((w << 23) & 0x7f800000u);
+        vs[4 * u + 1] = __uint_as_float((w << 15) & 0x7f800000u);
+        vs[4 * u + 2] = __uint_as_float((w << 7) & 0x7f800000u);
+        vs[4 * u + 3] = __uint_as_float((w >> 1) & 0x7f800000u);
       } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          ks[u] = scale_of(x.kscale[u]);
-          vs[u] = scale_of(x.vscale[u]);
-        }
+        for (int p = 0; p < 4; ++p)
+          kx[u][p] = *reinterpret_cast<const u32x4_t*>(stage + (16 * u + col) * 256 + (((4 * p + g4) ^ col) * 16));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vs[4 * u + i] = 1.f;
       }
     }
-    wave_lds_fence();  // the reads of the tile before
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int p = 0; p < TileRegs<FP8>::N; ++p) {
-        const int row = 16 * u + col;
-        if constexpr (FP8) {
-          put_v(row, 8 * p + 2 * g4, dequant8(u32x2_t{x.v[u][p][0], x.v[u][p][1]}, vs[u]));
-          put_v(row, 8 * p + 2 * g4 + 1, dequant8(u32x2_t{x.v[u][p][2], x.v[u][p][3]}, vs[u]));
-        } else {
-          put_v(row, 4 * p + g4, x.v[u][p]);
-        }
-      }
-    wave_lds_fence();
-    const uint32_t bad = x.bad;
     auto keys = [&](int u, bf16x8_t (&kf)[4]) {
 #pragma unroll
-      for (int p = 0; p < TileRegs<FP8>::N; ++p) {
+      for (int p = 0; p < (FP8 ? 2 : 4); ++p) {
         if constexpr (FP8) {
-          kf[2 * p] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][0], x.k[u][p][1]}, ks[u]));
-          kf[2 * p + 1] = as_bf16x8(dequant8(u32x2_t{x.k[u][p][2], x.k[u][p][3]}, ks[u]));
+          kf[2 * p] = as_bf16x8(dequant8(u32x2_t{kx[u][p][0], kx[u][p][1]}, ks[u]));
+          kf[2 * p + 1] = as_bf16x8(dequant8(u32x2_t{kx[u][p][2], kx[u][p][3]}, ks[u]));
         } else {
-          kf[p] = as_bf16x8(x.k[u][p]);
+          kf[p] = as_bf16x8(kx[u][p]);
         }
       }
     };
-    products(keys, [&](f32x4_t (&sc)[2], int) {
+    auto hide = [&](f32x4_t (&sc)[NB][2]) {
       if (bad) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if ((bad >> (16 * u + 4 * g4 + i)) & 1u) sc[u][i] = -INFINITY;
+            if ((bad >> (16 * u + 4 * g4 + i)) & 1u) {
+#pragma unroll
+              for (int b = 0; b < NB; ++b) sc[b][u][i] = -INFINITY;
+              vs[4 * u + i] = 0.f;  // the scale byte of a row that does not exist may be anything
+            }
       }
-    });
+    };
+    bf16x8_t pf[NB];
+    scores(keys, hide, vs, std::integral_constant<bool, FP8>(), pf);
+    if constexpr (FP8) {
+      u32x2_t x[8];
+      v_codes(stage + T::kV + vb8, x);
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) {
+        const bf16x8_t af = as_bf16x8(dequant8(x[dt], 1.f));
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          st.o[b][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pf[b], st.o[b][dt], 0, 0, 0);
+      }
+    } else {
+      add_bf16_rows(stage + T::kV, pf);
+    }
   };
 
-  // ---- cached tiles: this wavefront takes every fourth, the next one in flight ----
+  // ---- cached tiles: this wavefront takes every fourth, two in flight --------------
   {
-    TileRegs<FP8> x, y;
-    int t = t_begin + wave;
-    if (t < t_end) load_tile(t, x);
-    for (; t < t_end; t += 8) {
-      if (t + 4 < t_end) load_tile(t + 4, y);
-      compute_tile(x);
-      if (t + 4 < t_end) {
-        if (t + 8 < t_end) load_tile(t + 8, x);
-        compute_tile(y);
-      }
+    const int n = max(0, (t_end - t_begin - wave + 3) >> 2);  // this wavefront's tiles
+    const int first = t_begin + wave;
+    asm volatile("" ::: "memory");  // the page ids and q stay the oldest operations
+    if (n > 0) issue(my, first);
+    if (n > 1) issue(my + T::kStage, first + 4);
+    // q has landed, the tiles may be in flight
+    if (n > 1)
+      vm_wait<2 * T::kOps>();
+    else if (n == 1)
+      vm_wait<T::kOps>();
+    else
+      vm_wait<0>();
+    for (int i = 0; i < n; ++i) {
+      if (i + 1 < n)
+        vm_wait<T::kOps>();
+      else
+        vm_wait<0>();
+      uint8_t* const stage = my + (i & 1) * T::kStage;
+      compute_tile(stage, first + 4 * i);
+      wave_lds_fence();  // the tile's reads end before its stage is filled again
+      if (i + 2 < n) issue(stage, first + 4 * i + 8);
     }
   }
 
@@ -487,23 +538,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
           for (int p = 0; p < 4; ++p) vx[u][p] = finite_part(vx[u][p]);
       }
+      // V in bf16, as a tile of bf16 rows
       wave_lds_fence();
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) put_v(16 * u + col, 4 * p + g4, vx[u][p]);
+        for (int p = 0; p < 4; ++p) {
+          const int row = 16 * u + col;
+          *reinterpret_cast<u32x4_t*>(my + row * 256 + (((4 * p + g4) ^ (2 * (row & 7))) * 16)) = vx[u][p];
+        }
       wave_lds_fence();
       auto keys = [&](int u, bf16x8_t (&kf)[4]) {
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) kf[k4] = kx[u][k4];
       };
-      products(keys, [&](f32x4_t (&sc)[2], int b) {
+      auto hide = [&](f32x4_t (&sc)[NB][2]) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (t * kTileKeys + 16 * u + 4 * g4 + i >= lim[b]) sc[u][i] = -INFINITY;
-      });
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (t * kTileKeys + 16 * u + 4 * g4 + i >= lim[b]) sc[b][u][i] = -INFINITY;
+      };
+      const float one[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+      bf16x8_t pf[NB];
+      scores(keys, hide, one, std::false_type(), pf);
+      add_bf16_rows(my, pf);
       if (fix) {
         const int end = min((t + 1) * kTileKeys, sg.len);
         for (int j = t * kTileKeys; j < end; ++j)
@@ -526,8 +587,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 
   // ---- merge of the four wavefronts ------------------------------------------------
-  float* const ml = lds + park_off(NB);
-  __syncthreads();  // the V tiles are free
+  float* const ml = lds + 4 * PARK;
+  __syncthreads();  // the stages are free
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const float lt = row_sum4(st.l[b]);
@@ -610,7 +671,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   r /= a.n_split;
   const int hkv = r % a.Hkv;
   const int s = r / a.Hkv;
-  const Segment sg = segment<true>(a, s);
+  const Segment sg = segment(a, s);
   const int g = a.g;
   const int M = sg.len * g;
   const int m_base = mt * BM;
@@ -874,7 +935,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // of many parts is one round of loads rather than a long chain (28 rows of 128 parts:
 // 39 us with one group, see the launch).
 template <int G>
-__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, bool paged) {
+__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a) {
   constexpr int ROWS = 8 / G;
   __shared__ f32x4_t part[G > 1 ? 256 : 1];
   __shared__ float part_ml[G > 1 ? 16 : 1];
@@ -889,7 +950,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a, bool pa
   const int mrow = (int)(idx - (int64_t)pair * per);
   const int hkv = pair % a.Hkv;
   const int s = pair / a.Hkv;
-  const Segment sg = paged ? segment<true>(a, s) : segment<false>(a, s);
+  const Segment sg = segment(a, s);
   if (mrow >= sg.len * a.g) return;
   const int ns = splits_of(a, sg, mrow / bm);
   if (ns == 1) return;
@@ -949,11 +1010,11 @@ struct ChunkPlan {
   int bm, mtiles;                // M rows of a workgroup, M tiles
   int n_split, tiles_per_split;  // workgroups along the keys
 };
-static ChunkPlan chunk_plan(bool paged, int n_seg, int max_q, int max_cached, int Hq, int Hkv) {
+static ChunkPlan chunk_plan(int n_seg, int max_q, int max_cached, int Hq, int Hkv) {
   ChunkPlan p = {};
   const int64_t rows = (int64_t)max_q * (Hq / Hkv);
   const int64_t pairs = (int64_t)n_seg * Hkv;
-  p.tile_form = paged && rows > 64;
+  p.tile_form = rows > 64;
   if (p.tile_form) {
     p.nw = pairs * ((rows + 255) / 256) >= 256 ? 8 : 4;
     p.bm = 32 * p.nw;
@@ -991,17 +1052,14 @@ static bool chunk_sizes_ok(int n_seg, int max_q, int max_cached, int Hq, int Hkv
 
 extern "C" size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D) {
   if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D) || n_seg == 0 || max_q == 0) return 0;
-  // the larger of the two entry points' needs
-  const size_t paged = chunk_ws(chunk_plan(true, n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
-  const size_t slots = chunk_ws(chunk_plan(false, n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
-  return paged > slots ? paged : slots;
+  return chunk_ws(chunk_plan(n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
 }
 
 extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D, int* rows,
                                             int* n_split, int* grid) {
   if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
     return fail(DLLM_ERR_INVALID_ARG, "dllm_attn_chunk_launch_shape: unsupported sizes");
-  const ChunkPlan p = chunk_plan(true, n_seg, max_q, max_cached, Hq, Hkv);
+  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
   const bool none = n_seg == 0 || max_q == 0;
   if (rows) *rows = p.bm;
   if (n_split) *n_split = p.n_split;
@@ -1013,16 +1071,18 @@ extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached
   return DLLM_OK;
 }
 
-static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
-                     const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached, const void* k_cache,
-                     const void* v_cache, int cache_type, int64_t cache_rows, const int32_t* table, int max_pages,
-                     const int32_t* lens, int mask_block, int Hq, int Hkv, int D, int64_t q_stride, int64_t k_stride,
-                     int64_t v_stride, int64_t o_stride, float softmax_scale, void* workspace, size_t workspace_bytes,
-                     void* stream) {
+extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
+                                         const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
+                                         const void* k_cache, const void* v_cache, int cache_type, int num_pages,
+                                         const int32_t* page_table, int max_pages, const int32_t* cached_len,
+                                         int mask_block, int Hq, int Hkv, int D, int64_t q_stride, int64_t k_stride,
+                                         int64_t v_stride, int64_t o_stride, float softmax_scale, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  const char* name = "dllm_attn_chunk_paged_fwd";
   set_error("");
   int rc = common_checks(name, q, k, v, o, Hq, Hkv, D, q_stride, k_stride, v_stride, o_stride);
   if (rc) return rc;
-  if (n_seg < 0 || max_q < 0 || max_cached < 0 || mask_block < 0 || max_pages < 0 || cache_rows < 0)
+  if (n_seg < 0 || max_q < 0 || max_cached < 0 || mask_block < 0 || max_pages < 0)
     return fail(DLLM_ERR_INVALID_ARG, "%s: negative size", name);
   if (cache_type != DLLM_CACHE_BF16 && cache_type != DLLM_CACHE_FP8)
     return fail(DLLM_ERR_INVALID_ARG, "%s: cache type %d", name, cache_type);
@@ -1032,18 +1092,16 @@ static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dll
   if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
     return fail(DLLM_ERR_UNSUPPORTED, "%s: %d new rows of %d query heads per KV head, %d cached", name, max_q, Hq / Hkv,
                 max_cached);
-  if (!cu || !lens) return fail(DLLM_ERR_INVALID_ARG, "%s: null cu / lengths", name);
+  if (num_pages < 0 || num_pages > (1 << 23)) return fail(DLLM_ERR_INVALID_ARG, "%s: %d pages", name, num_pages);
+  if (!cu || !cached_len) return fail(DLLM_ERR_INVALID_ARG, "%s: null cu / lengths", name);
   const int64_t kvs = k_stride > v_stride ? k_stride : v_stride;
   if ((int64_t)max_q * (q_stride > kvs ? q_stride : kvs) * 2 + 4096 >= ((int64_t)1 << 32))
     return fail(DLLM_ERR_UNSUPPORTED, "%s: a segment spans more than 4 GiB of q / k / v", name);
   if (cache_type == DLLM_CACHE_BF16 && (int64_t)Hkv * HD * 2 * kPageRows >= ((int64_t)1 << 31))
     return fail(DLLM_ERR_UNSUPPORTED, "%s: %d KV heads", name, Hkv);
-  if (cache_rows > ((int64_t)1 << 31)) return fail(DLLM_ERR_UNSUPPORTED, "%s: more than 2^31 cache rows", name);
-  if (cache_rows % kPageRows && (paged || cache_type == DLLM_CACHE_FP8))
-    return fail(DLLM_ERR_INVALID_ARG, "%s: the cache must be whole 256-row pages", name);
-  if (max_cached > 0 && cache_rows > 0) {
-    if (!k_cache || !v_cache || !table || (paged && max_pages == 0))
-      return fail(DLLM_ERR_INVALID_ARG, "%s: null cache / %s", name, paged ? "page table" : "slots");
+  if (max_cached > 0 && num_pages > 0) {
+    if (!k_cache || !v_cache || !page_table || max_pages == 0)
+      return fail(DLLM_ERR_INVALID_ARG, "%s: null cache / page table", name);
     if (!aligned16(k_cache) || !aligned16(v_cache))
       return fail(DLLM_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", name);
   }
@@ -1052,14 +1110,14 @@ static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dll
   a.q = q; a.k = k; a.v = v; a.o = o;
   a.kc = reinterpret_cast<const uint8_t*>(k_cache);
   a.vc = reinterpret_cast<const uint8_t*>(v_cache);
-  a.cu = cu; a.seg_ids = seg_ids; a.table = table; a.lens = lens;
+  a.cu = cu; a.seg_ids = seg_ids; a.table = page_table; a.lens = cached_len;
   a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.o_stride = o_stride;
-  a.cache_rows = cache_rows;
+  a.cache_rows = (int64_t)num_pages * kPageRows;
   a.max_pages = max_pages; a.max_q = max_q; a.max_cached = max_cached;
   a.n_seg = n_seg; a.Hkv = Hkv; a.g = Hq / Hkv;
   a.mask_block = mask_block;
   a.scale_log2 = softmax_scale * kLog2e;
-  const ChunkPlan p = chunk_plan(paged, n_seg, max_q, max_cached, Hq, Hkv);
+  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
   a.bm = p.bm; a.tile_form = p.tile_form;
   a.mtiles = p.mtiles; a.n_split = p.n_split; a.tiles_per_split = p.tiles_per_split;
   const size_t need = chunk_ws(p, n_seg, Hkv);
@@ -1085,55 +1143,25 @@ static int chunk_fwd(const char* name, bool paged, const dllm_bf16* q, const dll
     kern<<<dim3(grid), dim3(threads), lds_bytes, st>>>(a);
     return check_launch(name);
   };
-  auto rows_form = [&](auto nb) {
-    constexpr int NB = decltype(nb)::value;
-    return fp8 ? (paged ? chunk_rows_kernel<NB, true, true> : chunk_rows_kernel<NB, true, false>)
-               : (paged ? chunk_rows_kernel<NB, false, true> : chunk_rows_kernel<NB, false, false>);
-  };
   constexpr int kTileLds = 2 * 2 * kBigTile * 256;
   if (p.tile_form && p.nw == 8)
     rc = launch(fp8 ? chunk_tile_kernel<8, true> : chunk_tile_kernel<8, false>, 512, kTileLds);
   else if (p.tile_form)
     rc = launch(fp8 ? chunk_tile_kernel<4, true> : chunk_tile_kernel<4, false>, 256, kTileLds);
   else if (p.nb == 1)
-    rc = launch(rows_form(std::integral_constant<int, 1>()), 256, rows_lds(1));
+    rc = fp8 ? launch(chunk_rows_kernel<1, true>, 256, rows_lds<1, true>())
+             : launch(chunk_rows_kernel<1, false>, 256, rows_lds<1, false>());
   else
-    rc = launch(rows_form(std::integral_constant<int, 2>()), 256, rows_lds(2));
+    rc = fp8 ? launch(chunk_rows_kernel<2, true>, 256, rows_lds<2, true>())
+             : launch(chunk_rows_kernel<2, false>, 256, rows_lds<2, false>());
   if (rc) return rc;
   if (p.n_split > 1) {
     const int64_t rows = (int64_t)n_seg * Hkv * p.mtiles * p.bm;
     if (p.n_split > 8)
-      chunk_combine_kernel<8><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a, paged);
+      chunk_combine_kernel<8><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a);
     else
-      chunk_combine_kernel<1><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a, paged);
+      chunk_combine_kernel<1><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a);
     rc = check_launch(name);
   }
   return rc;
-}
-
-extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
-                                         const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
-                                         const void* k_cache, const void* v_cache, int cache_type, int num_pages,
-                                         const int32_t* page_table, int max_pages, const int32_t* cached_len,
-                                         int mask_block, int Hq, int Hkv, int D, int64_t q_stride_tok,
-                                         int64_t k_stride_tok, int64_t v_stride_tok, int64_t o_stride_tok,
-                                         float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* name = "dllm_attn_chunk_paged_fwd";
-  if (num_pages < 0 || num_pages > (1 << 23)) return fail(DLLM_ERR_INVALID_ARG, "%s: %d pages", name, num_pages);
-  return chunk_fwd(name, true, q, k, v, o, cu, seg_ids, n_seg, max_q, max_cached, k_cache, v_cache, cache_type,
-                   (int64_t)num_pages * kPageRows, page_table, max_pages, cached_len, mask_block, Hq, Hkv, D,
-                   q_stride_tok, k_stride_tok, v_stride_tok, o_stride_tok, softmax_scale, workspace, workspace_bytes,
-                   stream);
-}
-
-extern "C" int dllm_attn_chunk_slots_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
-                                         const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
-                                         const void* k_cache, const void* v_cache, int cache_type, int64_t cache_slots,
-                                         const int32_t* slots, const int32_t* slot_off, int mask_block, int Hq, int Hkv,
-                                         int D, int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
-                                         int64_t o_stride_tok, float softmax_scale, void* workspace,
-                                         size_t workspace_bytes, void* stream) {
-  return chunk_fwd("dllm_attn_chunk_slots_fwd", false, q, k, v, o, cu, seg_ids, n_seg, max_q, max_cached, k_cache,
-                   v_cache, cache_type, cache_slots, slots, 0, slot_off, mask_block, Hq, Hkv, D, q_stride_tok,
-                   k_stride_tok, v_stride_tok, o_stride_tok, softmax_scale, workspace, workspace_bytes, stream);
 }

@@ -75,11 +75,6 @@ SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I,
          _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
     ),
-    "dllm_attn_chunk_slots_fwd": (
-        _I,
-        [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I64, _P, _P, _I, _I, _I, _I,
-         _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
-    ),
     "dllm_select_kv_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
     "dllm_select_kv_store": (
         _I,
@@ -375,13 +370,6 @@ def attn_chunk_paged_fwd_raw(*args) -> None:
     rc = _lib_now().dllm_attn_chunk_paged_fwd(*args)
     if rc != DLLM_OK:
         _check(rc, "dllm_attn_chunk_paged_fwd")
-
-
-def attn_chunk_slots_fwd_raw(*args) -> None:
-    """dllm_attn_chunk_slots_fwd over device addresses the caller has already checked."""
-    rc = _lib_now().dllm_attn_chunk_slots_fwd(*args)
-    if rc != DLLM_OK:
-        _check(rc, "dllm_attn_chunk_slots_fwd")
 
 
 JOB_COLS = 8  # row0, n_tok, blk_start, blk_len, n_keep, slot_off, head_select, pool_k

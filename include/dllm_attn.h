@@ -243,10 +243,9 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * that a row does not see do not reach it.  Rows of o outside the segments are not
  * written.
  *
- * _paged_fwd: cached row r of segment s is row r % 256 of page page_table[s *
- * max_pages + r / 256], n = cached_len[s].  _slots_fwd: it is cache slot
- * slots[slot_off[s] + r], n = slot_off[s+1] - slot_off[s].  A row whose page or slot is
- * outside the cache (or whose page index is >= max_pages) is left out of the softmax.
+ * Cached row r of segment s is row r % 256 of page page_table[s * max_pages + r / 256],
+ * n = cached_len[s].  A row whose page is outside the cache (or whose page index is >=
+ * max_pages) is left out of the softmax.
  * max_q and max_cached must bound L and n of every segment: longer segments are
  * cut there.  D must be 128, Hq a multiple of Hkv, softmax_scale positive; pointers are
  * 16-byte aligned, token strides multiples of 8 elements, and a segment's new rows span
@@ -268,12 +267,6 @@ int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm
                               int Hq, int Hkv, int D, int64_t q_stride_tok, int64_t k_stride_tok,
                               int64_t v_stride_tok, int64_t o_stride_tok, float softmax_scale, void* workspace,
                               size_t workspace_bytes, void* stream);
-int dllm_attn_chunk_slots_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
-                              const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
-                              const void* k_cache, const void* v_cache, int cache_type, int64_t cache_slots,
-                              const int32_t* slots, const int32_t* slot_off, int mask_block, int Hq, int Hkv, int D,
-                              int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok, int64_t o_stride_tok,
-                              float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * K5 / K6 -- sparse KV selection fused with the KV-cache scatter (mode 1 /

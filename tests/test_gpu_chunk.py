@@ -224,44 +224,27 @@ def test_rows_outside_the_segments_stay(dev):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
-@pytest.mark.parametrize("lens,cached", [([1, 1], [700, 40]), ([32, 8], [300, 0]), ([150], [600])])
-def test_slot_lists(dev, bits, lens, cached):
-    """The slot-list form over rows in any order, some of them outside the cache, and a
-    subset of a packed batch by segment ids."""
+@pytest.mark.parametrize("lens,cached", [([1, 1, 9], [700, 40, 5]), ([32, 3, 8], [300, 9, 0]), ([150, 2, 70], [600, 8, 20])])
+def test_some_sequences_of_a_packed_batch(dev, bits, lens, cached):
+    """Segment ids: the sequences of a launch in another order, one of them not in it."""
     b = Batch(dev, lens, cached, 4, 2, bits, seed=12)
-    g = torch.Generator().manual_seed(1)
-    rows = b.pages * 256
-    ids = list(range(len(lens)))[::-1]
-    lists = {}
-    for i in ids:
-        s = torch.randperm(rows, generator=g)[:cached[i]].to(torch.int64)
-        if cached[i] > 20:
-            s[7], s[cached[i] - 1] = -1, rows
-        lists[i] = s
-    off = np.concatenate([[0], np.cumsum([cached[i] for i in ids])])
-    slots = torch.cat([lists[i] for i in ids] + [torch.zeros(1, dtype=torch.int64)]).to(torch.int32).to(dev)
+    ids = [2, 0]
+    plan = ChunkPlan([lens[i] for i in ids], [cached[i] for i in ids], [b.tables[i] for i in ids], dev)
     cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device=dev)
-    seg, offs = torch.tensor(ids, dtype=torch.int32, device=dev), torch.tensor(off, dtype=torch.int32, device=dev)
+    seg = torch.tensor(ids, dtype=torch.int32, device=dev)
     q, k, v = b.q.to(dev), b.k.to(dev), b.v.to(dev)
-    o = torch.empty_like(q)
-    max_q, max_c = max(lens), max(cached)
-    ws = torch.empty(max(16, _capi.chunk_workspace_size(len(ids), max_q, max_c, 4, 2, 128)), dtype=torch.uint8, device=dev)
+    o = torch.full_like(q, 5.0)
+    ws = torch.empty(max(16, _capi.chunk_workspace_size(2, plan.max_q, plan.max_cached, 4, 2, 128)), dtype=torch.uint8,
+                     device=dev)
     kind = _capi.CACHE_FP8 if bits == 8 else _capi.CACHE_BF16
-    _capi.attn_chunk_slots_fwd_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu.data_ptr(), seg.data_ptr(),
-                                   len(ids), max_q, max_c, b.kc.data_ptr(), b.vc.data_ptr(), kind, rows,
-                                   slots.data_ptr(), offs.data_ptr(), 0, 4, 2, 128, 512, 256, 256, 512, SCALE,
-                                   ws.data_ptr(), ws.numel(), _capi._stream(dev))
-    r0 = 0
-    for i, L in enumerate(lens):
-        s = lists[i].numpy()
-        s = s[(s >= 0) & (s < rows)]
-        if bits == 8:
-            kc, vc = quant.load(b.kc.cpu().numpy(), s), quant.load(b.vc.cpu().numpy(), s)
-        else:
-            kc, vc = _np(b.kc.view(-1, 2, 128))[s], _np(b.vc.view(-1, 2, 128))[s]
-        x = [_np(t[r0:r0 + L]) for t in (b.q, b.k, b.v)]
-        check(o[r0:r0 + L], *chunk.attend(*x, kc, vc, SCALE), L + cached[i], f"sequence {i}")
-        r0 += L
+    _, n, tables = plan._args
+    _capi.attn_chunk_paged_fwd_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu.data_ptr(), seg.data_ptr(),
+                                   2, plan.max_q, plan.max_cached, b.kc.data_ptr(), b.vc.data_ptr(), kind, b.pages,
+                                   tables, plan.max_pages, n, 0, 4, 2, 128, 512, 256, 256, 512, SCALE, ws.data_ptr(),
+                                   ws.numel(), _capi._stream(dev))
+    assert (o[lens[0]:lens[0] + lens[1]] == 5).all()
+    o[lens[0]:lens[0] + lens[1]] = b.run(0).view(-1, 4, 128)[lens[0]:lens[0] + lens[1]]
+    b.verify(o, 0)
 
 
 @pytest.mark.parametrize("bits", [8, 16])
