@@ -20,6 +20,7 @@
 #include "attn_tile.h"
 #include "quant.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace dllm {
@@ -31,40 +32,23 @@ struct ChunkArgs {
   uint16_t* o;
   const uint8_t* kc;      // cache: records (8-bit) or bf16 rows [pages * 256][Hkv][128]
   const uint8_t* vc;
-  const int32_t* cu;
-  const int32_t* seg_ids;
-  const int32_t* table;   // page table [n_seg][max_pages]
-  const int32_t* lens;    // cached lengths [n_seg]
   float* ws;
   int64_t q_stride, k_stride, v_stride, o_stride;
   int64_t cache_rows;     // rows of the cache, whole pages
-  int max_pages, max_q, max_cached;
-  int n_seg, Hkv, g, mtiles, n_split, tiles_per_split;
+  int max_q, max_cached;
+  int g;
   int mask_block;
-  int bm;                 // M rows of a workgroup
-  int tile_form;          // chunk_tile_kernel (else chunk_rows_kernel)
-  int logical_blocks, xcd_chunk;
   float scale_log2;
 };
 
-constexpr int kTileKeys = 32;   // keys of a wavefront's tile
+constexpr int kTileKeys = 32;   // keys of a wavefront's tile (chunk_rows_kernel)
+constexpr int kBigTile = 64;    // keys of a workgroup's tile (chunk_tile_kernel)
 constexpr int kMaxSplitTiles = 62 * kPageRows / kTileKeys;  // chunk_rows_kernel: at most 63 pages, one a lane
 
-// Segment s: new rows' first row and count, cached rows.
+// A segment: new rows' first row and count, cached rows.
 struct Segment {
   int row0, len, cached;
 };
-__device__ __forceinline__ Segment segment(const ChunkArgs& a, int s) {
-  Segment g;
-  const int id = a.seg_ids ? a.seg_ids[s] : s;
-  g.row0 = a.cu[id];
-  g.len = a.cu[id + 1] - g.row0;
-  g.cached = a.lens[s];
-  // what the launch was sized for
-  g.len = min(max(g.len, 0), a.max_q);
-  g.cached = min(max(g.cached, 0), a.max_cached);
-  return g;
-}
 
 // New rows that new row t sees.
 __device__ __forceinline__ int visible(const Segment& g, int t, int mask_block) {
@@ -73,20 +57,68 @@ __device__ __forceinline__ int visible(const Segment& g, int t, int mask_block) 
   return (int)min((int64_t)g.len, end);
 }
 
-constexpr int kBigTile = 64;    // keys of chunk_tile_kernel's tiles
-
-// Splits that hold keys of M tile mt (at least one).  chunk_rows_kernel deals the
-// cached tiles alone, the new rows belonging to the last split; chunk_tile_kernel
-// the cached tiles and those of the new rows that the M tile sees.
-__device__ __forceinline__ int splits_of(const ChunkArgs& a, const Segment& g, int mt) {
+// Splits that hold keys of the M tile whose last token is `last` (at least one).  The
+// rows form deals the cached tiles alone, the new rows belonging to the last split; the
+// tile form the cached tiles and those of the new rows that the M tile sees.
+template <bool TILE>
+__device__ __forceinline__ int splits_of(const ChunkArgs& a, int tiles_per_split, const Segment& g, int last) {
   int tiles;
-  if (a.tile_form) {
-    const int last = min((mt + 1) * a.bm, g.len * a.g) - 1;
-    tiles = (g.cached + kBigTile - 1) / kBigTile + (visible(g, last / a.g, a.mask_block) + kBigTile - 1) / kBigTile;
-  } else {
+  if (TILE)
+    tiles = (g.cached + kBigTile - 1) / kBigTile + (visible(g, last, a.mask_block) + kBigTile - 1) / kBigTile;
+  else
     tiles = (g.cached + kTileKeys - 1) / kTileKeys;
-  }
-  return max(1, (tiles + a.tiles_per_split - 1) / a.tiles_per_split);
+  return max(1, (int)((uint32_t)(tiles + tiles_per_split - 1) / (uint32_t)tiles_per_split));
+}
+
+// The tables and the launch's geometry come as leading scalar arguments (14 dwords): the
+// library is built with kernel argument preloading, so they are in SGPRs when a wave
+// starts instead of a load away -- a load that queues behind the keys that
+// workgroups which started earlier are already streaming.
+#define CHUNK_PARAMS                                                                                            \
+  const int32_t *__restrict__ cu, const int32_t *__restrict__ seg_ids, const int32_t *__restrict__ lens,       \
+      const int32_t *__restrict__ table, int chunk_pages, int logical_blocks, int mtiles, int max_split,       \
+      int tiles_per_split, int Hkv, ChunkArgs a
+// chunk_pages: the XCD interleave's chunk (1 .. 16) + 32 x the page table's row length.
+
+// A workgroup's work: one M tile and split of one (segment, KV head), M tiles fastest.
+// Every segment has max_split splits; those past its end stop at once.
+// (Numbering only the work that exists, by a prefix sum over the segments in every
+// workgroup, made the first loads wait for another one: 32 ragged single tokens, 28/4
+// heads, 25.4 -> 26 to 30 us.)
+struct Work {
+  int s, hkv, split, mt;
+};
+__device__ __forceinline__ Work work_of(int L, int mtiles, int max_split, int Hkv) {
+  Work w;
+  uint32_t r = (uint32_t)L;
+  w.mt = (int)(r % (uint32_t)mtiles);
+  r /= (uint32_t)mtiles;
+  w.split = (int)(r % (uint32_t)max_split);
+  r /= (uint32_t)max_split;
+  w.hkv = (int)(r % (uint32_t)Hkv);
+  w.s = (int)(r / (uint32_t)Hkv);
+  return w;
+}
+__device__ __forceinline__ Segment segment(const ChunkArgs& a, const int32_t* cu, const int32_t* seg_ids,
+                                           const int32_t* lens, int s) {
+  Segment g;
+  const int id = seg_ids ? seg_ids[s] : s;
+  g.row0 = cu[id];
+  // no more than the launch was sized for
+  g.len = min(max(cu[id + 1] - g.row0, 0), a.max_q);
+  g.cached = min(max(lens[s], 0), a.max_cached);
+  return g;
+}
+
+// The part of M row `row` (of BM) of workgroup L: 128 floats, and the row's m and l
+// behind all parts.
+template <int BM>
+__device__ __forceinline__ float* part_o(const ChunkArgs& a, int L, int row) {
+  return a.ws + ((int64_t)L * BM + row) * HD;
+}
+template <int BM>
+__device__ __forceinline__ float* part_ml(const ChunkArgs& a, int logical_blocks, int L, int row) {
+  return a.ws + (int64_t)logical_blocks * BM * HD + ((int64_t)L * BM + row) * 2;
 }
 
 __device__ __forceinline__ float row_max4(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -267,42 +299,39 @@ __device__ __forceinline__ void v_rows(const uint8_t* vb_ptr, u32x2_t (&r)[16]) 
 }
 
 template <int NB, bool FP8>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(CHUNK_PARAMS) {
   using T = RowsTile<FP8>;
   constexpr int BM = 16 * NB;
   constexpr int PARK = park_floats(NB);
   extern __shared__ __attribute__((aligned(16))) float lds[];  // rows_lds() bytes
-  const int L = xcd_remap(blockIdx.x, a.xcd_chunk);
-  if (L >= a.logical_blocks) return;
-  int r = L;
-  const int mt = r % a.mtiles;
-  r /= a.mtiles;
-  const int split = r % a.n_split;
-  r /= a.n_split;
-  const int hkv = r % a.Hkv;
-  const int s = r / a.Hkv;
-  const Segment sg = segment(a, s);
+  const int L = xcd_remap(blockIdx.x, chunk_pages & 31);
+  if (L >= logical_blocks) return;
+  const int max_pages = chunk_pages >> 5;
+  const Work wk = work_of(L, mtiles, max_split, Hkv);
+  const int s = wk.s, hkv = wk.hkv, split = wk.split;
+  const int lane = threadIdx.x & 63;
+  const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
+  const int t_begin = split * tiles_per_split;
+  // Page ids of the split, one a lane (a split spans at most 63): a tile's loads
+  // then wait for no load of their own.  Their address needs no other load either.
+  const int pg0 = t_begin * kTileKeys / kPageRows;
+  const int page_reg = n_pages > 0 && max_pages > 0
+                           ? table[(int64_t)s * max_pages + min(pg0 + lane, max_pages - 1)] : -1;
+  const Segment sg = segment(a, cu, seg_ids, lens, s);
   const int g = a.g;
   const int M = sg.len * g;
-  const int m_base = mt * BM;
+  const int m_base = wk.mt * BM;
   if (m_base >= M) return;
-  const int ns = splits_of(a, sg, mt);
+  const int ns = splits_of<false>(a, tiles_per_split, sg, sg.len - 1);
   if (split >= ns) return;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lane = tid & 63;
   const int col = lane & 15, g4 = lane >> 4;
   uint8_t* const my = reinterpret_cast<uint8_t*>(lds) + wave * 2 * T::kStage;
 
   const int tiles = (sg.cached + kTileKeys - 1) / kTileKeys;
-  const int t_begin = split * a.tiles_per_split;
-  const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
-  const int t_end = n_pages ? min(tiles, t_begin + a.tiles_per_split) : t_begin;  // no cache: nothing to read
-  const uint32_t bf_row = (uint32_t)(a.Hkv * HD * 2);
-  // Page ids of the split, one a lane (a split spans at most 63): a tile's loads
-  // then wait for no load of their own.
-  const int pg0 = t_begin * kTileKeys / kPageRows;
-  const int page_reg = t_begin < t_end ? a.table[(int64_t)s * a.max_pages + min(pg0 + lane, a.max_pages - 1)] : -1;
+  const int t_end = n_pages ? min(tiles, t_begin + tiles_per_split) : t_begin;  // no cache: nothing to read
+  const uint32_t bf_row = (uint32_t)(Hkv * HD * 2);
 
   // ---- Q^T operands and the rows' limits ------------------------------------
   bf16x8_t qf[NB][4];
@@ -329,7 +358,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   auto page_of = [&](int t) -> int {
     const int pg = t * kTileKeys / kPageRows;
     const int pid = __builtin_amdgcn_readlane(page_reg, (pg - pg0) & 63);
-    return pg < a.max_pages && (uint32_t)pid < n_pages ? pid : -1;
+    return pg < max_pages && (uint32_t)pid < n_pages ? pid : -1;
   };
   // DMA of cached tile t into a stage; rows past the cached length, and all rows of a
   // page outside the cache, arrive as zeros through the buffer's bound.
@@ -338,7 +367,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int row0 = t * kTileKeys & (kPageRows - 1);
     const int rows = pid < 0 ? 0 : min(sg.cached - t * kTileKeys, kTileKeys);
     if constexpr (FP8) {
-      const int64_t rec = ((int64_t)max(pid, 0) * a.Hkv + hkv) * kRecord;
+      const int64_t rec = ((int64_t)max(pid, 0) * Hkv + hkv) * kRecord;
       const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
       const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.vc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
       // lane l of instruction j: row 8 j + l / 8, physical chunk l % 8
@@ -473,12 +502,87 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   };
 
+  // ---- new rows (the last split's), bf16 from k / v ------------------------------
+  // Before the cached tiles: their loads are among the first, beside the first tile's DMA.
+  const int n = max(0, (t_end - t_begin - wave + 3) >> 2);  // this wavefront's cached tiles
+  const int first = t_begin + wave;
+  bool fixed = false, started = false;
+  const uint32_t vS = (uint32_t)(a.v_stride * 2), vb = (uint32_t)(sg.len - 1) * vS + HD * 2;
+  const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD, vb);
+  const int turn = max(t_end - t_begin, 0);
+  if (split == ns - 1) {
+    const uint32_t kS = (uint32_t)(a.k_stride * 2), kb = (uint32_t)(sg.len - 1) * kS + HD * 2;
+    const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.k + (int64_t)sg.row0 * a.k_stride + hkv * HD, kb);
+    // the furthest new row that any of this workgroup's rows sees
+    const int last = min(m_base + BM, M) - 1;
+    const int see = visible(sg, last / g, a.mask_block);
+    const int new_tiles = (see + kTileKeys - 1) / kTileKeys;
+    for (int t = (wave - turn) & 3; t < new_tiles; t += 4) {
+      bf16x8_t kx[2][4];
+      u32x4_t vx[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t row = (uint32_t)(t * kTileKeys + 16 * u + col);
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const uint32_t off = FP8 ? (uint32_t)((k4 >> 1) * 128 + g4 * 32 + (k4 & 1) * 16) : (uint32_t)(k4 * 64 + g4 * 16);
+          kx[u][k4] = as_bf16x8(bload(krs, row < (uint32_t)sg.len ? row * kS + off : kb, 0u));
+          vx[u][k4] = bload(vrs, row < (uint32_t)sg.len ? row * vS + (uint32_t)(k4 * 64 + g4 * 16) : vb, 0u);
+        }
+      }
+      if (!started && n > 0) issue(my, first);
+      started = true;
+      // A NaN or infinity in a V row that some M row does not see would reach that row
+      // as 0 * V.  Such elements (rare) are multiplied as zeros and added at the end
+      // to the rows that see them.
+      bool odd = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) odd |= has_nonfinite(vx[u][p]);
+      const bool fix = __builtin_amdgcn_ballot_w64(odd) != 0;
+      if (fix) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) vx[u][p] = finite_part(vx[u][p]);
+      }
+      // V in bf16, as a tile of bf16 rows, where the second stage will be
+      wave_lds_fence();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int row = 16 * u + col;
+          *reinterpret_cast<u32x4_t*>(my + T::kStage + row * 256 + (((4 * p + g4) ^ (2 * (row & 7))) * 16)) = vx[u][p];
+        }
+      wave_lds_fence();
+      auto keys = [&](int u, bf16x8_t (&kf)[4]) {
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) kf[k4] = kx[u][k4];
+      };
+      auto hide = [&](f32x4_t (&sc)[NB][2]) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (t * kTileKeys + 16 * u + 4 * g4 + i >= lim[b]) sc[b][u][i] = -INFINITY;
+      };
+      const float one[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+      bf16x8_t pf[NB];
+      scores(keys, hide, one, std::false_type(), pf);
+      add_bf16_rows(my + T::kStage, pf);
+      fixed |= fix;
+    }
+  }
+
   // ---- cached tiles: this wavefront takes every fourth, two in flight --------------
   {
-    const int n = max(0, (t_end - t_begin - wave + 3) >> 2);  // this wavefront's tiles
-    const int first = t_begin + wave;
     asm volatile("" ::: "memory");  // the page ids and q stay the oldest operations
-    if (n > 0) issue(my, first);
+    wave_lds_fence();               // the new rows' V has been read
+    if (!started && n > 0) issue(my, first);
     if (n > 1) issue(my + T::kStage, first + 4);
     // q has landed, the tiles may be in flight
     if (n > 1)
@@ -499,88 +603,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   }
 
-  // ---- new rows (the last split's), bf16 from k / v ------------------------------
-  if (split == ns - 1) {
-    const uint32_t kS = (uint32_t)(a.k_stride * 2), vS = (uint32_t)(a.v_stride * 2);
-    const uint32_t kb = (uint32_t)(sg.len - 1) * kS + HD * 2, vb = (uint32_t)(sg.len - 1) * vS + HD * 2;
-    const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.k + (int64_t)sg.row0 * a.k_stride + hkv * HD, kb);
-    const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD, vb);
-    // the furthest new row that any of this workgroup's rows sees
-    const int last = min(m_base + BM, M) - 1;
-    const int see = visible(sg, last / g, a.mask_block);
-    const int new_tiles = (see + kTileKeys - 1) / kTileKeys;
-    const int turn = max(t_end - t_begin, 0);
-    for (int t = (wave - turn) & 3; t < new_tiles; t += 4) {
-      bf16x8_t kx[2][4];
-      u32x4_t vx[2][4];
+  if (fixed) {
+#pragma unroll 1
+    for (int j = 0; j < sg.len; ++j) {
+      if ((((j / kTileKeys) + turn - wave) & 3) != 0) continue;  // a key of another wavefront
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t row = (uint32_t)(t * kTileKeys + 16 * u + col);
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const uint32_t off = FP8 ? (uint32_t)((k4 >> 1) * 128 + g4 * 32 + (k4 & 1) * 16) : (uint32_t)(k4 * 64 + g4 * 16);
-          kx[u][k4] = as_bf16x8(bload(krs, row < (uint32_t)sg.len ? row * kS + off : kb, 0u));
-          vx[u][k4] = bload(vrs, row < (uint32_t)sg.len ? row * vS + (uint32_t)(k4 * 64 + g4 * 16) : vb, 0u);
-        }
-      }
-      // A NaN or infinity in a V row that some M row does not see would reach that row
-      // as 0 * V.  Such elements (rare) are multiplied as zeros and added afterwards
-      // to the rows that see them.
-      bool odd = false;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int p = 0; p < 4; ++p) odd |= has_nonfinite(vx[u][p]);
-      const bool fix = __builtin_amdgcn_ballot_w64(odd) != 0;
-      if (fix) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int p = 0; p < 4; ++p) vx[u][p] = finite_part(vx[u][p]);
-      }
-      // V in bf16, as a tile of bf16 rows
-      wave_lds_fence();
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int row = 16 * u + col;
-          *reinterpret_cast<u32x4_t*>(my + row * 256 + (((4 * p + g4) ^ (2 * (row & 7))) * 16)) = vx[u][p];
-        }
-      wave_lds_fence();
-      auto keys = [&](int u, bf16x8_t (&kf)[4]) {
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) kf[k4] = kx[u][k4];
-      };
-      auto hide = [&](f32x4_t (&sc)[NB][2]) {
+      for (int dt = 0; dt < 8; ++dt) {
+        const u32x2_t w = __builtin_bit_cast(
+            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(vrs, (int)((uint32_t)j * vS + (uint32_t)(32 * dt + 8 * g4)), 0, 0));
 #pragma unroll
         for (int b = 0; b < NB; ++b)
+          if (j < lim[b]) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (t * kTileKeys + 16 * u + 4 * g4 + i >= lim[b]) sc[b][u][i] = -INFINITY;
-      };
-      const float one[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-      bf16x8_t pf[NB];
-      scores(keys, hide, one, std::false_type(), pf);
-      add_bf16_rows(my, pf);
-      if (fix) {
-        const int end = min((t + 1) * kTileKeys, sg.len);
-        for (int j = t * kTileKeys; j < end; ++j)
-#pragma unroll
-          for (int dt = 0; dt < 8; ++dt) {
-            const u32x2_t w = __builtin_bit_cast(
-                u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(vrs, (int)((uint32_t)j * vS + (uint32_t)(32 * dt + 8 * g4)), 0, 0));
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-              if (j < lim[b]) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-                  if ((h & 0x7f80u) == 0x7f80u) st.o[b][dt][i] += bf16_bits_to_f32(h);
-                }
-              }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+              if ((h & 0x7f80u) == 0x7f80u) st.o[b][dt][i] += bf16_bits_to_f32(h);
+            }
           }
       }
     }
@@ -619,7 +657,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   const int tok = m / g, head = hkv * g + (m - tok * g);
   const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-  const int64_t rec = ((((int64_t)s * a.Hkv + hkv) * a.mtiles + mt) * a.n_split + split) * BM + row;
 #pragma unroll
   for (int j = 0; j < DPT / 4; ++j) {
     const int d = d0 + 4 * TPR * j;
@@ -635,49 +672,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const u32x2_t w2 = {cvt_pk_bf16(acc[0] * inv, acc[1] * inv), cvt_pk_bf16(acc[2] * inv, acc[3] * inv)};
       *reinterpret_cast<u32x2_t*>(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + head * HD + d) = w2;
     } else {
-      *reinterpret_cast<f32x4_t*>(a.ws + rec * HD + d) = acc;
+      *reinterpret_cast<f32x4_t*>(part_o<BM>(a, L, row) + d) = acc;
     }
   }
   if (ns > 1 && d0 == 0) {
-    float* pml = a.ws + (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * BM * HD + rec * 2;
+    float* const pml = part_ml<BM>(a, logical_blocks, L, row);
     pml[0] = mx;
     pml[1] = lsum;
   }
 }
 
 // ---------------------------------------------------------------------------
-// Many M rows: NW wavefronts of 32 M rows share 64-key tiles of K and V in LDS
+// Many M rows: four wavefronts of 32 M rows share 64-key tiles of K and V in LDS
 // (bf16, the swizzled layout of attn_tile.h), two stages.  The tile sequence is the
-// cached rows' tiles, then those of the new rows.  While tile t is computed, tile t + 1
-// is on its way: bf16 rows by DMA into the other stage; 8-bit rows into registers
-// (16 bytes a thread and matrix with eight wavefronts), converted and written to the
-// other stage after the products -- once per workgroup, not once per wavefront.
-template <int NW, bool FP8>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_tile_kernel(ChunkArgs a) {
+// cached rows' tiles, then those of the new rows.  While a tile is computed, the next one
+// is on its way: bf16 rows by DMA into the other stage; 8-bit rows into registers (32
+// bytes a thread and matrix), converted and written to the other stage after the
+// products -- once per workgroup, not once per wavefront.  Two workgroups fit a CU, so
+// that one computes while the other one waits at its barrier (eight wavefronts in one
+// workgroup: 2048 rows behind 6144 cached, 32 heads, 381 against 333 us).
+constexpr int kTileRows = 128;
+constexpr int kTileStage = 2 * kBigTile * 256;
+template <bool FP8>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_tile_kernel(CHUNK_PARAMS) {
   constexpr int TK = kBigTile;
-  constexpr int STAGE = 2 * TK * 256;
-  constexpr int BM = 32 * NW;
-  constexpr int DMA = TK * 256 / 1024 / NW;  // DMA instructions of one matrix, tile and wavefront
-  constexpr int PER = TK * 8 / (64 * NW);    // 8-bit rows: 16-byte pieces of one matrix and thread
+  constexpr int BM = kTileRows;
+  constexpr int DMA = TK * 256 / 1024 / 4;   // DMA instructions of one matrix, tile and wavefront
+  constexpr int PER = TK * 8 / 256;          // 8-bit rows: 16-byte pieces of one matrix and thread
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
-  uint8_t* const lds = reinterpret_cast<uint8_t*>(lds_f);
-  const int L = xcd_remap(blockIdx.x, a.xcd_chunk);
-  if (L >= a.logical_blocks) return;
-  int r = L;
-  // the last M tiles first: with a causal mask they see the most keys
-  const int mt = a.mtiles - 1 - r % a.mtiles;
-  r /= a.mtiles;
-  const int split = r % a.n_split;
-  r /= a.n_split;
-  const int hkv = r % a.Hkv;
-  const int s = r / a.Hkv;
-  const Segment sg = segment(a, s);
+  uint8_t* const lds = reinterpret_cast<uint8_t*>(lds_f);  // two stages
+  const int L = xcd_remap(blockIdx.x, chunk_pages & 31);
+  if (L >= logical_blocks) return;
+  const int max_pages = chunk_pages >> 5;
+  const Work wk = work_of(L, mtiles, max_split, Hkv);
+  const int s = wk.s, hkv = wk.hkv;
+  const Segment sg = segment(a, cu, seg_ids, lens, s);
   const int g = a.g;
   const int M = sg.len * g;
-  const int m_base = mt * BM;
+  const int m_base = (mtiles - 1 - wk.mt) * BM;  // the last M tiles first: with a causal mask they see the most keys
   if (m_base >= M) return;
-  const int ns = splits_of(a, sg, mt);
-  if (split >= ns) return;
+  const int tok_first = m_base / g, tok_last = (min(m_base + BM, M) - 1) / g;
+  const int ns = splits_of<true>(a, tiles_per_split, sg, tok_last);
+  if (wk.split >= ns) return;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
@@ -685,24 +721,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int rl = lane >> 4, P = lane & 15;
 
   const int t_cached = (sg.cached + TK - 1) / TK;
-  const int see_last = visible(sg, (min(m_base + BM, M) - 1) / g, a.mask_block);
-  const int see_first = visible(sg, m_base / g, a.mask_block);
-  const int t_all = t_cached + (see_last + TK - 1) / TK;
-  const int t0 = split * a.tiles_per_split, t1 = min(t_all, t0 + a.tiles_per_split);
+  const int see_first = visible(sg, tok_first, a.mask_block);
+  const int t_all = t_cached + (visible(sg, tok_last, a.mask_block) + TK - 1) / TK;
+  const int t0 = wk.split * tiles_per_split, t1 = min(t_all, t0 + tiles_per_split);
+  const int c1 = min(t1, t_cached);          // cached tiles t0 .. c1 - 1, then new ones
   const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
-  const int32_t* const table = a.table + (int64_t)s * a.max_pages;
-  const uint32_t bf_row = (uint32_t)(a.Hkv * HD * 2);
-  const uint32_t kS = (uint32_t)(a.k_stride * 2), vS = (uint32_t)(a.v_stride * 2);
-  const uint16_t* const knew = a.k + (int64_t)sg.row0 * a.k_stride + hkv * HD;
-  const uint16_t* const vnew = a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD;
+  const int32_t* const pages = table + (int64_t)s * max_pages;
+  const uint32_t bf_row = (uint32_t)(Hkv * HD * 2);
 
-  // page of cached tile t, or -1 (then its rows are left out)
-  auto page_of = [&](int t) -> int {
-    const int pg = t * TK / kPageRows;
-    if (n_pages == 0 || pg >= a.max_pages) return -1;
-    const int pid = table[pg];
-    return (uint32_t)pid < n_pages ? pid : -1;
+  // Page ids, one a lane: a tile's loads wait for no load of their own (with a scalar
+  // load of the id in every turn the loop took 10 % longer).  Every 64 pages the next ones.
+  int pg0 = t0 * TK / kPageRows, page_reg = -1;
+  auto fetch_pages = [&](int pg) {
+    pg0 = pg;
+    page_reg = pages[min(pg0 + lane, max_pages - 1)];
   };
+  if (n_pages > 0 && t0 < c1) fetch_pages(pg0);
   // `rows` rows (none: zeros) of kb / vb with strides kr / vr to a stage
   auto dma_rows = [&](uint8_t* stage, const void* kb, const void* vb, int rows, uint32_t kr, uint32_t vr) {
     const __amdgpu_buffer_rsrc_t krs = make_rsrc(kb, rows > 0 ? (uint32_t)(rows - 1) * kr + HD * 2 : 0u);
@@ -715,45 +749,50 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       dma16(vrs, stage + TK * 256 + q * 1024, row * vr + (uint32_t)((P ^ (4 * rl)) * 16));
     }
   };
+  auto issue_new = [&](uint8_t* stage, int t) {
+    const int j0 = (t - t_cached) * TK;
+    dma_rows(stage, a.k + (int64_t)(sg.row0 + j0) * a.k_stride + hkv * HD,
+             a.v + (int64_t)(sg.row0 + j0) * a.v_stride + hkv * HD, sg.len - j0, (uint32_t)(a.k_stride * 2),
+             (uint32_t)(a.v_stride * 2));
+  };
   u32x4_t kx[PER], vx[PER];
   uint32_t ksc[PER], vsc[PER];
-  // Tile t on its way to `stage`; true where it goes through registers.
-  auto issue = [&](uint8_t* stage, int t) -> bool {
-    if (t >= t_cached) {
-      const int j0 = (t - t_cached) * TK;
-      dma_rows(stage, knew + (int64_t)j0 * a.k_stride, vnew + (int64_t)j0 * a.v_stride, sg.len - j0, kS, vS);
-      return false;
-    }
-    const int pid = page_of(t);
+  // Cached tile t on its way to `stage` (8-bit rows: to registers); false where its
+  // page is outside the cache.
+  auto issue_cached = [&](uint8_t* stage, int t) -> bool {
+    const int pg = t * TK / kPageRows;
+    if (n_pages > 0 && pg - pg0 >= 64) fetch_pages(pg);
+    int pid = __builtin_amdgcn_readlane(page_reg, pg - pg0);
+    const bool ok = pg < max_pages && (uint32_t)pid < n_pages;
+    pid = ok ? pid : 0;
     const int row0 = t * TK & (kPageRows - 1);
-    const int rows = pid < 0 ? 0 : min(sg.cached - t * TK, TK);
+    const int rows = ok ? min(sg.cached - t * TK, TK) : 0;
     if constexpr (FP8) {
-      const int64_t rec = ((int64_t)max(pid, 0) * a.Hkv + hkv) * kRecord;
-      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
-      const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.vc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
+      const int64_t rec = ((int64_t)pid * Hkv + hkv) * kRecord + row0 * kQuantD;
+      const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec, (uint32_t)rows * kQuantD);
+      const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.vc + rec, (uint32_t)rows * kQuantD);
+      const int64_t sc = ((int64_t)pid * Hkv + hkv) * kRecord + kScaleOff + row0;
+      const __amdgpu_buffer_rsrc_t ksr = make_rsrc(a.kc + sc, (uint32_t)rows), vsr = make_rsrc(a.vc + sc, (uint32_t)rows);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int piece = i * 64 * NW + tid, row = piece >> 3;
+        const int piece = i * 256 + tid;
         kx[i] = bload(krs, (uint32_t)piece * 16u, 0u);
         vx[i] = bload(vrs, (uint32_t)piece * 16u, 0u);
-        ksc[i] = vsc[i] = 127u;
-        if (row < rows) {
-          ksc[i] = a.kc[rec + kScaleOff + row0 + row];
-          vsc[i] = a.vc[rec + kScaleOff + row0 + row];
-        }
+        // a row that does not exist: byte 0, which scales its zeros by 2^-127
+        ksc[i] = __builtin_amdgcn_raw_buffer_load_b8(ksr, piece >> 3, 0, 0);
+        vsc[i] = __builtin_amdgcn_raw_buffer_load_b8(vsr, piece >> 3, 0, 0);
       }
-      return true;
     } else {
-      const int64_t off = ((int64_t)max(pid, 0) * kPageRows + row0) * bf_row + hkv * HD * 2;
+      const int64_t off = ((int64_t)pid * kPageRows + row0) * bf_row + hkv * HD * 2;
       dma_rows(stage, a.kc + off, a.vc + off, rows, bf_row, bf_row);
-      return false;
     }
+    return ok;
   };
   auto put = [&](uint8_t* stage) {
     if constexpr (FP8) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int piece = i * 64 * NW + tid, row = piece >> 3, ch = (piece & 7) * 2;
+        const int piece = i * 256 + tid, row = piece >> 3, ch = (piece & 7) * 2;
         const float ks = scale_of(ksc[i]), vs = scale_of(vsc[i]);
         uint8_t* const kr = stage + row * 256;
         uint8_t* const vr = stage + TK * 256 + row * 256;
@@ -765,7 +804,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   };
 
-  bf16x8_t qf[1][8];
+  bf16x8_t qf[8];
   const int m_lane = m_base + wave * 32 + lrow;
   const int lim = visible(sg, min(m_lane / g, sg.len - 1), a.mask_block);
   {
@@ -776,7 +815,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const bool ok = m_lane < M;
     const uint32_t qoff = (uint32_t)tok * qS + (uint32_t)((hkv * g + m_lane - tok * g) * HD + hl * 8) * 2u;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) qf[0][kk] = as_bf16x8(bload(qrs, ok ? qoff + (uint32_t)kk * 32u : qbytes, 0u));
+    for (int kk = 0; kk < 8; ++kk) qf[kk] = as_bf16x8(bload(qrs, ok ? qoff + (uint32_t)kk * 32u : qbytes, 0u));
   }
   // of this wavefront's rows: the least and the most that any sees
   const int lim_lo = __builtin_amdgcn_readfirstlane(visible(sg, min((m_base + wave * 32) / g, sg.len - 1), a.mask_block));
@@ -790,39 +829,89 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   dense_state_init(st);
   const float c = a.scale_log2;
 
-  if (t0 < t1) {
-    if (issue(lds, t0)) put(lds);
+  // One tile: scores, the keys from `valid` on hidden unless all are seen, softmax, V.
+  // (One instance of it for all tiles: three -- whole cached tiles, the last one, new
+  // ones -- spilled registers.)
+  auto compute = [&](const uint8_t* cur, bool whole, int valid) {
+    f32x16_t sacc[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sacc[b][i] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const bf16x8_t af =
+            as_bf16x8(*reinterpret_cast<const u32x4_t*>(cur + b * 32 * 256 + (ad.kbase ^ (uint32_t)(32 * kk))));
+        sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, qf[kk], sacc[b], 0, 0, 0);
+      }
+    if (!whole) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (b * 32 + 8 * (i >> 2) + 4 * hl + (i & 3) >= valid) sacc[b][i] = -INFINITY;
+    }
+    bf16x8_t pf[4];
+    dense_softmax<2, false>(sacc, st.oacc[0], st.m_run[0], st.l_run[0], st.thr[0], st.neg_m[0], pf, c, TK, 0, hl);
+#pragma unroll
+    for (int cch = 0; cch < 4; ++cch)
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const uint8_t* vp = cur + TK * 256 + (ad.vbase ^ (uint32_t)(64 * db)) + cch * 16 * 256;
+        const u32x2_t x0 = ds_read_tr16(vp), x1 = ds_read_tr16(vp + 8 * 256);
+        st.oacc[0][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(u32x4_t{x0[0], x0[1], x1[0], x1[1]}),
+                                                                 pf[cch], st.oacc[0][db], 0, 0, 0);
+      }
+  };
+  auto stage_of = [&](int t) { return lds + ((t - t0) & 1) * kTileStage; };
+  auto tile_done = [&] {  // every wavefront's part of the next tile has arrived, this one's stage is free
     vm_wait<0>();
     __syncthreads();
+  };
+
+  bool ok = true;  // whether the page of the tile at hand is in the cache
+  if (t0 < c1) {
+    ok = issue_cached(stage_of(t0), t0);
+    put(stage_of(t0));
+    tile_done();
+  } else if (t0 < t1) {
+    issue_new(stage_of(t0), t0);
+    tile_done();
   }
+  bool fixed = false;
   for (int t = t0; t < t1; ++t) {
-    uint8_t* const cur = lds + ((t - t0) & 1) * STAGE;
-    uint8_t* const nxt = lds + ((t - t0 + 1) & 1) * STAGE;
-    const bool more = t + 1 < t1;
-    const bool regs = more && issue(nxt, t + 1);
-    // keys of the tile that this lane's row sees, the least of the wavefront's rows, and the most
-    int valid, lo, hi;
-    bool fix = false;
-    if (t < t_cached) {
-      valid = lo = hi = page_of(t) < 0 ? 0 : min(sg.cached - t * TK, TK);
+    uint8_t* const cur = stage_of(t);
+    uint8_t* const nxt = stage_of(t + 1);
+    bool next_ok = true;
+    if (t + 1 < c1)
+      next_ok = issue_cached(nxt, t + 1);
+    else if (t + 1 < t1)
+      issue_new(nxt, t + 1);
+    bool run = live && ok, whole;
+    int valid;
+    if (t < c1) {
+      valid = sg.cached - t * TK;
+      whole = valid >= TK;
     } else {
       const int j0 = (t - t_cached) * TK;
       valid = lim - j0;
-      lo = lim_lo - j0;
-      hi = lim_hi - j0;
+      whole = lim_lo - j0 >= TK;
+      run = run && lim_hi > j0;
       if (see_first - j0 < TK && see_first < sg.len) {
         // Some M row of the workgroup does not see all of the tile: a NaN or infinity in V
         // would reach it as 0 * V.  Every wavefront looks through the whole tile, so all agree;
-        // such elements are multiplied as zeros and added below to the rows that see them.
+        // such elements are multiplied as zeros and added at the end to the rows that see them.
         bool odd = false;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < TK * 256 / 1024; ++i)
           odd |= has_nonfinite(*reinterpret_cast<const u32x4_t*>(cur + TK * 256 + i * 1024 + lane * 16));
-        fix = __builtin_amdgcn_ballot_w64(odd) != 0;
-        if (fix) {
+        if (__builtin_amdgcn_ballot_w64(odd)) {
+          fixed = true;
           __syncthreads();
 #pragma unroll 1
-          for (int i = wave; i < TK * 256 / 1024; i += NW) {
+          for (int i = wave; i < TK * 256 / 1024; i += 4) {
             u32x4_t* const p = reinterpret_cast<u32x4_t*>(cur + TK * 256 + i * 1024 + lane * 16);
             *p = finite_part(*p);
           }
@@ -830,68 +919,34 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         }
       }
     }
-    if (live && hi > 0) {
-      f32x16_t sacc[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sacc[b][i] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const bf16x8_t af =
-              as_bf16x8(*reinterpret_cast<const u32x4_t*>(cur + b * 32 * 256 + (ad.kbase ^ (uint32_t)(32 * kk))));
-          sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, qf[0][kk], sacc[b], 0, 0, 0);
-        }
-      if (lo < TK) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (b * 32 + 8 * (i >> 2) + 4 * hl + (i & 3) >= valid) sacc[b][i] = -INFINITY;
-      }
-      bf16x8_t pf[4];
-      dense_softmax<2, false>(sacc, st.oacc[0], st.m_run[0], st.l_run[0], st.thr[0], st.neg_m[0], pf, c, TK, 0, hl);
-#pragma unroll
-      for (int cch = 0; cch < 4; ++cch)
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          const uint8_t* vp = cur + TK * 256 + (ad.vbase ^ (uint32_t)(64 * db)) + cch * 16 * 256;
-          const u32x2_t x0 = ds_read_tr16(vp), x1 = ds_read_tr16(vp + 8 * 256);
-          st.oacc[0][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(u32x4_t{x0[0], x0[1], x1[0], x1[1]}),
-                                                                   pf[cch], st.oacc[0][db], 0, 0, 0);
-        }
-      if (fix) {
-        const int j0 = (t - t_cached) * TK, end = min(j0 + TK, sg.len);
+    if (run) compute(cur, whole, valid);
+    if (t + 1 < c1) put(nxt);
+    ok = next_ok;
+    if (t + 1 < t1) tile_done();
+  }
+  if (fixed) {
+    const uint16_t* const vnew = a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD;
+    const int end = min((t1 - t_cached) * TK, sg.len);
 #pragma unroll 1
-        for (int j = j0; j < end; ++j)
+    for (int j = max(t0 - t_cached, 0) * TK; j < end; ++j)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * hl;
-            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vnew + (int64_t)j * a.v_stride + d);
-            if (j < lim) {
+      for (int i = 0; i < 16; ++i) {
+        const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * hl;
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vnew + (int64_t)j * a.v_stride + d);
+        if (j < lim) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-                if ((h & 0x7f80u) == 0x7f80u) st.oacc[0][i >> 2][4 * (i & 3) + e] += bf16_bits_to_f32(h);
-              }
-            }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+            if ((h & 0x7f80u) == 0x7f80u) st.oacc[0][i >> 2][4 * (i & 3) + e] += bf16_bits_to_f32(h);
           }
+        }
       }
-    }
-    if (regs) put(nxt);
-    if (more) {
-      vm_wait<0>();
-      __syncthreads();
-    }
   }
 
   const float l_tot = pair_sum32(st.l_run[0]);
   if (ns > 1) {
     if (m_lane < M) {
-      const int64_t rec = ((((int64_t)s * a.Hkv + hkv) * a.mtiles + mt) * a.n_split + split) * BM + wave * 32 + lrow;
-      float* const po = a.ws + rec * HD;
+      float* const po = part_o<BM>(a, L, wave * 32 + lrow);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * hl;
@@ -900,7 +955,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                     st.oacc[0][i >> 2][4 * (i & 3) + 2], st.oacc[0][i >> 2][4 * (i & 3) + 3]};
       }
       if (hl == 0) {
-        float* const pml = a.ws + (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * BM * HD + rec * 2;
+        float* const pml = part_ml<BM>(a, logical_blocks, L, wave * 32 + lrow);
         pml[0] = st.m_run[0];
         pml[1] = l_tot;
       }
@@ -933,64 +988,59 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // Joins the parts of every (segment, KV head, M row) whose keys were split.  G groups of
 // 32 threads (four d each) share a row's parts, each taking every G-th, so that a row
 // of many parts is one round of loads rather than a long chain (28 rows of 128 parts:
-// 39 us with one group, see the launch).
-template <int G>
-__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a) {
-  constexpr int ROWS = 8 / G;
+// 39 us with one group, 9 with eight).
+template <int BM, bool TILE, int G>
+__global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
+  static_assert(G == 1 || G == 8, "a workgroup holds eight rows or one");
   __shared__ f32x4_t part[G > 1 ? 256 : 1];
-  __shared__ float part_ml[G > 1 ? 16 : 1];
-  const int bm = a.bm;
+  __shared__ float part_s[G > 1 ? 16 : 1];
   const int grp = threadIdx.x >> 5;
-  const int64_t idx = (int64_t)blockIdx.x * ROWS + grp / G;
   const int sub = grp % G;
   const int d0 = (threadIdx.x & 31) * 4;
-  const int per = a.mtiles * bm;
-  const int pair = (int)(idx / per);  // (segment, KV head)
-  if (pair >= a.n_seg * a.Hkv) return;
-  const int mrow = (int)(idx - (int64_t)pair * per);
-  const int hkv = pair % a.Hkv;
-  const int s = pair / a.Hkv;
-  const Segment sg = segment(a, s);
+  // grid: rows of the largest segment, KV heads, segments
+  const int mrow = blockIdx.x * (8 / G) + grp / G;
+  const int hkv = blockIdx.y, s = blockIdx.z;
+  const Segment sg = segment(a, cu, seg_ids, lens, s);
   if (mrow >= sg.len * a.g) return;
-  const int ns = splits_of(a, sg, mrow / bm);
-  if (ns == 1) return;
-  const int64_t recs = (int64_t)a.n_seg * a.Hkv * a.mtiles * a.n_split * bm;
-  const int64_t rec0 = (((int64_t)s * a.Hkv + hkv) * a.mtiles + mrow / bm) * a.n_split * bm + mrow % bm;
-  const float* const ml = a.ws + recs * HD;
+  const int mt = mrow / BM, row = mrow % BM;
+  const int parts = splits_of<TILE>(a, tiles_per_split, sg, TILE ? (min((mt + 1) * BM, sg.len * a.g) - 1) / a.g : 0);
+  if (parts == 1) return;
+  // part p of this row: workgroup L0 + p * mtiles (the tile form counts its M tiles from the last)
+  const int L0 = (s * Hkv + hkv) * max_split * mtiles + (TILE ? mtiles - 1 - mt : mt);
   float mx = -INFINITY;
 #pragma unroll 8
-  for (int p = sub; p < ns; p += G) mx = fmaxf(mx, ml[(rec0 + (int64_t)p * bm) * 2]);
+  for (int p = sub; p < parts; p += G) mx = fmaxf(mx, part_ml<BM>(a, logical_blocks, L0 + p * mtiles, row)[0]);
   const float mu = mx == -INFINITY ? 0.f : mx;
   float l = 0.f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int p = sub; p < ns; p += G) {
-    const int64_t rec = rec0 + (int64_t)p * bm;
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.ws + rec * HD + d0);
-    const float mp = ml[rec * 2];
-    const float w = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mu);
-    l += ml[rec * 2 + 1] * w;
+  for (int p = sub; p < parts; p += G) {
+    const int at = L0 + p * mtiles;
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(part_o<BM>(a, at, row) + d0);
+    const float* const ml = part_ml<BM>(a, logical_blocks, at, row);
+    const float w = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mu);
+    l += ml[1] * w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
   }
-  if constexpr (G > 1) {  // G = 8: the workgroup holds one row
+  if constexpr (G > 1) {
     part[threadIdx.x] = acc;
     if ((threadIdx.x & 31) == 0) {
-      part_ml[2 * sub] = mx;
-      part_ml[2 * sub + 1] = l;
+      part_s[2 * sub] = mx;
+      part_s[2 * sub + 1] = l;
     }
     __syncthreads();
     if (sub) return;
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < G; ++i) top = fmaxf(top, part_ml[2 * i]);
+    for (int i = 0; i < G; ++i) top = fmaxf(top, part_s[2 * i]);
     const float tu = top == -INFINITY ? 0.f : top;
     l = 0.f;
     acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const float w = part_ml[2 * i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(part_ml[2 * i] - tu);
-      l += part_ml[2 * i + 1] * w;
+      const float w = part_s[2 * i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(part_s[2 * i] - tu);
+      l += part_s[2 * i + 1] * w;
       const f32x4_t x = part[32 * i + (threadIdx.x & 31)];
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
@@ -1005,75 +1055,98 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkArgs a) {
 // ---- launch plan ---------------------------------------------------------------------
 struct ChunkPlan {
   bool tile_form;
-  int nw;                        // chunk_tile_kernel: wavefronts
   int nb;                        // chunk_rows_kernel: 16-row blocks
-  int bm, mtiles;                // M rows of a workgroup, M tiles
-  int n_split, tiles_per_split;  // workgroups along the keys
+  int bm;                        // M rows of a workgroup
+  int max_split, tiles_per_split;
+  int mtiles;                    // of the largest segment
+  int64_t logical;               // workgroups
 };
-static ChunkPlan chunk_plan(int n_seg, int max_q, int max_cached, int Hq, int Hkv) {
+// total_q / total_cached: the segments' sums, or an upper bound of them.
+static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached, int Hq,
+                            int Hkv) {
   ChunkPlan p = {};
-  const int64_t rows = (int64_t)max_q * (Hq / Hkv);
-  const int64_t pairs = (int64_t)n_seg * Hkv;
+  const int64_t g = Hq / Hkv, rows = max_q * g;
   p.tile_form = rows > 64;
-  if (p.tile_form) {
-    p.nw = pairs * ((rows + 255) / 256) >= 256 ? 8 : 4;
-    p.bm = 32 * p.nw;
-  } else {
-    p.nb = rows <= 16 ? 1 : 2;
-    p.bm = 16 * p.nb;
-  }
+  p.nb = rows <= 16 ? 1 : 2;
+  p.bm = p.tile_form ? kTileRows : 16 * p.nb;
   p.mtiles = (int)((rows + p.bm - 1) / p.bm);
-  const int64_t groups = pairs * p.mtiles;
+  // M tiles and tiles of all segments, at most
+  const int64_t all_m = std::min(n_seg * p.mtiles, total_q * g / p.bm + n_seg);
   const int64_t key = p.tile_form ? kBigTile : kTileKeys;
   const int64_t tiles = (max_cached + key - 1) / key + (p.tile_form ? (max_q + key - 1) / key : 0);
-  const int64_t least = 8;  // tiles of a split
-  int64_t want = groups > 0 ? 512 / groups : 1;
-  if (want > (tiles + least - 1) / least) want = (tiles + least - 1) / least;
-  if (want < 1) want = 1;
-  int64_t tps = (tiles + want - 1) / want;
-  if (!p.tile_form) tps = (tps + 3) / 4 * 4 < kMaxSplitTiles ? (tps + 3) / 4 * 4 : kMaxSplitTiles;
-  p.tiles_per_split = tps > 0 ? (int)tps : 4;
-  p.n_split = tiles > 0 ? (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
+  const int64_t all_t =
+      std::min(n_seg * tiles, p.tile_form ? (total_cached + total_q + 2 * (key - 1) * n_seg) / key
+                                          : (total_cached + (key - 1) * n_seg) / key);
+  // Splits while one generation of 256 workgroups, one a CU, holds them all: a CU takes in
+  // about 27 KB a microsecond however many workgroups it has, and every further
+  // one pays for its start and the joining.  Segments count as the average one.
+  const int64_t least = 8;
+  int64_t tps = tiles;
+  if (n_seg * Hkv * p.mtiles * 2 <= (p.tile_form ? 512 : 256) && tiles > 24) {
+    tps = (int64_t)((double)all_m * (double)all_t / (double)n_seg * Hkv / (p.tile_form ? 512 : 256) + 0.999);
+    if (tps < least) tps = least;
+  }
+  if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
+  if (tps < 1) tps = 1;
+  if (tps > 0x3fffffff) tps = 0x3fffffff;
+  p.tiles_per_split = (int)tps;
+  p.max_split = (int)std::max<int64_t>(1, (tiles + tps - 1) / tps);
+  p.logical = n_seg * Hkv * p.mtiles * p.max_split;
   return p;
 }
-static size_t chunk_ws(const ChunkPlan& p, int n_seg, int Hkv) {
-  if (p.n_split <= 1) return 0;
-  return (size_t)n_seg * Hkv * p.mtiles * p.n_split * p.bm * (HD + 2) * sizeof(float);
+static size_t chunk_ws(const ChunkPlan& p) {
+  return p.max_split <= 1 ? 0 : (size_t)p.logical * p.bm * (HD + 2) * sizeof(float);
 }
 
 }  // namespace dllm
 
 using namespace dllm;
 
-static bool chunk_sizes_ok(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D) {
-  return D == HD && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && n_seg >= 0 && max_q >= 0 && max_cached >= 0 &&
-         max_cached <= 0x7fffffff - 64 && (int64_t)max_q * (Hq / Hkv) <= (1 << 30);
+static bool chunk_sizes_ok(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached, int Hq, int Hkv,
+                           int D) {
+  return D == HD && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && n_seg >= 0 && max_q >= 0 && max_cached >= 0 && total_q >= 0 &&
+         total_cached >= 0 && max_cached <= 0x7fffffff - 64 && (int64_t)max_q * (Hq / Hkv) <= (1 << 30);
+}
+// Sums that are not given, or beyond what the largest segment allows.
+static int64_t chunk_total(int64_t total, int n_seg, int most) {
+  const int64_t bound = (int64_t)n_seg * most;
+  return total > 0 && total < bound ? total : bound;
 }
 
-extern "C" size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D) {
-  if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D) || n_seg == 0 || max_q == 0) return 0;
-  return chunk_ws(chunk_plan(n_seg, max_q, max_cached, Hq, Hkv), n_seg, Hkv);
+extern "C" size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int64_t total_q,
+                                                 int64_t total_cached, int Hq, int Hkv, int D) {
+  if (!chunk_sizes_ok(n_seg, max_q, max_cached, total_q, total_cached, Hq, Hkv, D) || n_seg == 0 || max_q == 0) return 0;
+  return chunk_ws(chunk_plan(n_seg, max_q, max_cached, chunk_total(total_q, n_seg, max_q),
+                             chunk_total(total_cached, n_seg, max_cached), Hq, Hkv));
 }
 
-extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D, int* rows,
-                                            int* n_split, int* grid) {
-  if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
+static int chunk_grid(const ChunkPlan& p, int* chunk) {
+  // the M tiles of a (segment, KV head) read the same keys: next to each other on one XCD
+  *chunk = p.mtiles < 16 ? p.mtiles : 16;
+  const int64_t grain = 8 * (int64_t)*chunk;
+  return (int)((p.logical + grain - 1) / grain * grain);
+}
+
+extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached,
+                                            int Hq, int Hkv, int D, int* rows, int* n_split, int* grid) {
+  if (!chunk_sizes_ok(n_seg, max_q, max_cached, total_q, total_cached, Hq, Hkv, D))
     return fail(DLLM_ERR_INVALID_ARG, "dllm_attn_chunk_launch_shape: unsupported sizes");
-  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
-  const bool none = n_seg == 0 || max_q == 0;
-  if (rows) *rows = p.bm;
-  if (n_split) *n_split = p.n_split;
-  if (grid) {
-    const int64_t logical = (int64_t)n_seg * Hkv * p.mtiles * p.n_split;
-    const int64_t grain = 8 * (int64_t)(p.mtiles < 16 ? p.mtiles : 16);
-    *grid = none ? 0 : (int)((logical + grain - 1) / grain * grain);
+  ChunkPlan p = {};
+  int chunk, blocks = 0;
+  if (n_seg > 0 && max_q > 0) {
+    p = chunk_plan(n_seg, max_q, max_cached, chunk_total(total_q, n_seg, max_q),
+                   chunk_total(total_cached, n_seg, max_cached), Hq, Hkv);
+    blocks = p.logical > (1 << 28) ? 0 : chunk_grid(p, &chunk);
   }
+  if (rows) *rows = p.bm;
+  if (n_split) *n_split = p.max_split;
+  if (grid) *grid = blocks;
   return DLLM_OK;
 }
 
 extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
                                          const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
-                                         const void* k_cache, const void* v_cache, int cache_type, int num_pages,
+                                         int64_t total_q, int64_t total_cached, const void* k_cache, const void* v_cache, int cache_type, int num_pages,
                                          const int32_t* page_table, int max_pages, const int32_t* cached_len,
                                          int mask_block, int Hq, int Hkv, int D, int64_t q_stride, int64_t k_stride,
                                          int64_t v_stride, int64_t o_stride, float softmax_scale, void* workspace,
@@ -1082,14 +1155,15 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
   set_error("");
   int rc = common_checks(name, q, k, v, o, Hq, Hkv, D, q_stride, k_stride, v_stride, o_stride);
   if (rc) return rc;
-  if (n_seg < 0 || max_q < 0 || max_cached < 0 || mask_block < 0 || max_pages < 0)
+  if (n_seg < 0 || max_q < 0 || max_cached < 0 || mask_block < 0 || max_pages < 0 || total_q < 0 ||
+      total_cached < 0)
     return fail(DLLM_ERR_INVALID_ARG, "%s: negative size", name);
   if (cache_type != DLLM_CACHE_BF16 && cache_type != DLLM_CACHE_FP8)
     return fail(DLLM_ERR_INVALID_ARG, "%s: cache type %d", name, cache_type);
   if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY))
     return fail(DLLM_ERR_INVALID_ARG, "%s: softmax_scale must be positive and finite", name);
   if (n_seg == 0 || max_q == 0) return DLLM_OK;
-  if (!chunk_sizes_ok(n_seg, max_q, max_cached, Hq, Hkv, D))
+  if (!chunk_sizes_ok(n_seg, max_q, max_cached, total_q, total_cached, Hq, Hkv, D))
     return fail(DLLM_ERR_UNSUPPORTED, "%s: %d new rows of %d query heads per KV head, %d cached", name, max_q, Hq / Hkv,
                 max_cached);
   if (num_pages < 0 || num_pages > (1 << 23)) return fail(DLLM_ERR_INVALID_ARG, "%s: %d pages", name, num_pages);
@@ -1105,22 +1179,22 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
     if (!aligned16(k_cache) || !aligned16(v_cache))
       return fail(DLLM_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", name);
   }
-  if ((int64_t)n_seg * max_pages >= ((int64_t)1 << 31)) return fail(DLLM_ERR_INVALID_ARG, "%s: page table too large", name);
+  if ((int64_t)n_seg * max_pages >= ((int64_t)1 << 31) || max_pages >= (1 << 26)) return fail(DLLM_ERR_INVALID_ARG, "%s: page table too large", name);
   ChunkArgs a = {};
   a.q = q; a.k = k; a.v = v; a.o = o;
   a.kc = reinterpret_cast<const uint8_t*>(k_cache);
   a.vc = reinterpret_cast<const uint8_t*>(v_cache);
-  a.cu = cu; a.seg_ids = seg_ids; a.table = page_table; a.lens = cached_len;
   a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.o_stride = o_stride;
   a.cache_rows = (int64_t)num_pages * kPageRows;
-  a.max_pages = max_pages; a.max_q = max_q; a.max_cached = max_cached;
-  a.n_seg = n_seg; a.Hkv = Hkv; a.g = Hq / Hkv;
+  a.max_q = max_q; a.max_cached = max_cached;
+  a.g = Hq / Hkv;
   a.mask_block = mask_block;
   a.scale_log2 = softmax_scale * kLog2e;
-  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, Hq, Hkv);
-  a.bm = p.bm; a.tile_form = p.tile_form;
-  a.mtiles = p.mtiles; a.n_split = p.n_split; a.tiles_per_split = p.tiles_per_split;
-  const size_t need = chunk_ws(p, n_seg, Hkv);
+  const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, chunk_total(total_q, n_seg, max_q),
+                                 chunk_total(total_cached, n_seg, max_cached), Hq, Hkv);
+  if (p.logical > (int64_t)1 << 28 || n_seg > 65535 || Hkv > 65535)
+    return fail(DLLM_ERR_INVALID_ARG, "%s: problem too large", name);
+  const size_t need = chunk_ws(p);
   if (need) {
     if (!workspace || workspace_bytes < need)
       return fail(DLLM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", name, need,
@@ -1128,40 +1202,35 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
     if (!aligned16(workspace)) return fail(DLLM_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
     a.ws = reinterpret_cast<float*>(workspace);
   }
-  const int64_t logical = (int64_t)n_seg * Hkv * p.mtiles * p.n_split;
-  if (logical > (int64_t)1 << 28) return fail(DLLM_ERR_INVALID_ARG, "%s: problem too large", name);
-  a.logical_blocks = (int)logical;
-  // the row blocks of a (segment, KV head) read the same keys: next to each other on one XCD
-  a.xcd_chunk = p.mtiles < 16 ? p.mtiles : 16;
-  const int64_t grain = 8 * (int64_t)a.xcd_chunk;
-  const unsigned grid = (unsigned)((logical + grain - 1) / grain * grain);
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const bool fp8 = cache_type == DLLM_CACHE_FP8;
-  auto launch = [&](auto kern, int threads, int lds_bytes) -> int {
-    int e = set_lds(kern, lds_bytes, name);
-    if (e) return e;
-    kern<<<dim3(grid), dim3(threads), lds_bytes, st>>>(a);
+  int chunk;
+  const int grid = chunk_grid(p, &chunk);
+  const int chunk_pages = chunk + 32 * (max_cached > 0 ? max_pages : 0);
+  auto start = [&](auto kern, dim3 blocks, int lds_bytes) {
+    kern<<<blocks, dim3(256), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
+        cu, seg_ids, cached_len, page_table, chunk_pages, (int)p.logical, p.mtiles, p.max_split, p.tiles_per_split, Hkv, a);
     return check_launch(name);
   };
-  constexpr int kTileLds = 2 * 2 * kBigTile * 256;
-  if (p.tile_form && p.nw == 8)
-    rc = launch(fp8 ? chunk_tile_kernel<8, true> : chunk_tile_kernel<8, false>, 512, kTileLds);
-  else if (p.tile_form)
-    rc = launch(fp8 ? chunk_tile_kernel<4, true> : chunk_tile_kernel<4, false>, 256, kTileLds);
+  const bool fp8 = cache_type == DLLM_CACHE_FP8;
+  auto launch = [&](auto kern, int lds_bytes) -> int {
+    int e = set_lds(kern, lds_bytes, name);
+    if (e) return e;
+    return start(kern, dim3((unsigned)grid), lds_bytes);
+  };
+  if (p.tile_form)
+    rc = launch(fp8 ? chunk_tile_kernel<true> : chunk_tile_kernel<false>, 2 * kTileStage);
   else if (p.nb == 1)
-    rc = fp8 ? launch(chunk_rows_kernel<1, true>, 256, rows_lds<1, true>())
-             : launch(chunk_rows_kernel<1, false>, 256, rows_lds<1, false>());
+    rc = fp8 ? launch(chunk_rows_kernel<1, true>, rows_lds<1, true>())
+             : launch(chunk_rows_kernel<1, false>, rows_lds<1, false>());
   else
-    rc = fp8 ? launch(chunk_rows_kernel<2, true>, 256, rows_lds<2, true>())
-             : launch(chunk_rows_kernel<2, false>, 256, rows_lds<2, false>());
-  if (rc) return rc;
-  if (p.n_split > 1) {
-    const int64_t rows = (int64_t)n_seg * Hkv * p.mtiles * p.bm;
-    if (p.n_split > 8)
-      chunk_combine_kernel<8><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a);
-    else
-      chunk_combine_kernel<1><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st>>>(a);
-    rc = check_launch(name);
-  }
-  return rc;
+    rc = fp8 ? launch(chunk_rows_kernel<2, true>, rows_lds<2, true>())
+             : launch(chunk_rows_kernel<2, false>, rows_lds<2, false>());
+  if (rc || p.max_split == 1) return rc;
+  auto join = [&](auto one, auto eight) {
+    const bool many = p.max_split > 8;
+    const int64_t rows = (int64_t)max_q * a.g;
+    return start(many ? eight : one, dim3((unsigned)(many ? rows : (rows + 7) / 8), (unsigned)Hkv, (unsigned)n_seg), 0);
+  };
+  if (p.tile_form) return join(chunk_combine_kernel<kTileRows, true, 1>, chunk_combine_kernel<kTileRows, true, 8>);
+  return p.nb == 1 ? join(chunk_combine_kernel<16, false, 1>, chunk_combine_kernel<16, false, 8>)
+                   : join(chunk_combine_kernel<32, false, 1>, chunk_combine_kernel<32, false, 8>);
 }

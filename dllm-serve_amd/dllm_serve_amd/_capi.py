@@ -68,11 +68,11 @@ SIGNATURES = {
     "dllm_quant_page_bytes": (_SZ, [_I]),
     "dllm_store_kvcache_fp8": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I, _I, _I, _P]),
     "dllm_load_kvcache_fp8": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I, _I, _I, _P]),
-    "dllm_attn_chunk_workspace_size": (_SZ, [_I, _I, _I, _I, _I, _I]),
-    "dllm_attn_chunk_launch_shape": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "dllm_attn_chunk_workspace_size": (_SZ, [_I, _I, _I, _I64, _I64, _I, _I, _I]),
+    "dllm_attn_chunk_launch_shape": (_I, [_I, _I, _I, _I64, _I64, _I, _I, _I, _P, _P, _P]),
     "dllm_attn_chunk_paged_fwd": (
         _I,
-        [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I,
+        [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I64, _I64, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I,
          _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
     ),
     "dllm_select_kv_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
@@ -352,15 +352,16 @@ def load_kvcache_fp8(key, value, k_pages, v_pages, slot_mapping, n_tok, Hkv, D):
     _check(rc, "dllm_load_kvcache_fp8")
 
 
-def chunk_workspace_size(n_seg, max_q, max_cached, Hq, Hkv, D) -> int:
-    return int(_lib_now().dllm_attn_chunk_workspace_size(n_seg, max_q, max_cached, Hq, Hkv, D))
+def chunk_workspace_size(n_seg, max_q, max_cached, Hq, Hkv, D, total_q=0, total_cached=0) -> int:
+    return int(_lib_now().dllm_attn_chunk_workspace_size(n_seg, max_q, max_cached, total_q, total_cached, Hq, Hkv, D))
 
 
-def chunk_launch_shape(n_seg, max_q, max_cached, Hq, Hkv, D) -> dict:
+def chunk_launch_shape(n_seg, max_q, max_cached, Hq, Hkv, D, total_q=0, total_cached=0) -> dict:
     """Launch shape of the chunk attention for these sizes (no launch): M rows
-    per workgroup, workgroups along the keys, grid."""
+    per workgroup, workgroups along the keys at most, grid."""
     vals = [ctypes.c_int(0) for _ in range(3)]
-    _check(load().dllm_attn_chunk_launch_shape(n_seg, max_q, max_cached, Hq, Hkv, D, *[ctypes.byref(x) for x in vals]),
+    _check(load().dllm_attn_chunk_launch_shape(n_seg, max_q, max_cached, total_q, total_cached, Hq, Hkv, D,
+                                               *[ctypes.byref(x) for x in vals]),
            "dllm_attn_chunk_launch_shape")
     return dict(rows=vals[0].value, n_split=vals[1].value, grid=vals[2].value)
 

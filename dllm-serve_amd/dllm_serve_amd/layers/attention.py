@@ -160,7 +160,7 @@ class ChunkPlan:
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.n_seg = B = len(seqlens)
-        self.total_rows = sum(seqlens)
+        self.total_rows, self.total_cached = sum(seqlens), sum(cached)
         self.max_q, self.max_cached = max(seqlens, default=0), max(cached, default=0)
         self.max_pages = W = max(need, default=0)
         self.max_page = max((p for t, n in zip(tables, need) for p in t[:n]), default=-1)
@@ -226,14 +226,15 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
         raise ValueError(f"a block table names page {plan.max_page} of a cache of {pages}")
     with _on_device(dev):
         o = torch.empty(nq, Hq * D, dtype=torch.bfloat16, device=dev)
-        need = _capi.chunk_workspace_size(plan.n_seg, plan.max_q, plan.max_cached, Hq, Hkv, D)
+        need = _capi.chunk_workspace_size(plan.n_seg, plan.max_q, plan.max_cached, Hq, Hkv, D, plan.total_rows,
+                                          plan.total_cached)
         # from the allocator at every call: a plan may be used on several streams and in several graphs
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         if nq:
             cu, lens, tables = plan._args
             _capi.attn_chunk_paged_fwd_raw(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, None, plan.n_seg, plan.max_q,
-                plan.max_cached, k_cache.data_ptr(), v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens,
+                plan.max_cached, plan.total_rows, plan.total_cached, k_cache.data_ptr(), v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens,
                 plan.mask_block, Hq, Hkv, D, q_st, k_st, v_st, o.stride(0), float(softmax_scale),
                 None if ws is None else ws.data_ptr(), need, _capi._stream(dev))
     return o

@@ -247,7 +247,9 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * n = cached_len[s].  A row whose page is outside the cache (or whose page index is >=
  * max_pages) is left out of the softmax.
  * max_q and max_cached must bound L and n of every segment: longer segments are
- * cut there.  D must be 128, Hq a multiple of Hkv, softmax_scale positive; pointers are
+ * cut there.  total_q and total_cached must bound their sums (0: not known), which
+ * lets the work be dealt evenly when the segments differ; beyond them rows are left
+ * unwritten.  D must be 128, Hq a multiple of Hkv, softmax_scale positive; pointers are
  * 16-byte aligned, token strides multiples of 8 elements, and a segment's new rows span
  * at most 4 GiB of q, k or v.  workspace: dllm_attn_chunk_workspace_size(...) bytes
  * (0 where one workgroup takes all keys of a row), any contents; calls that may
@@ -255,14 +257,16 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  */
 #define DLLM_CACHE_BF16 0
 #define DLLM_CACHE_FP8 1
-size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D);
+size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached,
+                                      int Hq, int Hkv, int D);
 /* Launch shape for these sizes, without launching: M rows (tokens x Hq / Hkv) of a
  * workgroup, workgroups along the keys, grid.  Any output pointer may be null. */
-int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int Hq, int Hkv, int D, int* rows,
-                                 int* n_split, int* grid);
+int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached, int Hq,
+                                 int Hkv, int D, int* rows, int* n_split, int* grid);
 int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
                               const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
-                              const void* k_cache, const void* v_cache, int cache_type, int num_pages,
+                              int64_t total_q, int64_t total_cached, const void* k_cache, const void* v_cache,
+                              int cache_type, int num_pages,
                               const int32_t* page_table, int max_pages, const int32_t* cached_len, int mask_block,
                               int Hq, int Hkv, int D, int64_t q_stride_tok, int64_t k_stride_tok,
                               int64_t v_stride_tok, int64_t o_stride_tok, float softmax_scale, void* workspace,

@@ -18,7 +18,7 @@ def _err(rc):
 
 
 def _paged(**kw):
-    a = dict(q=FAKE, k=FAKE, v=FAKE, o=FAKE, cu=FAKE, ids=None, n_seg=1, max_q=1, max_cached=64, kc=FAKE, vc=FAKE, kind=1,
+    a = dict(q=FAKE, k=FAKE, v=FAKE, o=FAKE, cu=FAKE, ids=None, n_seg=1, max_q=1, max_cached=64, tq=0, tc=0, kc=FAKE, vc=FAKE, kind=1,
              pages=4, table=FAKE, max_pages=1, lens=FAKE, mask=1, Hq=4, Hkv=2, D=128, qs=512, ks=256, vs=256, os=512,
              scale=0.1, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
@@ -34,6 +34,9 @@ def _paged(**kw):
     (dict(ks=128), "INVALID_ARG", "smaller"),
     (dict(n_seg=-1), "INVALID_ARG", "negative"),
     (dict(mask=-1), "INVALID_ARG", "negative"),
+    (dict(tq=-1), "INVALID_ARG", "negative"),
+    (dict(tc=-1), "INVALID_ARG", "negative"),
+    (dict(n_seg=70000, max_pages=1, max_cached=0), "INVALID_ARG", "too large"),
     (dict(kind=2), "INVALID_ARG", "cache type"),
     (dict(scale=0.0), "INVALID_ARG", "softmax_scale"),
     (dict(scale=-1.0), "INVALID_ARG", "softmax_scale"),

@@ -216,7 +216,7 @@ def test_rows_outside_the_segments_stay(dev):
     q, k, v = (torch.cat([t, t[:2]]).to(dev) for t in (b.q, b.k, b.v))
     cu, lens, tables = plan._args
     _capi.attn_chunk_paged_fwd_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, None, 2, 4, 300,
-                                   b.kc.data_ptr(), b.vc.data_ptr(), _capi.CACHE_FP8, b.pages, tables, plan.max_pages,
+                                   7, 310, b.kc.data_ptr(), b.vc.data_ptr(), _capi.CACHE_FP8, b.pages, tables, plan.max_pages,
                                    lens, 1, 2, 2, 128, 256, 256, 256, 256, SCALE, ws.data_ptr(), ws.numel(),
                                    _capi._stream(dev))
     assert (o[7:] == 3).all()
@@ -239,7 +239,7 @@ def test_some_sequences_of_a_packed_batch(dev, bits, lens, cached):
     kind = _capi.CACHE_FP8 if bits == 8 else _capi.CACHE_BF16
     _, n, tables = plan._args
     _capi.attn_chunk_paged_fwd_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu.data_ptr(), seg.data_ptr(),
-                                   2, plan.max_q, plan.max_cached, b.kc.data_ptr(), b.vc.data_ptr(), kind, b.pages,
+                                   2, plan.max_q, plan.max_cached, 0, 0, b.kc.data_ptr(), b.vc.data_ptr(), kind, b.pages,
                                    tables, plan.max_pages, n, 0, 4, 2, 128, 512, 256, 256, 512, SCALE, ws.data_ptr(),
                                    ws.numel(), _capi._stream(dev))
     assert (o[lens[0]:lens[0] + lens[1]] == 5).all()
