@@ -1066,7 +1066,12 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
                             int Hkv) {
   ChunkPlan p = {};
   const int64_t g = Hq / Hkv, rows = max_q * g;
-  p.tile_form = rows > 64;
+  // Tiles of 128 rows pay where they fill the card, three workgroups on four CUs, or where
+  // there are many of them; otherwise the rows form, whose wavefronts share the keys.
+  // 32/32 heads, rows / tiles in us: 8 x 100 rows behind 2000 84 / 75, 4 x 256 behind
+  // 1000 59 / 51, but 1 x 300 behind 1000 31 / 38, 1 x 130 behind 500 16 / 20; 28/4 heads,
+  // 1 x 1000 behind 1000 83 / 55, but 16 x 32 behind 384 - 1280 25 / 39, 4 x 100 behind 700 21 / 31.
+  p.tile_form = rows > 1024 || (rows > 64 && n_seg * Hkv * ((rows + 127) / 128) >= 192);
   p.nb = rows <= 16 ? 1 : 2;
   p.bm = p.tile_form ? kTileRows : 16 * p.nb;
   p.mtiles = (int)((rows + p.bm - 1) / p.bm);
@@ -1077,15 +1082,17 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   const int64_t all_t =
       std::min(n_seg * tiles, p.tile_form ? (total_cached + total_q + 2 * (key - 1) * n_seg) / key
                                           : (total_cached + (key - 1) * n_seg) / key);
-  // Splits while one generation of 256 workgroups, one a CU, holds them all: a CU takes in
-  // about 27 KB a microsecond however many workgroups it has, and every further
-  // one pays for its start and the joining.  Segments count as the average one.
-  const int64_t least = 8;
-  int64_t tps = tiles;
-  if (n_seg * Hkv * p.mtiles * 2 <= (p.tile_form ? 512 : 256) && tiles > 24) {
-    tps = (int64_t)((double)all_m * (double)all_t / (double)n_seg * Hkv / (p.tile_form ? 512 : 256) + 0.999);
-    if (tps < least) tps = least;
-  }
+  // Keys are split where the work, dealt evenly to one workgroup a CU (tiles: two, whose
+  // phases overlap), gives each at most half of the longest segment.  A CU takes in
+  // about 27 KB a microsecond however many workgroups it has, and every further one
+  // pays for its start and the joining (8 x 32 rows behind 608 - 1216, 32/32 heads, 256
+  // workgroups: 20 us, split in two 30).  Few keys are not split: the joining takes 4
+  // us, a turn of the rows form's wavefronts (four tiles) 0.8: one token behind
+  // 511 rows 9.9 us whole, 11.4 in two.
+  const int64_t least = p.tile_form ? 4 : 8;
+  int64_t tps = (int64_t)((double)all_m * (double)all_t / (double)n_seg * Hkv / (p.tile_form ? 512 : 256) + 0.999);
+  if (tps < least) tps = least;
+  if (tps * 2 > tiles || tiles <= (p.tile_form ? 8 : 24)) tps = tiles;
   if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
   if (tps < 1) tps = 1;
   if (tps > 0x3fffffff) tps = 0x3fffffff;

@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -133,6 +134,99 @@ PyObject* attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// An 8-bit cache (uint8 [pages, heads, bytes of a page]), or null.
+const at::Tensor* pages_of(PyObject* o, int64_t heads, int device) {
+  const at::Tensor* t = plain(o, at::kByte);
+  if (!t || t->get_device() != device || t->dim() != 3 || t->size(1) != heads ||
+      t->size(2) != (int64_t)dllm_quant_page_bytes(128) || !t->is_contiguous())
+    return nullptr;
+  return t;
+}
+
+// quant_copy(key, value, k_cache, v_cache, slot_mapping, store) -> True or None
+PyObject* quant_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6 || !PyBool_Check(a[5])) Py_RETURN_NONE;
+  const bool store = a[5] == Py_True;
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *k = plain(a[0], at::kBFloat16), *v = plain(a[1], at::kBFloat16), *slot = plain(a[4], at::kInt);
+    if (!k || !v || !slot || k->dim() != 3 || !token_rows(*k, k->size(1), 128) || k->size(0) > INT32_MAX ||
+        v->dim() != 3 || !token_rows(*v, k->size(1), 128) || v->size(0) != k->size(0) || slot->numel() != k->size(0) ||
+        !slot->is_contiguous())
+      Py_RETURN_NONE;
+    const int dev = k->get_device();
+    const at::Tensor *kp = pages_of(a[2], k->size(1), dev), *vp = pages_of(a[3], k->size(1), dev);
+    if (!kp || !vp || v->get_device() != dev || slot->get_device() != dev || c10::hip::current_device() != dev)
+      Py_RETURN_NONE;
+    void* st = stream_of(dev);
+    const int rc = no_gil([&] {
+      return (store ? dllm_store_kvcache_fp8(ptr<dllm_bf16>(*k), k->stride(0), ptr<dllm_bf16>(*v), v->stride(0),
+                                             ptr<uint8_t>(*kp), ptr<uint8_t>(*vp), std::min(kp->size(0), vp->size(0)),
+                                             ptr<int32_t>(*slot), (int)k->size(0), (int)k->size(1), 128, st)
+                    : dllm_load_kvcache_fp8(ptr<dllm_bf16>(*k), k->stride(0), ptr<dllm_bf16>(*v), v->stride(0),
+                                            ptr<uint8_t>(*kp), ptr<uint8_t>(*vp), std::min(kp->size(0), vp->size(0)),
+                                            ptr<int32_t>(*slot), (int)k->size(0), (int)k->size(1), 128, st));
+    });
+    if (rc != DLLM_OK) return refused(store ? "dllm_store_kvcache_fp8" : "dllm_load_kvcache_fp8", rc);
+    Py_RETURN_TRUE;
+  });
+}
+
+// chunk(q, k, v, k_cache, v_cache, plan: bytes, scale) -> output or None.
+struct ChunkTables {
+  int64_t device, rows, n_seg, max_q, max_cached, total_cached, max_pages, max_page, mask_block, cu, lens, tables;
+};
+
+PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7 || !PyBytes_CheckExact(a[5]) || PyBytes_GET_SIZE(a[5]) != (Py_ssize_t)sizeof(ChunkTables) ||
+      !PyFloat_CheckExact(a[6]))
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    ChunkTables p;
+    std::memcpy(&p, PyBytes_AS_STRING(a[5]), sizeof(p));
+    const at::Tensor* t[3];
+    int64_t heads[3];
+    for (int i = 0; i < 3; ++i) {
+      t[i] = plain(a[i], at::kBFloat16);
+      if (!t[i] || t[i]->get_device() != p.device || t[i]->dim() < 2 || t[i]->size(0) != p.rows) Py_RETURN_NONE;
+      heads[i] = t[i]->dim() == 2 ? t[i]->size(1) / 128 : t[i]->size(1);
+      if (heads[i] <= 0 || !token_rows(*t[i], heads[i], 128)) Py_RETURN_NONE;
+    }
+    const int64_t Hq = heads[0], Hkv = heads[1];
+    if (heads[2] != Hkv || Hq % Hkv || p.rows == 0 || c10::hip::current_device() != p.device) Py_RETURN_NONE;
+    const at::Tensor *kc = pages_of(a[3], Hkv, (int)p.device), *vc = pages_of(a[4], Hkv, (int)p.device);
+    const int kind = kc ? DLLM_CACHE_FP8 : DLLM_CACHE_BF16;
+    if (!kc) {
+      kc = plain(a[3], at::kBFloat16);
+      vc = plain(a[4], at::kBFloat16);
+      for (const at::Tensor* c : {kc, vc})
+        if (!c || c->get_device() != p.device || c->dim() != 4 || c->size(1) != 256 || c->size(2) != Hkv ||
+            c->size(3) != 128 || !c->is_contiguous())
+          Py_RETURN_NONE;
+    }
+    if (!vc) Py_RETURN_NONE;
+    const int64_t pages = std::min(kc->size(0), vc->size(0));
+    if (p.max_page >= pages || pages > INT32_MAX) Py_RETURN_NONE;
+    at::Tensor o = at::empty({p.rows, Hq * 128}, t[0]->options());
+    const size_t nb = dllm_attn_chunk_workspace_size((int)p.n_seg, (int)p.max_q, (int)p.max_cached, p.rows,
+                                                     p.total_cached, (int)Hq, (int)Hkv, 128);
+    at::Tensor ws;
+    if (nb) ws = at::empty({(int64_t)nb}, t[0]->options().dtype(at::kByte));
+    const float scale = (float)PyFloat_AS_DOUBLE(a[6]);
+    void* st = stream_of((int)p.device);
+    auto dev_i32 = [](int64_t x) { return reinterpret_cast<const int32_t*>(x); };
+    const int rc = no_gil([&] {
+      return dllm_attn_chunk_paged_fwd(ptr<dllm_bf16>(*t[0]), ptr<dllm_bf16>(*t[1]), ptr<dllm_bf16>(*t[2]),
+                                       ptr<dllm_bf16>(o), dev_i32(p.cu), nullptr, (int)p.n_seg, (int)p.max_q,
+                                       (int)p.max_cached, p.rows, p.total_cached, kc->data_ptr(), vc->data_ptr(), kind,
+                                       (int)pages, dev_i32(p.tables), (int)p.max_pages, dev_i32(p.lens),
+                                       (int)p.mask_block, (int)Hq, (int)Hkv, 128, t[0]->stride(0), t[1]->stride(0),
+                                       t[2]->stride(0), o.stride(0), scale, nb ? ws.data_ptr() : nullptr, nb, st);
+    });
+    if (rc != DLLM_OK) return refused("dllm_attn_chunk_paged_fwd", rc);
+    return THPVariable_Wrap(std::move(o));
+  });
+}
+
 // rope(positions, query, key, cos_sin_cache, head_size, inplace) -> (query, key) or None
 PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 6 || !PyLong_CheckExact(a[4]) || !PyBool_Check(a[5])) Py_RETURN_NONE;
@@ -239,6 +333,8 @@ PyObject* unmask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, doc }
 PyMethodDef methods[] = {
     FN(attn, "attn(q, k, v, k_cache, v_cache, plan, scale) -> output or None"),
+    FN(quant_copy, "quant_copy(key, value, k_cache, v_cache, slot_mapping, store) -> True or None"),
+    FN(chunk, "chunk(q, k, v, k_cache, v_cache, plan, scale) -> output or None"),
     FN(rope, "rope(positions, query, key, cos_sin_cache, head_size, inplace) -> (query, key) or None"),
     FN(softmax_max, "softmax_max(logits) -> (x0, x0_p) or None"),
     FN(unmask, "unmask(tokens, seq_params, max_win, x0, conf, mask_id) -> counts or None"),

@@ -122,6 +122,9 @@ def _on_device(device: torch.device):
 
 
 def _quant_copy(copy, key, value, k_cache, v_cache, slot_mapping) -> None:
+    if _capi.native is not None and _capi.native.quant_copy(key, value, k_cache, v_cache, slot_mapping,
+                                                            copy is _capi.store_kvcache_fp8):
+        return
     N, num_heads, head_dim = key.shape
     assert value.shape == key.shape and value.device == key.device
     assert key.stride(-1) == 1 and value.stride(-1) == 1
@@ -150,8 +153,8 @@ class ChunkPlan:
         tables = [[int(p) for p in t] for t in block_tables]
         if not (len(seqlens) == len(cached) == len(tables)):
             raise ValueError(f"{len(seqlens)} sequences, {len(cached)} cached lengths, {len(tables)} block tables")
-        if any(n < 0 for n in seqlens + cached) or mask_block < 0:
-            raise ValueError("lengths and mask_block must not be negative")
+        if any(n < 0 for n in seqlens + cached) or not 0 <= mask_block < 2**31:
+            raise ValueError("lengths and mask_block must not be negative (nor mask_block exceed int32)")
         need = [-(-n // _capi.PAGE_ROWS) for n in cached]
         for b, (t, n) in enumerate(zip(tables, need)):
             if len(t) < n or any(p < 0 for p in t[:n]):
@@ -179,6 +182,10 @@ class ChunkPlan:
         dev = host.to(self.device, non_blocking=True)
         self.cu, self.cached_lens, self.block_tables = dev[:B + 1], dev[B + 1:2 * B + 1], dev[2 * B + 1:]
         self._args = (self.cu.data_ptr(), self.cached_lens.data_ptr(), self.block_tables.data_ptr())
+        # the same for the native form (csrc/native.cpp, ChunkTables)
+        self._packed = struct.pack(
+            "=12q", -1 if self.device.index is None else self.device.index, self.total_rows, B, self.max_q,
+            self.max_cached, self.total_cached, W, self.max_page, self.mask_block, *self._args)
 
 
 def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -191,6 +198,10 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
     caches are 8-bit pages (quantized_pages) or bf16 [num_pages, 256, Hkv,
     128]; the new rows are read from k / v, so they may be stored before or after."""
     D = 128
+    if _capi.native is not None:
+        o = _capi.native.chunk(q, k, v, k_cache, v_cache, plan._packed, float(softmax_scale))
+        if o is not None:
+            return o
     for t, n in ((q, "q"), (k, "k"), (v, "v")):
         if t.dtype != torch.bfloat16:
             raise TypeError(f"bf16 {n} expected, got {t.dtype}")

@@ -104,7 +104,27 @@ SHAPES = [
     ([260, 70], [511, 0], 4, 4, 0),
     ([100, 20], [1500, 0], 2, 1, 1),   # many rows, keys split, a short sequence beside a long one
     ([520], [700], 2, 1, 16),          # the new rows' own tiles are split as well
+    # more than 1024 rows of a KV head: tiles of 128 rows
+    ([65], [90], 16, 1, 32),
+    ([70, 9, 0], [40, 512, 3], 16, 1, 1),
+    ([65, 1, 80], [700, 0, 1500], 16, 1, 1),
+    ([300], [0], 4, 1, 0),
+    ([130], [64], 14, 1, 5),
+    ([66], [4200], 16, 1, 1),
 ]
+
+
+def _forms(n):
+    """Query heads per KV head with which n new rows take the rows form, and the tile form."""
+    return 2, -(-1032 // n)
+
+
+def test_the_shapes_take_both_forms():
+    rows = {_capi.chunk_launch_shape(len(a), max(a), max(b), Hq, Hkv, 128, sum(a), sum(b))["rows"]
+            for a, b, Hq, Hkv, _ in SHAPES}
+    assert rows == {16, 32, 128}
+    shape = _capi.chunk_launch_shape(3, 80, 1500, 16, 1, 128, 146, 2200)
+    assert shape["rows"] == 128 and shape["n_split"] > 1
 
 
 @pytest.mark.parametrize("bits", [8, 16])
@@ -129,16 +149,17 @@ def test_ragged_batch_whose_short_sequences_leave_splits_empty(dev, bits):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
-def test_large_scores(dev, bits):
+@pytest.mark.parametrize("g", _forms(70))
+def test_large_scores(dev, bits, g):
     """Scores of hundreds: the maximum moves, most probabilities vanish."""
-    b = Batch(dev, [40, 1], [300, 600], 2, 1, bits, seed=5, kv_scale=4.0)
+    b = Batch(dev, [70, 1], [300, 600], g, 1, bits, seed=5, kv_scale=4.0)
     b.verify(b.run(1, scale=0.5), 1, scale=0.5)
 
 
 @pytest.mark.parametrize("bits", [8, 16])
-@pytest.mark.parametrize("L", [5, 40, 140])
-def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L):
-    b = Batch(dev, [L], [70], 2, 2, bits, seed=6)
+@pytest.mark.parametrize("L,g", [(5, 1), (40, 1), (140, 1), (70, 15), (130, 9)])
+def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L, g):
+    b = Batch(dev, [L], [70], 2 * g, 2, bits, seed=6)
     b.v[L - 1, 0, 3] = float("nan")
     b.v[L - 2, 1, 9] = float("inf")
     b.k[L - 1, 1, 0] = float("nan")
@@ -150,14 +171,15 @@ def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L):
     ref, spread, reach = chunk.attend(*x, b.cache_rows(b.kc, 0), b.cache_rows(b.vc, 0), SCALE, 1)
     check(out[ref_rows], ref[ref_rows], spread[ref_rows], reach[ref_rows], L + 70)
     o = _np(out).reshape(ref.shape)
-    assert np.isnan(o[L - 1]).all(axis=-1)[1]          # a NaN score
-    assert o[L - 2, 1, 9] == np.inf and np.isnan(o[L - 1, 1, 9])
+    assert np.isnan(o[L - 1]).all(axis=-1)[g:].all()   # a NaN score
+    assert (o[L - 2, g:, 9] == np.inf).all() and np.isnan(o[L - 1, g:, 9]).all()
 
 
 @pytest.mark.parametrize("bits", [8, 16])
-def test_stale_rows_behind_the_cached_length(dev, bits):
+@pytest.mark.parametrize("g", _forms(20))
+def test_stale_rows_behind_the_cached_length(dev, bits, g):
     """The rest of the last page holds NaN: it takes no part."""
-    b = Batch(dev, [1, 20], [40, 300], 2, 2, bits, seed=7)
+    b = Batch(dev, [1, 20], [40, 300], 2 * g, 2, bits, seed=7)
     want = [b.run(m) for m in (0, 1)]
     for s, c in enumerate(b.cached):
         page, row = b.tables[s][-1], c % 256
@@ -171,8 +193,9 @@ def test_stale_rows_behind_the_cached_length(dev, bits):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
-def test_pages_outside_the_cache_are_left_out(dev, bits):
-    b = Batch(dev, [3, 1], [600, 520], 2, 1, bits, seed=8)
+@pytest.mark.parametrize("g", _forms(20))
+def test_pages_outside_the_cache_are_left_out(dev, bits, g):
+    b = Batch(dev, [20, 1], [600, 520], g, 1, bits, seed=8)
     plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
     # a table that lost a page after the plan was made, as a runner's bug would
     t = plan.block_tables.view(2, plan.max_pages)
@@ -187,8 +210,9 @@ def test_pages_outside_the_cache_are_left_out(dev, bits):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
-def test_empty_cache_and_no_sequences(dev, bits):
-    b = Batch(dev, [5, 33], [0, 0], 2, 2, bits, seed=9, spare=0)
+@pytest.mark.parametrize("g", _forms(33))
+def test_empty_cache_and_no_sequences(dev, bits, g):
+    b = Batch(dev, [5, 33], [0, 0], 2 * g, 2, bits, seed=9, spare=0)
     assert b.kc.shape[0] == 0
     b.verify(b.run(1), 1)
     b = Batch(dev, [], [], 2, 2, bits, seed=9)
@@ -245,6 +269,25 @@ def test_some_sequences_of_a_packed_batch(dev, bits, lens, cached):
     assert (o[lens[0]:lens[0] + lens[1]] == 5).all()
     o[lens[0]:lens[0] + lens[1]] = b.run(0).view(-1, 4, 128)[lens[0]:lens[0] + lens[1]]
     b.verify(o, 0)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_native_and_python_calls_agree(dev, bits, monkeypatch):
+    b = Batch(dev, [1, 30], [2500, 90], 14, 2, bits, seed=17)
+    want = b.run(1)
+    pages = quantized_pages(1, 2, device=dev), quantized_pages(1, 2, device=dev)
+    slots = torch.arange(31, dtype=torch.int32, device=dev)
+    store_kvcache(b.k.to(dev), b.v.to(dev), *pages, slots)
+    back = [torch.empty_like(b.k, device=dev) for _ in range(2)]
+    load_kvcache(*back, *pages, slots)
+    monkeypatch.setattr(_capi, "native", None)
+    assert torch.equal(b.run(1), want)
+    again = quantized_pages(1, 2, device=dev), quantized_pages(1, 2, device=dev)
+    store_kvcache(b.k.to(dev), b.v.to(dev), *again, slots)
+    assert all(torch.equal(x, y) for x, y in zip(pages, again))
+    out = [torch.empty_like(b.k, device=dev) for _ in range(2)]
+    load_kvcache(*out, *pages, slots)
+    assert all(torch.equal(x, y) for x, y in zip(back, out))
 
 
 @pytest.mark.parametrize("bits", [8, 16])
