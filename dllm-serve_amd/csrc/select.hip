@@ -28,7 +28,7 @@
 // The arithmetic follows a fixed, order-defined rule (f64 sums in a stated
 // order, explicit f32 / bf16 rounding points, ties to the lower candidate
 // index), so the selected indices are reproducible bit for bit on the CPU.
-#include "common.h"
+#include "quant.h"
 
 #include <math.h>
 
@@ -620,7 +620,25 @@ __device__ __forceinline__ uint16_t raw_bits(const SelArgs& a, const Job& jb, in
 // -- into their cache slots by the whole workgroup: item i = (rank r0 + i / 16,
 // 16-byte chunk i % 16), eight items per thread in flight.  cand(r) gives the
 // candidate of rank r.
-template <typename CandFn>
+// One 16-byte piece (chunk chk of KV head h's 128 values) of a row of K and V to 8-bit
+// pages; the sixteen lanes of a row share its slot.  Every lane of the wavefront is
+// active; a slot outside the cache stores nothing.
+__device__ __forceinline__ void store_quant(const SelArgs& a, int h, int chk, int64_t slot, u32x4_t kx, u32x4_t vx) {
+  uint32_t kb, vb;
+  const u32x2_t kc = quant_row16(kx, kb), vc = quant_row16(vx, vb);
+  if (slot < 0 || slot >= a.cache_slots) return;
+  uint8_t* const kp = reinterpret_cast<uint8_t*>(a.k_cache) + record_off((uint32_t)slot, a.Hkv, h);
+  uint8_t* const vp = reinterpret_cast<uint8_t*>(a.v_cache) + record_off((uint32_t)slot, a.Hkv, h);
+  const int r = (int)(slot & (kPageRows - 1));
+  *reinterpret_cast<u32x2_t*>(kp + r * kQuantD + chk * 8) = kc;
+  *reinterpret_cast<u32x2_t*>(vp + r * kQuantD + chk * 8) = vc;
+  if (chk == 0) {
+    kp[kScaleOff + r] = (uint8_t)kb;
+    vp[kScaleOff + r] = (uint8_t)vb;
+  }
+}
+
+template <bool QUANT, typename CandFn>
 __device__ __forceinline__ void copy_selected(const SelArgs& a, const Job& jb, int h, int r0, int r1, CandFn cand) {
   const int64_t row_elems = (int64_t)a.Hkv * SHD;
   const int n_items = (r1 - r0) * 16;
@@ -635,6 +653,7 @@ __device__ __forceinline__ void copy_selected(const SelArgs& a, const Job& jb, i
     for (int u = 0; u < kPer; ++u) {
       const int i = i0 + u * kTopkThreads + (int)threadIdx.x;
       slot[u] = -1;
+      if constexpr (QUANT) kx[u] = vx[u] = u32x4_t{0, 0, 0, 0};
       if (i < n_items) {
         const int r = r0 + (i >> 4), chk = i & 15;
         const int j = cand(r);
@@ -648,11 +667,14 @@ __device__ __forceinline__ void copy_selected(const SelArgs& a, const Job& jb, i
       }
     }
 #pragma unroll
-    for (int u = 0; u < kPer; ++u)
-      if (slot[u] >= 0 && slot[u] < a.cache_slots) {
+    for (int u = 0; u < kPer; ++u) {
+      if constexpr (QUANT) {
+        store_quant(a, h, (int)threadIdx.x & 15, slot[u], kx[u], vx[u]);
+      } else if (slot[u] >= 0 && slot[u] < a.cache_slots) {
         st128(a.k_cache + slot[u] * row_elems + e[u], kx[u]);
         st128(a.v_cache + slot[u] * row_elems + e[u], vx[u]);
       }
+    }
   }
 }
 
@@ -666,6 +688,8 @@ __device__ __forceinline__ void copy_selected(const SelArgs& a, const Job& jb, i
 // LDS: 128 KiB pool (small path: raw bits, order keys and 32-bit sort keys of
 // up to kLdsCand candidates, then the selected candidates in rank order;
 // large path: kSortCap 64-bit sort keys) + the shared scratch.
+// QUANT: the cache is 8-bit pages (quant.h); rows are quantised as they are copied.
+template <bool QUANT>
 __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t pool[128 * 1024];
   __shared__ TopkShared sh;
@@ -781,6 +805,7 @@ __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
       for (int u = 0; u < kPre; ++u) {
         const int i = u * kTopkThreads + tid;
         pc[u] = -1;
+        if constexpr (QUANT) pk[u] = pv[u] = u32x4_t{0, 0, 0, 0};
         if (i < n_items) {
           const int j = 0xffff - (int)(skey[p0 + (i >> 4)] & 0xffffu);
           const int64_t row = (int64_t)jb.row0 + cand_row(jb, j);
@@ -802,7 +827,9 @@ __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
       const int64_t row_elems = (int64_t)a.Hkv * SHD;
 #pragma unroll
       for (int u = 0; u < kPre; ++u) {
-        if (pc[u] >= 0) {
+        if constexpr (QUANT) {
+          store_quant(a, h, tid & 15, pc[u] >= 0 ? slot_l[rank_of[pc[u]]] : -1, pk[u], pv[u]);
+        } else if (pc[u] >= 0) {
           const int64_t slot = slot_l[rank_of[pc[u]]];
           const int64_t e = (int64_t)h * SHD + ((u * kTopkThreads + tid) & 15) * 8;
           if (slot >= 0 && slot < a.cache_slots) {
@@ -820,6 +847,7 @@ __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
         for (int u = 0; u < kPer; ++u) {
           const int i = i0 + u * kTopkThreads + tid;
           slot[u] = -1;
+          if constexpr (QUANT) kx[u] = vx[u] = u32x4_t{0, 0, 0, 0};
           if (i < n_items) {
             const int j = 0xffff - (int)(skey[p0 + (i >> 4)] & 0xffffu);
             const int64_t row = (int64_t)jb.row0 + cand_row(jb, j);
@@ -832,7 +860,9 @@ __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
           const int i = i0 + u * kTopkThreads + tid;
-          if (slot[u] >= 0 && slot[u] < a.cache_slots) {
+          if constexpr (QUANT) {
+            store_quant(a, h, i & 15, slot[u], kx[u], vx[u]);
+          } else if (slot[u] >= 0 && slot[u] < a.cache_slots) {
             const int64_t e = (int64_t)h * SHD + (i & 15) * 8;
             st128(a.k_cache + slot[u] * row_elems + e, kx[u]);
             st128(a.v_cache + slot[u] * row_elems + e, vx[u]);
@@ -868,7 +898,7 @@ __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
     }
     __syncthreads();
     const int r0 = (int)((int64_t)nk * part / a.n_part), r1 = (int)((int64_t)nk * (part + 1) / a.n_part);
-    copy_selected(a, jb, h, r0, r1, [&](int r) { return selc[r]; });
+    copy_selected<QUANT>(a, jb, h, r0, r1, [&](int r) { return selc[r]; });
     return;
   }
 
@@ -945,7 +975,7 @@ __global__ __launch_bounds__(kTopkThreads) void topk_kernel(SelArgs a) {
     radix_pass(sh, a.ckey1 + sbase, a.cidx1 + sbase, nullptr, so, nk, 8, io);
   }
   __syncthreads();  // the workgroup's writes of so are visible to it
-  copy_selected(a, jb, h, 0, nk, [&](int r) { return so[r]; });
+  copy_selected<QUANT>(a, jb, h, 0, nk, [&](int r) { return so[r]; });
 }
 
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -978,13 +1008,12 @@ extern "C" size_t dllm_select_kv_workspace_size(int n_job, int max_kc, int Hq, i
   return sel_layout(n_job, max_kc, Hq, Hkv).total;
 }
 
-extern "C" int dllm_select_kv_store(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, int64_t n_rows,
-                                    int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
-                                    const int32_t* jobs, int n_job, int max_kc, int max_keep, int Hq, int Hkv, int D,
-                                    float sqrt_d, dllm_bf16* k_cache, dllm_bf16* v_cache, int64_t cache_slots,
-                                    const int32_t* slots, int64_t n_slots, int64_t* idx_out, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
-  const char* name = "dllm_select_kv_store";
+// quant: k_cache / v_cache are 8-bit pages of cache_slots rows.
+static int select_impl(const char* name, bool quant, const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v,
+                       int64_t n_rows, int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
+                       const int32_t* jobs, int n_job, int max_kc, int max_keep, int Hq, int Hkv, int D, float sqrt_d,
+                       dllm_bf16* k_cache, dllm_bf16* v_cache, int64_t cache_slots, const int32_t* slots,
+                       int64_t n_slots, int64_t* idx_out, void* workspace, size_t workspace_bytes, void* stream) {
   set_error("");
   if (D != SHD) return fail(DLLM_ERR_UNSUPPORTED, "%s: head_dim %d not supported (the kernels handle 128)", name, D);
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv) return fail(DLLM_ERR_INVALID_ARG, "%s: Hq=%d / Hkv=%d", name, Hq, Hkv);
@@ -1061,6 +1090,33 @@ extern "C" int dllm_select_kv_store(const dllm_bf16* q, const dllm_bf16* k, cons
   // enough top-k workgroups to give every CU one (256 CUs), at most four per (job, KV head)
   const int64_t pairs = (int64_t)n_job * Hkv;
   a.n_part = (int)max((int64_t)1, min((int64_t)4, 256 / pairs));
-  topk_kernel<<<dim3(Hkv, n_job, a.n_part), dim3(kTopkThreads), 0, st>>>(a);
+  auto topk = quant ? topk_kernel<true> : topk_kernel<false>;
+  topk<<<dim3(Hkv, n_job, a.n_part), dim3(kTopkThreads), 0, st>>>(a);
   return check_launch(name);
+}
+
+extern "C" int dllm_select_kv_store(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, int64_t n_rows,
+                                    int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
+                                    const int32_t* jobs, int n_job, int max_kc, int max_keep, int Hq, int Hkv, int D,
+                                    float sqrt_d, dllm_bf16* k_cache, dllm_bf16* v_cache, int64_t cache_slots,
+                                    const int32_t* slots, int64_t n_slots, int64_t* idx_out, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  return select_impl("dllm_select_kv_store", false, q, k, v, n_rows, q_stride_tok, k_stride_tok, v_stride_tok, jobs,
+                     n_job, max_kc, max_keep, Hq, Hkv, D, sqrt_d, k_cache, v_cache, cache_slots, slots, n_slots, idx_out,
+                     workspace, workspace_bytes, stream);
+}
+
+extern "C" int dllm_select_kv_store_fp8(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, int64_t n_rows,
+                                        int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
+                                        const int32_t* jobs, int n_job, int max_kc, int max_keep, int Hq, int Hkv,
+                                        int D, float sqrt_d, uint8_t* k_pages, uint8_t* v_pages, int64_t num_pages,
+                                        const int32_t* slots, int64_t n_slots, int64_t* idx_out, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  const char* name = "dllm_select_kv_store_fp8";
+  if (num_pages < 0 || num_pages > ((int64_t)1 << 23))
+    return fail(DLLM_ERR_INVALID_ARG, "%s: %lld pages (at most 2^23)", name, (long long)num_pages);
+  return select_impl(name, true, q, k, v, n_rows, q_stride_tok, k_stride_tok, v_stride_tok, jobs, n_job, max_kc,
+                     max_keep, Hq, Hkv, D, sqrt_d, reinterpret_cast<dllm_bf16*>(k_pages),
+                     reinterpret_cast<dllm_bf16*>(v_pages), num_pages * kPageRows, slots, n_slots, idx_out, workspace,
+                     workspace_bytes, stream);
 }

@@ -81,6 +81,11 @@ SIGNATURES = {
         [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I, _I, _I, _I, _I, _I, _F,
          _P, _P, _I64, _P, _I64, _P, _P, _SZ, _P],
     ),
+    "dllm_select_kv_store_fp8": (
+        _I,
+        [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I, _I, _I, _I, _I, _I, _F,
+         _P, _P, _I64, _P, _I64, _P, _P, _SZ, _P],
+    ),
     "dllm_rope_neox": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I, _I, _I, _P]),
     "dllm_softmax_max_workspace_size": (_SZ, [_I, _I]),
     "dllm_softmax_max_split_workspace_size": (_SZ, [_I, _I]),
@@ -382,18 +387,22 @@ def select_workspace_size(n_job, max_kc, Hq, Hkv, D) -> int:
 
 def select_kv_store(q, k, v, jobs, n_job, max_kc, max_keep, sqrt_d, k_cache, v_cache, slots, idx_out, workspace):
     """K5/K6: selection + fused cache scatter; jobs int32 [n_job, 8] carry each
-    sequence's head_select and pool_kernel (see include/dllm_attn.h)."""
+    sequence's head_select and pool_kernel (see include/dllm_attn.h).  Into 8-bit
+    pages (uint8) the rows are quantised as they are copied."""
     _require_gpu(q, k, v, jobs, k_cache, v_cache, slots)
     lib = load()
     Hq, Hkv, D = q.shape[1], k.shape[1], q.shape[2]
+    quant = k_cache.dtype == torch.uint8
+    name = "dllm_select_kv_store_fp8" if quant else "dllm_select_kv_store"
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    rc = lib.dllm_select_kv_store(
+    rc = getattr(lib, name)(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), min(q.shape[0], k.shape[0], v.shape[0]),
         q.stride(0), k.stride(0), v.stride(0),
         jobs.data_ptr(), n_job, max_kc, max_keep, Hq, Hkv, D, float(sqrt_d),
-        k_cache.data_ptr(), v_cache.data_ptr(), min(k_cache.numel(), v_cache.numel()) // (Hkv * D),
+        k_cache.data_ptr(), v_cache.data_ptr(),
+        min(k_cache.numel(), v_cache.numel()) // (Hkv * (PAGE_BYTES if quant else D)),
         slots.data_ptr(), slots.numel(), _ptr(idx_out), _ptr(workspace), ws_bytes, _stream(q.device))
-    _check(rc, "dllm_select_kv_store")
+    _check(rc, name)
 
 
 def rope_neox(q_in, q_out, k_in, k_out, positions, cos_sin_cache, n_tok, Hq, Hkv, D):

@@ -86,6 +86,11 @@ class DeviceStepState:
             off.append(len(pages))
         self.pages = torch.tensor(pages or [0], dtype=torch.int32, device=self.device)
         self.page_off = torch.tensor(off, dtype=torch.int32, device=self.device)
+        # the same per sequence, for attention over 8-bit pages
+        width = max([1] + [len(s.block_table) for s in seqs if s.sparse_state is not None])
+        self.block_tables = torch.tensor([(list(s.block_table) if s.sparse_state is not None else [])
+                                          + [-1] * (width - (len(s.block_table) if s.sparse_state is not None else 0))
+                                          for s in seqs], dtype=torch.int32, device=self.device)
         self.tok_stride = int(tok_stride)
         rows_cap = sum(s.num_tokens for s in seqs)
         slots_cap = max(1, sum(s.num_tokens for s in seqs if s.sparse_state is not None))
@@ -126,7 +131,7 @@ class DeviceStepState:
                          self.token_index, self.smp_params, self.smp_rows, self.counts)
         plan = StepPlan.from_device(lay, self.device, self.cu, self.dense_ids[:max(1, lay.n_dense)],
                                     self.cached_ids[:max(1, lay.n_cached)], self.slot_off[:lay.n_cached + 1],
-                                    self.jobs[:_capi.JOB_COLS * max(1, lay.n_job)], self.slots)
+                                    self.jobs[:_capi.JOB_COLS * max(1, lay.n_job)], self.slots, self.block_tables)
         return StepTables(lay, plan, self.positions[:lay.total_rows], self.token_index[:lay.total_rows],
                           self.smp_params, self.smp_rows[:n_win], max((w[2] for w in wins), default=0),
                           self.counts)

@@ -15,6 +15,12 @@ head_dim, scale, num_kv_heads, causal)``, ``.forward(q, k, v)``,
   straight from the paged cache by slot, without the reference's gather and
   concatenation copies.
 
+A cache of 8-bit pages (engine.kv_cache, ``quantized=True``) is written by the
+same selection, its rows quantised on the way, and state 2 then attends over
+the pages.  ``chunk_attention`` is the same attention for callers with their
+own tables: chunks of any length over 8-bit or bf16 pages, bidirectional,
+causal or causal between blocks.
+
 Per step the layer builds one launch plan from ``context.seqs`` (host
 integers only, no device synchronisation) and caches it on the Context, so
 the 32 layers of a forward reuse it.  Every kernel runs on the caller's
@@ -318,6 +324,9 @@ class StepLayout:
         self.n_cached = len(self.cached)
         self.max_q_cached = max((rows[i] for i in self.cached), default=0)
         self.max_keys_cached = max((rows[i] + keeps[i] for i in self.cached), default=0)
+        self.max_keep_cached = max((keeps[i] for i in self.cached), default=0)
+        self.rows_cached = sum(rows[i] for i in self.cached)
+        self.keeps_cached = sum(keeps[i] for i in self.cached)
         self.total_slots = sum(keeps[i] for i in self.cached + self.jobs_idx)
         # a launch over every sequence in batch order gets no id table: the
         # kernels then read a segment's offsets one dependent load earlier
@@ -338,7 +347,8 @@ class StepPlan:
     ``StepPlan.from_device`` wraps tables the device-side builder wrote."""
 
     _SCALARS = ("n_seq", "total_rows", "any_skipped", "n_dense", "max_q_dense", "n_job", "max_kc", "max_keep",
-                "max_blk", "n_cached", "max_q_cached", "max_keys_cached", "dense_identity", "cached_identity")
+                "max_blk", "n_cached", "max_q_cached", "max_keys_cached", "max_keep_cached", "rows_cached",
+                "keeps_cached", "dense_identity", "cached_identity")
 
     def __init__(self, context, device: torch.device, num_kv_heads: int = 0, head_dim: int = 0, num_heads: int = 0,
                  layout: StepLayout | None = None):
@@ -394,6 +404,10 @@ class StepPlan:
         self.cached_ids = dev[o:o + max(1, len(cached))]; o += max(1, len(cached))
         self.slot_off = dev[o:o + slot_off.size]; o += slot_off.size
         self.jobs = dev[o:o + jobs.size]
+        tables = [getattr(seqs[i], "block_table", None) for i in cached]
+        if all(t is not None for t in tables):
+            self._keeps = [keeps[i] for i in cached]
+            self._block_tables = [list(t)[:-(-n // _capi.PAGE_ROWS)] for n, t in zip(self._keeps, tables)]
 
     def _take(self, lay: StepLayout, device) -> None:
         self.device = device
@@ -403,12 +417,18 @@ class StepPlan:
         self._args = {}
         self._packed = {}
         self.last_idx = None
+        self._block_tables = None
+        self._pages = None
 
     @classmethod
-    def from_device(cls, lay: StepLayout, device, cu, dense_ids, cached_ids, slot_off, jobs, slots) -> "StepPlan":
-        """Plan over tables already on the device (written by dllm_step_build)."""
+    def from_device(cls, lay: StepLayout, device, cu, dense_ids, cached_ids, slot_off, jobs, slots,
+                    block_tables=None) -> "StepPlan":
+        """Plan over tables already on the device (written by dllm_step_build).
+        block_tables: int32 [n_seq, max_pages], the cache pages of every
+        sequence (needed with 8-bit pages)."""
         self = cls.__new__(cls)
         self._take(lay, device)
+        self._block_tables = block_tables
         self.cu, self.dense_ids, self.cached_ids = cu, dense_ids, cached_ids
         self.slot_off, self.jobs, self.slots = slot_off, jobs, slots
         return self
@@ -425,6 +445,30 @@ class StepPlan:
             t = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             self._ws[key] = t
         return t
+
+    def page_tables(self):
+        """(page table [n_cached, max_pages], cached lengths [n_cached]) of the
+        state-2 sequences on the device, int32: what attention over 8-bit
+        pages reads instead of the slot lists.  Their rows are the pages' rows in
+        order, as the slot lists of prepare_step and dllm_step_build name them."""
+        if self._pages is None:
+            t = self._block_tables
+            if t is None:
+                raise ValueError("8-bit pages need the sequences' block tables (seq.block_table)")
+            if not isinstance(t, torch.Tensor):
+                width = max(1, -(-self.max_keep_cached // _capi.PAGE_ROWS))
+                host = torch.full((self.n_cached, width), -1, dtype=torch.int32)
+                for r, pages in enumerate(t):
+                    if len(pages) < -(-self._keeps[r] // _capi.PAGE_ROWS):
+                        raise ValueError(f"cached sequence {r}: {self._keeps[r]} rows in {len(pages)} pages")
+                    host[r, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+                if self.device.type == "cuda":
+                    host = host.pin_memory()
+                t = host.to(self.device, non_blocking=True)
+            elif not self.cached_identity:
+                t = t.index_select(0, self.cached_ids)
+            self._pages = t, self.slot_off[1:] - self.slot_off[:-1]
+        return self._pages
 
     def launch_args(self, Hq: int, Hkv: int, D: int) -> dict:
         """Device addresses of the step's tables and the K3b workspace for
@@ -511,6 +555,11 @@ class Attention(nn.Module):
         cache that passed keeps passing while the same tensors keep their
         addresses and sizes."""
         kc, vc = self.k_cache, self.v_cache
+        if kc.dtype == torch.uint8:
+            if _check_pages(kc, vc, device) != self.num_kv_heads or self.head_dim != 128:
+                raise ValueError(f"8-bit pages of {kc.shape[1]} KV heads of 128, the layer has {self.num_kv_heads} of "
+                                 f"{self.head_dim}")
+            return kc.data_ptr(), vc.data_ptr(), min(kc.shape[0], vc.shape[0]) * _capi.PAGE_ROWS
         key = (kc.data_ptr(), vc.data_ptr(), kc.numel(), vc.numel(), device)
         ok = self._cache_ok
         if ok is not None and ok[0]() is kc and ok[1]() is vc and ok[2:7] == key:
@@ -573,8 +622,23 @@ class Attention(nn.Module):
             if not (self.k_cache.numel() and self.v_cache.numel()):
                 raise RuntimeError("cache state 2 needs k_cache/v_cache bound to this layer")
             kc, vc, cache_slots = self._check_cache(dev)
+            if self.k_cache.dtype == torch.uint8:
+                self._attend_pages(plan, args, qp, kp, vp, op, kc, vc, cache_slots, q_st, k_st, v_st, o_st, stream)
+                return o if o.dim() == 2 else o.view(-1, Hq * D)
             _capi.attn_block_cached_fwd_raw(qp, kp, vp, op, args["cu"], args["cached_ids"], plan.n_cached,
                                             plan.max_q_cached, plan.max_keys_cached, kc, vc, cache_slots,
                                             args["slots"], args["slot_off"], Hq, Hkv, D, q_st, k_st, v_st, o_st,
                                             float(self.scale), args["ws"], args["ws_bytes"], stream)
         return o if o.dim() == 2 else o.view(-1, Hq * D)
+
+    def _attend_pages(self, plan, args, qp, kp, vp, op, kc, vc, cache_slots, q_st, k_st, v_st, o_st, stream) -> None:
+        """The state-2 sequences' blocks against their cached rows in 8-bit pages and against themselves."""
+        Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        table, lens = plan.page_tables()
+        sizes = (plan.n_cached, plan.max_q_cached, plan.max_keep_cached)
+        need = _capi.chunk_workspace_size(*sizes, Hq, Hkv, D, plan.rows_cached, plan.keeps_cached)
+        ws = plan.workspace(("pages", Hq, Hkv, D), need)
+        _capi.attn_chunk_paged_fwd_raw(qp, kp, vp, op, args["cu"], args["cached_ids"], *sizes, plan.rows_cached,
+                                       plan.keeps_cached, kc, vc, _capi.CACHE_FP8, cache_slots // _capi.PAGE_ROWS,
+                                       table.data_ptr(), table.shape[1], lens.data_ptr(), 0, Hq, Hkv, D, q_st, k_st, v_st,
+                                       o_st, float(self.scale), None if ws is None else ws.data_ptr(), need, stream)

@@ -316,6 +316,15 @@ int dllm_select_kv_store(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16
                          dllm_bf16* k_cache, dllm_bf16* v_cache, int64_t cache_slots,
                          const int32_t* slots, int64_t n_slots, int64_t* idx_out,
                          void* workspace, size_t workspace_bytes, void* stream);
+/* The same selection, its rows quantised into 8-bit pages as they are copied (as
+ * dllm_store_kvcache_fp8 would store them; num_pages pages of 256 slots). */
+int dllm_select_kv_store_fp8(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, int64_t n_rows,
+                             int64_t q_stride_tok, int64_t k_stride_tok, int64_t v_stride_tok,
+                             const int32_t* jobs, int n_job, int max_kc, int max_keep,
+                             int Hq, int Hkv, int D, float sqrt_d,
+                             uint8_t* k_pages, uint8_t* v_pages, int64_t num_pages,
+                             const int32_t* slots, int64_t n_slots, int64_t* idx_out,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * K7 -- NeoX rotary embedding of q and k in one launch.  Replaces

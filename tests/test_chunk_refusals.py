@@ -143,3 +143,17 @@ def test_chunk_attention_refuses():
         chunk_attention(torch.zeros(3, 4, 64, dtype=BF16), k, k, kc, kc, plan, 0.1)
     with pytest.raises(ValueError, match="contiguous heads"):
         chunk_attention(q.transpose(0, 1).contiguous().transpose(0, 1), k, k, kc, kc, plan, 0.1)
+
+
+def test_quantising_selection_refuses():
+    lib = _capi.load()
+
+    def call(pages=4, kp=FAKE, ws=FAKE, ws_bytes=1 << 30, D=128):
+        return _err(lib.dllm_select_kv_store_fp8(FAKE, FAKE, FAKE, 300, 512, 256, 256, FAKE, 1, 268, 100, 4, 2, D, 11.3,
+                                                 kp, FAKE, pages, FAKE, 100, None, ws, ws_bytes, None))
+    assert call(D=64)[0] == _capi.DLLM_ERR_UNSUPPORTED
+    assert call(pages=-1)[0] == _capi.DLLM_ERR_INVALID_ARG
+    assert call(pages=(1 << 23) + 1)[0] == _capi.DLLM_ERR_INVALID_ARG
+    assert call(kp=ODD)[0] == _capi.DLLM_ERR_INVALID_ARG
+    assert call(kp=None)[0] == _capi.DLLM_ERR_INVALID_ARG
+    assert call(ws_bytes=16)[0] == _capi.DLLM_ERR_WORKSPACE
