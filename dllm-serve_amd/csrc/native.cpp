@@ -173,7 +173,7 @@ PyObject* quant_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // chunk(q, k, v, k_cache, v_cache, plan: bytes, scale) -> output or None.
 struct ChunkTables {
-  int64_t device, rows, n_seg, max_q, max_cached, total_cached, max_pages, max_page, mask_block, cu, lens, tables;
+  int64_t device, rows, n_seg, max_q, max_cached, total_cached, max_pages, max_page, mask_block, cu, lens, tables, seg_ids;
 };
 
 PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -216,7 +216,7 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto dev_i32 = [](int64_t x) { return reinterpret_cast<const int32_t*>(x); };
     const int rc = no_gil([&] {
       return dllm_attn_chunk_paged_fwd(ptr<dllm_bf16>(*t[0]), ptr<dllm_bf16>(*t[1]), ptr<dllm_bf16>(*t[2]),
-                                       ptr<dllm_bf16>(o), dev_i32(p.cu), nullptr, (int)p.n_seg, (int)p.max_q,
+                                       ptr<dllm_bf16>(o), dev_i32(p.cu), dev_i32(p.seg_ids), (int)p.n_seg, (int)p.max_q,
                                        (int)p.max_cached, p.rows, p.total_cached, kc->data_ptr(), vc->data_ptr(), kind,
                                        (int)pages, dev_i32(p.tables), (int)p.max_pages, dev_i32(p.lens),
                                        (int)p.mask_block, (int)Hq, (int)Hkv, 128, t[0]->stride(0), t[1]->stride(0),

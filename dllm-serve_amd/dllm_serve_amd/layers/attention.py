@@ -152,7 +152,15 @@ class ChunkPlan:
     needed are fine).  ``mask_block`` 0: the new rows see each other; b >= 1:
     a row sees the rows up to the end of its own block of b positions
     (1: causal), positions counted from the first cached row.  The tables are
-    uploaded with one asynchronous copy; nothing synchronises."""
+    uploaded with one asynchronous copy; nothing synchronises.
+
+    ``cached_lens`` and ``block_tables`` are in the order of the launch, which is
+    the sequences' own unless they feed _SORT_ROWS rows together: then those with
+    the most keys come first, so that no long workgroup starts when the others end."""
+
+    # The order costs a dependent load at the start of every workgroup, which only
+    # pieces of prompts are long enough not to feel.
+    _SORT_ROWS = 512
 
     def __init__(self, seqlens, cached_lens, block_tables, device, mask_block: int = 0):
         seqlens, cached = [int(n) for n in seqlens], [int(n) for n in cached_lens]
@@ -174,24 +182,30 @@ class ChunkPlan:
         self.max_pages = W = max(need, default=0)
         self.max_page = max((p for t, n in zip(tables, need) for p in t[:n]), default=-1)
         self.mask_block = int(mask_block)
-        flat = np.full(2 * B + 1 + B * W, -1, dtype=np.int64)
+        order = list(range(B))
+        if self.total_rows >= self._SORT_ROWS:
+            order.sort(key=lambda b: -(seqlens[b] + cached[b]))  # stable
+        flat = np.full(3 * B + 1 + B * W, -1, dtype=np.int64)
         flat[0] = 0
         flat[1:B + 1] = np.cumsum(seqlens)
-        flat[B + 1:2 * B + 1] = cached
-        for b, (t, n) in enumerate(zip(tables, need)):
-            flat[2 * B + 1 + b * W:2 * B + 1 + b * W + n] = t[:n]
+        flat[B + 1:2 * B + 1] = [cached[b] for b in order]
+        flat[2 * B + 1:3 * B + 1] = order
+        for i, b in enumerate(order):
+            flat[3 * B + 1 + i * W:3 * B + 1 + i * W + need[b]] = tables[b][:need[b]]
         if flat.max() >= 2**31:
             raise ValueError("chunk tables exceed int32")
         host = torch.from_numpy(flat.astype(np.int32))
         if self.device.type == "cuda":
             host = host.pin_memory()
         dev = host.to(self.device, non_blocking=True)
-        self.cu, self.cached_lens, self.block_tables = dev[:B + 1], dev[B + 1:2 * B + 1], dev[2 * B + 1:]
+        self.cu, self.cached_lens, self.block_tables = dev[:B + 1], dev[B + 1:2 * B + 1], dev[3 * B + 1:]
+        self._seg_ids = None if order == sorted(order) else dev[2 * B + 1:].data_ptr()
         self._args = (self.cu.data_ptr(), self.cached_lens.data_ptr(), self.block_tables.data_ptr())
         # the same for the native form (csrc/native.cpp, ChunkTables)
         self._packed = struct.pack(
-            "=12q", -1 if self.device.index is None else self.device.index, self.total_rows, B, self.max_q,
-            self.max_cached, self.total_cached, W, self.max_page, self.mask_block, *self._args)
+            "=13q", -1 if self.device.index is None else self.device.index, self.total_rows, B, self.max_q,
+            self.max_cached, self.total_cached, W, self.max_page, self.mask_block, *self._args,
+            self._seg_ids or 0)
 
 
 def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -250,9 +264,9 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
         if nq:
             cu, lens, tables = plan._args
             _capi.attn_chunk_paged_fwd_raw(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, None, plan.n_seg, plan.max_q,
-                plan.max_cached, plan.total_rows, plan.total_cached, k_cache.data_ptr(), v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens,
-                plan.mask_block, Hq, Hkv, D, q_st, k_st, v_st, o.stride(0), float(softmax_scale),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, plan._seg_ids, plan.n_seg,
+                plan.max_q, plan.max_cached, plan.total_rows, plan.total_cached, k_cache.data_ptr(),
+                v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens, plan.mask_block, Hq, Hkv, D, q_st, k_st, v_st, o.stride(0), float(softmax_scale),
                 None if ws is None else ws.data_ptr(), need, _capi._stream(dev))
     return o
 

@@ -363,3 +363,29 @@ def test_a_prompt_in_chunks_is_the_prompt_at_once(dev, mask_block):
     load_kvcache(ko, vo, kc, vc, (torch.tensor(table)[pos // 256] * 256 + pos % 256).to(torch.int32).to(dev))
     assert np.array_equal(_np(ko), quant.dequantise(*quant.quantise(_np(k[:at]))))
     assert np.array_equal(_np(vo), quant.dequantise(*quant.quantise(_np(v[:at]))))
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_pieces_are_launched_longest_first(dev, bits, monkeypatch):
+    """512 rows and more: the sequences in another order, here over several turns of the
+    order of the M tiles, both sides of the native call, from a graph as well."""
+    b = Batch(dev, [40, 0, 300, 1, 200, 260], [10, 5, 0, 520, 700, 30], 48, 48, bits, seed=21)
+    plan = ChunkPlan(b.lens, b.cached, b.tables, dev, mask_block=1)
+    assert plan._seg_ids is not None and plan.cached_lens.tolist() == [700, 520, 0, 30, 10, 5]
+    shape = _capi.chunk_launch_shape(6, plan.max_q, plan.max_cached, 48, 48, 128, plan.total_rows, plan.total_cached)
+    assert shape["rows"] == 128 and shape["n_split"] == 1 and shape["grid"] > 512
+    want = b.run(1)
+    b.verify(want, 1)
+    b.verify(b.run(0), 0)
+    q, k, v = b.q.to(dev), b.k.to(dev), b.v.to(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE), want)
+    monkeypatch.setattr(_capi, "native", None)
+    assert torch.equal(b.run(1), want)
