@@ -696,7 +696,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // bytes a thread and matrix), converted and written to the other stage after the
 // products -- once per workgroup, not once per wavefront.  Two workgroups fit a CU, so
 // that one computes while the other one waits at its barrier (eight wavefronts in one
-// workgroup: 2048 rows behind 6144 cached, 32 heads, 381 against 333 us).
+// workgroup: 2048 rows behind 6144 cached, 32 heads, 289 against 296 us, but 8 ragged
+// pieces, 28/4 heads, 147 against 139, 5 ragged ones, 32 heads, 212 against 199).
+// The bf16 form also runs into what a CU takes in, 32 KB a tile and workgroup; V reads
+// in one block that leaves the next tile's loads in flight were no faster.
 constexpr int kTileRows = 128;
 constexpr int kTileStage = 2 * kBigTile * 256;
 template <bool FP8>
@@ -886,6 +889,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     issue_new(stage_of(t0), t0);
     tile_done();
   }
+  // Q is waited for here: the compiler would else do so in every turn, and with it for
+  // the next tile's loads (8192 new rows, 32 heads, 8-bit, 684 -> 662 us).
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(qf[kk]));
   bool fixed = false;
   for (int t = t0; t < t1; ++t) {
     uint8_t* const cur = stage_of(t);
