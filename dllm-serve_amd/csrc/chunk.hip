@@ -21,6 +21,7 @@
 #include "quant.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace dllm {
 
@@ -49,18 +50,24 @@ struct Segment {
   int row0, len, cached;
 };
 
-// New rows that new row t sees.
+// New rows that new row t sees.  With r = n % b, the end of t's block is
+// ((r + t) / b + 1) b - r: divisions of 32 bits (one of 64 is over a hundred
+// instructions, and every wavefront starts with some).
 __device__ __forceinline__ int visible(const Segment& g, int t, int mask_block) {
   if (mask_block == 0) return g.len;
-  const int64_t end = (((int64_t)g.cached + t) / mask_block + 1) * mask_block - g.cached;
-  return (int)min((int64_t)g.len, end);
+  if (mask_block == 1) return min(g.len, t + 1);
+  const uint32_t b = (uint32_t)mask_block, r = (uint32_t)g.cached % b;
+  const uint32_t blocks = (r + (uint32_t)t) / b + 1;  // r < 2^31, t < 2^30
+  return (int)min((uint64_t)g.len, (uint64_t)blocks * b - r);
 }
 
 // Splits that hold keys of the M tile whose last token is `last` (at least one).  The
 // rows form deals the cached tiles alone, the new rows belonging to the last split; the
 // tile form the cached tiles and those of the new rows that the M tile sees.
 template <bool TILE>
-__device__ __forceinline__ int splits_of(const ChunkArgs& a, int tiles_per_split, const Segment& g, int last) {
+__device__ __forceinline__ int splits_of(const ChunkArgs& a, int max_split, int tiles_per_split, const Segment& g,
+                                         int last) {
+  if (max_split == 1) return 1;
   int tiles;
   if (TILE)
     tiles = (g.cached + kBigTile - 1) / kBigTile + (visible(g, last, a.mask_block) + kBigTile - 1) / kBigTile;
@@ -87,17 +94,29 @@ __device__ __forceinline__ int splits_of(const ChunkArgs& a, int tiles_per_split
 struct Work {
   int s, hkv, split, mt;
 };
+// r % n, and r / n left in r; a division is some twenty instructions at the start of
+// every wavefront, and n is often one.
+__device__ __forceinline__ int take(uint32_t& r, int n) {
+  if (n == 1) return 0;
+  const uint32_t x = r, q = x / (uint32_t)n;
+  r = q;
+  return (int)(x - q * (uint32_t)n);
+}
 __device__ __forceinline__ Work work_of(int L, int mtiles, int max_split, int Hkv) {
   Work w;
   uint32_t r = (uint32_t)L;
-  w.mt = (int)(r % (uint32_t)mtiles);
-  r /= (uint32_t)mtiles;
-  w.split = (int)(r % (uint32_t)max_split);
-  r /= (uint32_t)max_split;
-  w.hkv = (int)(r % (uint32_t)Hkv);
-  w.s = (int)(r / (uint32_t)Hkv);
+  w.mt = take(r, mtiles);
+  w.split = take(r, max_split);
+  w.hkv = take(r, Hkv);
+  w.s = (int)r;
   return w;
 }
+__device__ __forceinline__ int block_of(int chunk_pages) {
+  const int chunk = chunk_pages & 31;
+  return chunk == 1 ? (int)blockIdx.x : xcd_remap(blockIdx.x, chunk);
+}
+// Token of M row m (m >= 0).
+__device__ __forceinline__ int token_of(int m, int g) { return (int)((uint32_t)m / (uint32_t)g); }
 // The M tile of a workgroup of the tile form.  The last M tiles, which see the most keys
 // under a causal mask, come first, but first and last in turn from one 256 workgroups (one
 // a CU) to the next, so that a CU's workgroups come out even: 8192 new rows, 32 heads,
@@ -109,10 +128,19 @@ __device__ __forceinline__ Segment segment(const ChunkArgs& a, const int32_t* cu
                                            const int32_t* lens, int s) {
   Segment g;
   const int id = seg_ids ? seg_ids[s] : s;
-  g.row0 = cu[id];
+  int c0 = cu[id], c1 = cu[id + 1], n = lens[s];
+  // These and the arguments are waited for once: loaded where they are first used, they
+  // would make a chain of four loads at the start of every workgroup.  (This, the short
+  // divisions and the waits below: one token behind 32 rows 5.85 -> 4.7 us, behind 511 10.1
+  // -> 8.6, 32 ragged ones, 28/4 heads, 25.0 -> 22.7.)
+  asm volatile(""
+               : "+s"(c0), "+s"(c1), "+s"(n)
+               : "s"(a.q), "s"(a.k), "s"(a.v), "s"(a.o), "s"(a.kc), "s"(a.vc), "s"(a.ws), "s"(a.q_stride),
+                 "s"(a.k_stride), "s"(a.v_stride), "s"(a.o_stride), "s"(a.cache_rows));
+  g.row0 = c0;
   // no more than the launch was sized for
-  g.len = min(max(cu[id + 1] - g.row0, 0), a.max_q);
-  g.cached = min(max(lens[s], 0), a.max_cached);
+  g.len = min(max(c1 - c0, 0), a.max_q);
+  g.cached = min(max(n, 0), a.max_cached);
   return g;
 }
 
@@ -310,25 +338,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int BM = 16 * NB;
   constexpr int PARK = park_floats(NB);
   extern __shared__ __attribute__((aligned(16))) float lds[];  // rows_lds() bytes
-  const int L = xcd_remap(blockIdx.x, chunk_pages & 31);
+  const int L = block_of(chunk_pages);
   if (L >= logical_blocks) return;
   const int max_pages = chunk_pages >> 5;
   const Work wk = work_of(L, mtiles, max_split, Hkv);
   const int s = wk.s, hkv = wk.hkv, split = wk.split;
   const int lane = threadIdx.x & 63;
-  const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
   const int t_begin = split * tiles_per_split;
   // Page ids of the split, one a lane (a split spans at most 63): a tile's loads
   // then wait for no load of their own.  Their address needs no other load either.
   const int pg0 = t_begin * kTileKeys / kPageRows;
-  const int page_reg = n_pages > 0 && max_pages > 0
-                           ? table[(int64_t)s * max_pages + min(pg0 + lane, max_pages - 1)] : -1;
+  int page_reg = max_pages > 0 ? table[(int64_t)s * max_pages + min(pg0 + lane, max_pages - 1)] : -1;
   const Segment sg = segment(a, cu, seg_ids, lens, s);
+  const uint32_t n_pages = (uint32_t)min(a.cache_rows >> 8, (int64_t)1 << 23);
   const int g = a.g;
   const int M = sg.len * g;
   const int m_base = wk.mt * BM;
   if (m_base >= M) return;
-  const int ns = splits_of<false>(a, tiles_per_split, sg, sg.len - 1);
+  const int ns = splits_of<false>(a, max_split, tiles_per_split, sg, sg.len - 1);
   if (split >= ns) return;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -338,6 +365,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int tiles = (sg.cached + kTileKeys - 1) / kTileKeys;
   const int t_end = n_pages ? min(tiles, t_begin + tiles_per_split) : t_begin;  // no cache: nothing to read
   const uint32_t bf_row = (uint32_t)(Hkv * HD * 2);
+
+  // The page ids, sent for first, have arrived when the lengths have.  Waited for here,
+  // alone: at their first use the compiler would wait for all that is in flight by then.
+  asm volatile("" : "+v"(page_reg));
 
   // ---- Q^T operands and the rows' limits ------------------------------------
   bf16x8_t qf[NB][4];
@@ -349,7 +380,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int m = m_base + 16 * b + col;
-      const int tok = m / g;
+      const int tok = token_of(m, g);
       lim[b] = visible(sg, min(tok, sg.len - 1), a.mask_block);
       const uint32_t base = m < M ? (uint32_t)tok * qS + (uint32_t)((hkv * g + m - tok * g) * HD) * 2u : qbytes;
 #pragma unroll
@@ -368,10 +399,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   // DMA of cached tile t into a stage; rows past the cached length, and all rows of a
   // page outside the cache, arrive as zeros through the buffer's bound.
-  auto issue = [&](uint8_t* stage, int t) {
+  auto issue = [&](uint8_t* stage, int t, bool exists = true) {
     const int pid = page_of(t);
     const int row0 = t * kTileKeys & (kPageRows - 1);
-    const int rows = pid < 0 ? 0 : min(sg.cached - t * kTileKeys, kTileKeys);
+    const int rows = pid < 0 || !exists ? 0 : min(sg.cached - t * kTileKeys, kTileKeys);
     if constexpr (FP8) {
       const int64_t rec = ((int64_t)max(pid, 0) * Hkv + hkv) * kRecord;
       const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.kc + rec + row0 * kQuantD, (uint32_t)rows * kQuantD);
@@ -386,7 +417,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       // lanes 0 .. 7: K's scale bytes, 8 .. 15: V's (the others repeat them)
       const uint8_t* sp = (lane & 8 ? a.vc : a.kc) + rec + kScaleOff + row0 + (lane & 7) * 4;
-      __builtin_amdgcn_global_load_lds(sp, (__attribute__((address_space(3))) void*)(stage + T::kScales), 4, 0, 0);
+      // (in asm: after the builtin, which the compiler takes for an access that ends out of
+      // order, it waits for all that is in flight wherever it waits for anything)
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(stage + T::kScales);
+      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(sp) : "m0", "memory");
     } else {
       const int64_t off0 = ((int64_t)max(pid, 0) * kPageRows + row0) * bf_row + hkv * HD * 2;
       const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * bf_row + HD * 2 : 0u;
@@ -512,32 +546,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // Before the cached tiles: their loads are among the first, beside the first tile's DMA.
   const int n = max(0, (t_end - t_begin - wave + 3) >> 2);  // this wavefront's cached tiles
   const int first = t_begin + wave;
-  bool fixed = false, started = false;
+  bool fixed = false;
   const uint32_t vS = (uint32_t)(a.v_stride * 2), vb = (uint32_t)(sg.len - 1) * vS + HD * 2;
   const __amdgpu_buffer_rsrc_t vrs = make_rsrc(a.v + (int64_t)sg.row0 * a.v_stride + hkv * HD, vb);
   const int turn = max(t_end - t_begin, 0);
+  if (n > 0) issue(my, first);
   if (split == ns - 1) {
     const uint32_t kS = (uint32_t)(a.k_stride * 2), kb = (uint32_t)(sg.len - 1) * kS + HD * 2;
     const __amdgpu_buffer_rsrc_t krs = make_rsrc(a.k + (int64_t)sg.row0 * a.k_stride + hkv * HD, kb);
     // the furthest new row that any of this workgroup's rows sees
     const int last = min(m_base + BM, M) - 1;
-    const int see = visible(sg, last / g, a.mask_block);
+    const int see = visible(sg, token_of(last, g), a.mask_block);
     const int new_tiles = (see + kTileKeys - 1) / kTileKeys;
     for (int t = (wave - turn) & 3; t < new_tiles; t += 4) {
       bf16x8_t kx[2][4];
       u32x4_t vx[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t row = (uint32_t)(t * kTileKeys + 16 * u + col);
+        // rows that do not exist start past the bound and arrive as zeros
+        const uint32_t row = (uint32_t)min(t * kTileKeys + 16 * u + col, sg.len);
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
           const uint32_t off = FP8 ? (uint32_t)((k4 >> 1) * 128 + g4 * 32 + (k4 & 1) * 16) : (uint32_t)(k4 * 64 + g4 * 16);
-          kx[u][k4] = as_bf16x8(bload(krs, row < (uint32_t)sg.len ? row * kS + off : kb, 0u));
-          vx[u][k4] = bload(vrs, row < (uint32_t)sg.len ? row * vS + (uint32_t)(k4 * 64 + g4 * 16) : vb, 0u);
+          kx[u][k4] = as_bf16x8(bload(krs, row * kS + off, 0u));
+          vx[u][k4] = bload(vrs, row * vS + (uint32_t)(k4 * 64 + g4 * 16), 0u);
         }
       }
-      if (!started && n > 0) issue(my, first);
-      started = true;
       // A NaN or infinity in a V row that some M row does not see would reach that row
       // as 0 * V.  Such elements (rare) are multiplied as zeros and added at the end
       // to the rows that see them.
@@ -585,18 +619,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 
   // ---- cached tiles: this wavefront takes every fourth, two in flight --------------
-  {
-    asm volatile("" ::: "memory");  // the page ids and q stay the oldest operations
-    wave_lds_fence();               // the new rows' V has been read
-    if (!started && n > 0) issue(my, first);
-    if (n > 1) issue(my + T::kStage, first + 4);
-    // q has landed, the tiles may be in flight
-    if (n > 1)
-      vm_wait<2 * T::kOps>();
-    else if (n == 1)
-      vm_wait<T::kOps>();
-    else
-      vm_wait<0>();
+  if (n > 0) {
+    wave_lds_fence();  // the new rows' V has been read
+    issue(my + T::kStage, first + 4, n > 1);  // no second tile: as many operations, all zeros
+    // Q has landed, both tiles may be in flight.  (Where the compiler has to join paths with
+    // different operations, it waits for the tiles as well.)
+    vm_wait<2 * T::kOps>();
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) asm volatile("" : "+v"(qf[b][k4]));
     for (int i = 0; i < n; ++i) {
       if (i + 1 < n)
         vm_wait<T::kOps>();
@@ -661,7 +693,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mu);
     lsum += ml[(w * 2 + 1) * BM + row] * f[w];
   }
-  const int tok = m / g, head = hkv * g + (m - tok * g);
+  const int tok = token_of(m, g), head = hkv * g + (m - tok * g);
   const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
 #pragma unroll
   for (int j = 0; j < DPT / 4; ++j) {
@@ -710,7 +742,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int PER = TK * 8 / 256;          // 8-bit rows: 16-byte pieces of one matrix and thread
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
   uint8_t* const lds = reinterpret_cast<uint8_t*>(lds_f);  // two stages
-  const int L = xcd_remap(blockIdx.x, chunk_pages & 31);
+  const int L = block_of(chunk_pages);
   if (L >= logical_blocks) return;
   const int max_pages = chunk_pages >> 5;
   const Work wk = work_of(L, mtiles, max_split, Hkv);
@@ -720,8 +752,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int M = sg.len * g;
   const int m_base = tile_of(wk, L, mtiles, max_split) * BM;
   if (m_base >= M) return;
-  const int tok_first = m_base / g, tok_last = (min(m_base + BM, M) - 1) / g;
-  const int ns = splits_of<true>(a, tiles_per_split, sg, tok_last);
+  const int tok_first = token_of(m_base, g), tok_last = token_of(min(m_base + BM, M) - 1, g);
+  const int ns = splits_of<true>(a, max_split, tiles_per_split, sg, tok_last);
   if (wk.split >= ns) return;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -815,21 +847,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   bf16x8_t qf[8];
   const int m_lane = m_base + wave * 32 + lrow;
-  const int lim = visible(sg, min(m_lane / g, sg.len - 1), a.mask_block);
+  const int lim = visible(sg, min(token_of(m_lane, g), sg.len - 1), a.mask_block);
   {
     const uint32_t qS = (uint32_t)(a.q_stride * 2);
     const uint32_t qbytes = (uint32_t)sg.len * qS;
     const __amdgpu_buffer_rsrc_t qrs = make_rsrc(a.q + (int64_t)sg.row0 * a.q_stride, qbytes);
-    const int tok = m_lane / g;
+    const int tok = token_of(m_lane, g);
     const bool ok = m_lane < M;
     const uint32_t qoff = (uint32_t)tok * qS + (uint32_t)((hkv * g + m_lane - tok * g) * HD + hl * 8) * 2u;
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) qf[kk] = as_bf16x8(bload(qrs, ok ? qoff + (uint32_t)kk * 32u : qbytes, 0u));
   }
   // of this wavefront's rows: the least and the most that any sees
-  const int lim_lo = __builtin_amdgcn_readfirstlane(visible(sg, min((m_base + wave * 32) / g, sg.len - 1), a.mask_block));
+  const int lim_lo = __builtin_amdgcn_readfirstlane(visible(sg, min(token_of(m_base + wave * 32, g), sg.len - 1), a.mask_block));
   const int lim_hi =
-      __builtin_amdgcn_readfirstlane(visible(sg, (min(m_base + wave * 32 + 32, M) - 1) / g, a.mask_block));
+      __builtin_amdgcn_readfirstlane(visible(sg, token_of(min(m_base + wave * 32 + 32, M) - 1, g), a.mask_block));
   const bool live = m_base + wave * 32 < M;
 
   DenseAddr ad;
@@ -892,7 +924,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // Q is waited for here: the compiler would else do so in every turn, and with it for
   // the next tile's loads (8192 new rows, 32 heads, 8-bit, 684 -> 662 us).
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(qf[kk]));
+  for (int kk = 0; kk < 8; ++kk) asm volatile("" : : "v"(qf[kk]));
   bool fixed = false;
   for (int t = t0; t < t1; ++t) {
     uint8_t* const cur = stage_of(t);
@@ -992,7 +1024,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int row = 4 * j + rl, m = m_base + wave * 32 + row;
     const u32x4_t v = *reinterpret_cast<const u32x4_t*>(ot + row * 256 + ((P ^ (row & 15)) * 16));
     if (m < M) {
-      const int tok = m / g;
+      const int tok = token_of(m, g);
       st128(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + (hkv * g + m - tok * g) * HD + P * 8, v);
     }
   }
@@ -1013,28 +1045,54 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
   // grid: rows of the largest segment, KV heads, segments
   const int mrow = blockIdx.x * (8 / G) + grp / G;
   const int hkv = blockIdx.y, s = blockIdx.z;
-  const Segment sg = segment(a, cu, seg_ids, lens, s);
-  if (mrow >= sg.len * a.g) return;
   const int mt = mrow / BM, row = mrow % BM;
-  const int parts = splits_of<TILE>(a, tiles_per_split, sg, TILE ? (min((mt + 1) * BM, sg.len * a.g) - 1) / a.g : 0);
-  if (parts == 1) return;
+  if (mt >= mtiles) return;
   // part p of this row: workgroup L0 + p * mtiles (the tile form counts its M tiles from the last)
   const int L0 = (s * Hkv + hkv) * max_split * mtiles + (TILE ? mtiles - 1 - mt : mt);
-  float mx = -INFINITY;
-#pragma unroll 8
-  for (int p = sub; p < parts; p += G) mx = fmaxf(mx, part_ml<BM>(a, logical_blocks, L0 + p * mtiles, row)[0]);
-  const float mu = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int p = sub; p < parts; p += G) {
-    const int at = L0 + p * mtiles;
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(part_o<BM>(a, at, row) + d0);
-    const float* const ml = part_ml<BM>(a, logical_blocks, at, row);
-    const float w = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mu);
-    l += ml[1] * w;
+  // A round of eight parts; those past the end, which hold anything, are left out after.
+  f32x4_t x[8];
+  float pm[8], pl[8];
+  auto fetch = [&](int p0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
+    for (int i = 0; i < 8; ++i) {
+      const int at = L0 + min(p0 + i * G, max_split - 1) * mtiles;
+      x[i] = *reinterpret_cast<const f32x4_t*>(part_o<BM>(a, at, row) + d0);
+      const float* const ml = part_ml<BM>(a, logical_blocks, at, row);
+      pm[i] = ml[0];
+      pl[i] = ml[1];
+    }
+  };
+  fetch(sub);  // before the lengths that tell how many there are
+  const Segment sg = segment(a, cu, seg_ids, lens, s);
+  const int M = sg.len * a.g;
+  const int parts = splits_of<TILE>(a, max_split, tiles_per_split, sg,
+                                    TILE ? token_of(min((mt + 1) * BM, max(M, 1)) - 1, a.g) : 0);
+  float mx = -INFINITY, l = 0.f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int p0 = sub;;) {
+    float top = mx;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (p0 + i * G >= parts) pm[i] = -INFINITY;
+      top = fmaxf(top, pm[i]);
+    }
+    const float mu = top == -INFINITY ? 0.f : top;
+    const float w0 = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mu);
+    l *= w0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= w0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (pm[i] != -INFINITY) {
+        const float w = __builtin_amdgcn_exp2f(pm[i] - mu);
+        l += pl[i] * w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += x[i][e] * w;
+      }
+    mx = top;
+    p0 += 8 * G;
+    if (p0 >= parts) break;
+    fetch(p0);
   }
   if constexpr (G > 1) {
     part[threadIdx.x] = acc;
@@ -1043,7 +1101,6 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
       part_s[2 * sub + 1] = l;
     }
     __syncthreads();
-    if (sub) return;
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < G; ++i) top = fmaxf(top, part_s[2 * i]);
@@ -1059,8 +1116,9 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
       for (int e = 0; e < 4; ++e) acc[e] += x[e] * w;
     }
   }
+  if (mrow >= M || parts == 1 || sub) return;  // one part: its workgroup wrote the row
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  const int tok = mrow / a.g, head = hkv * a.g + (mrow - tok * a.g);
+  const int tok = token_of(mrow, a.g), head = hkv * a.g + (mrow - tok * a.g);
   const u32x2_t w2 = {cvt_pk_bf16(acc[0] * inv, acc[1] * inv), cvt_pk_bf16(acc[2] * inv, acc[3] * inv)};
   *reinterpret_cast<u32x2_t*>(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + head * HD + d0) = w2;
 }
@@ -1226,7 +1284,7 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
   }
   int chunk;
   const int grid = chunk_grid(p, &chunk);
-  const int chunk_pages = chunk + 32 * (max_cached > 0 ? max_pages : 0);
+  const int chunk_pages = chunk + 32 * (max_cached > 0 && num_pages > 0 ? max_pages : 0);
   auto start = [&](auto kern, dim3 blocks, int lds_bytes) {
     kern<<<blocks, dim3(256), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
         cu, seg_ids, cached_len, page_table, chunk_pages, (int)p.logical, p.mtiles, p.max_split, p.tiles_per_split, Hkv, a);
