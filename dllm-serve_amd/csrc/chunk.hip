@@ -1153,17 +1153,29 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   const int64_t all_t =
       std::min(n_seg * tiles, p.tile_form ? (total_cached + total_q + 2 * (key - 1) * n_seg) / key
                                           : (total_cached + (key - 1) * n_seg) / key);
-  // Keys are split where the work, dealt evenly to one workgroup a CU (tiles: two, whose
-  // phases overlap), gives each at most half of the longest segment.  A CU takes in
-  // about 27 KB a microsecond however many workgroups it has, and every further one
-  // pays for its start and the joining (8 x 32 rows behind 608 - 1216, 32/32 heads, 256
-  // workgroups: 20 us, split in two 30).  Few keys are not split: the joining takes 4
-  // us, a turn of the rows form's wavefronts (four tiles) 0.8: one token behind
-  // 511 rows 9.9 us whole, 11.4 in two.
-  const int64_t least = p.tile_form ? 4 : 8;
-  int64_t tps = (int64_t)((double)all_m * (double)all_t / (double)n_seg * Hkv / (p.tile_form ? 512 : 256) + 0.999);
-  if (tps < least) tps = least;
-  if (tps * 2 > tiles || tiles <= (p.tile_form ? 8 : 24)) tps = tiles;
+  // Keys are split where that shortens the longest workgroup: tile form, to half or less;
+  // rows form, to two thirds.  Every workgroup pays for its start and the joining (8 x 32
+  // rows behind 608 - 1216, 32/32 heads, 256 workgroups: 20 us, split in two 30), and few
+  // keys are not split: the joining takes 3 us, a turn of the rows form's wavefronts (four
+  // tiles) 0.8: one token behind 511 rows 8.6 us whole, 8.8 in four, behind 1000 9.5 in eight.
+  // Tile form: the work dealt to two workgroups a CU, whose phases overlap.  Rows form,
+  // sequences of one length: as many parts as give every CU one workgroup (one token behind
+  // 131071, 28/4 heads: 256 workgroups 29.6 us, 384 34, 512 31).  Of different lengths:
+  // 384 workgroups, half a part each lost to the last ones, of 12 tiles at least (32
+  // single tokens, 28/4 heads: at most 256 workgroups 24.7 us, 384 21.4; 40 of them 51.6 and 39.5,
+  // with 448 44.7; eight shorter ones 11.2, in parts of 8 tiles 12.9).
+  const int64_t groups = all_m * Hkv;  // (M tile, KV head) pairs, each with its own parts
+  const double work = (double)groups * (double)all_t / (double)n_seg;
+  int64_t tps;
+  if (p.tile_form) {
+    tps = std::max<int64_t>((int64_t)(work / 512 + 0.999), 4);
+  } else if (total_cached == n_seg * max_cached) {
+    const int64_t parts = std::max<int64_t>(1, 256 / groups);
+    tps = std::max<int64_t>((tiles + parts - 1) / parts, 4);
+  } else {
+    tps = groups < 768 ? std::max<int64_t>((int64_t)(work / (384 - 0.5 * (double)groups) + 0.999), 12) : tiles;
+  }
+  if (p.tile_form ? tps * 2 > tiles || tiles <= 8 : tps * 3 > tiles * 2 || tiles <= 24) tps = tiles;
   if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
   if (tps < 1) tps = 1;
   if (tps > 0x3fffffff) tps = 0x3fffffff;
