@@ -4,23 +4,22 @@
 // Sixteen lanes carry one (token, KV head) row of K and of V, eight elements each:
 // one 16-byte load, the row's maximum by four cross-lane steps, one 8-byte store
 // (the sixteen lanes write a whole 128-byte line), and one lane's scale byte.  The
-// reverse reads 8 bytes and the scale and writes 16.  Both are bound by memory: 516
-// bytes read and written per row and matrix pair for 258 on the other side.
+// reverse reads 8 bytes and the scale and writes 16.  Both are bound by memory: 512
+// bytes per row of K and V on one side, 258 on the other.
 #include "quant.h"
 
 namespace dllm {
 
-struct QuantArgs {
-  uint16_t* k;  // token rows (read by the store, written by the load)
-  uint16_t* v;
-  uint8_t* kp;  // pages
-  uint8_t* vp;
-  const int32_t* slot;
-  int64_t k_stride, v_stride;  // elements
-  int64_t n_slots;
-  int rows, Hkv;               // rows = n_tok * Hkv
-  int chunk;                   // consecutive workgroups of an XCD
-};
+// Leading scalar arguments (13 dwords): the library is built with kernel argument
+// preloading, so a wave's first loads wait for no load of their addresses.
+//   slot, k, v   slots; token rows (read by the store, written by the load)
+//   rows         n_tok * Hkv
+//   chunk        consecutive workgroups of an XCD
+//   *_stride     elements
+//   kp, vp       pages
+#define QUANT_PARAMS                                                                                     \
+  const int32_t *__restrict__ slots, uint16_t *__restrict__ k, uint16_t *__restrict__ v, int rows, int Hkv, \
+      int chunk, int64_t k_stride, int64_t v_stride, uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n_slots
 
 template <bool VEC>
 __device__ __forceinline__ u32x4_t ld_row8(const uint16_t* p) {
@@ -46,8 +45,8 @@ __device__ __forceinline__ void st_row8(uint16_t* p, u32x4_t x) {
 // U rows of sixteen lanes in flight; a workgroup takes 16 U consecutive (token,
 // head) rows.
 template <bool VEC, int U>
-__global__ __launch_bounds__(256) void kv_quant_store(QuantArgs a) {
-  const int L = (int)(blockIdx.x & 7) * a.chunk + (int)(blockIdx.x >> 3);
+__global__ __launch_bounds__(256) void kv_quant_store(QUANT_PARAMS) {
+  const int L = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
   const int lane16 = threadIdx.x & 15;
   const int row0 = L * 16 * U + (threadIdx.x >> 4);
   u32x4_t kx[U], vx[U];
@@ -59,13 +58,13 @@ __global__ __launch_bounds__(256) void kv_quant_store(QuantArgs a) {
     slot[u] = -1;
     head[u] = 0;
     kx[u] = vx[u] = u32x4_t{0, 0, 0, 0};
-    if (row < a.rows) {
-      const int tok = (int)((uint32_t)row / (uint32_t)a.Hkv);
-      head[u] = row - tok * a.Hkv;
+    if (row < rows) {
+      const int tok = (int)((uint32_t)row / (uint32_t)Hkv);
+      head[u] = row - tok * Hkv;
       const int64_t e = (int64_t)head[u] * kQuantD + lane16 * 8;
-      slot[u] = a.slot[tok];
-      kx[u] = ld_row8<VEC>(a.k + (int64_t)tok * a.k_stride + e);
-      vx[u] = ld_row8<VEC>(a.v + (int64_t)tok * a.v_stride + e);
+      slot[u] = slots[tok];
+      kx[u] = ld_row8<VEC>(k + (int64_t)tok * k_stride + e);
+      vx[u] = ld_row8<VEC>(v + (int64_t)tok * v_stride + e);
     }
   }
 #pragma unroll
@@ -73,21 +72,21 @@ __global__ __launch_bounds__(256) void kv_quant_store(QuantArgs a) {
     uint32_t kb, vb;
     const u32x2_t kc = quant_row16(kx[u], kb);
     const u32x2_t vc = quant_row16(vx[u], vb);
-    if (slot[u] < 0 || slot[u] >= a.n_slots) continue;
-    const int64_t rec = record_off((uint32_t)slot[u], a.Hkv, head[u]);
+    if (slot[u] < 0 || slot[u] >= n_slots) continue;
+    const int64_t rec = record_off((uint32_t)slot[u], Hkv, head[u]);
     const int r = (int)(slot[u] & (kPageRows - 1));
-    *reinterpret_cast<u32x2_t*>(a.kp + rec + r * kQuantD + lane16 * 8) = kc;
-    *reinterpret_cast<u32x2_t*>(a.vp + rec + r * kQuantD + lane16 * 8) = vc;
+    *reinterpret_cast<u32x2_t*>(kp + rec + r * kQuantD + lane16 * 8) = kc;
+    *reinterpret_cast<u32x2_t*>(vp + rec + r * kQuantD + lane16 * 8) = vc;
     if (lane16 == 0) {
-      a.kp[rec + kScaleOff + r] = (uint8_t)kb;
-      a.vp[rec + kScaleOff + r] = (uint8_t)vb;
+      kp[rec + kScaleOff + r] = (uint8_t)kb;
+      vp[rec + kScaleOff + r] = (uint8_t)vb;
     }
   }
 }
 
 template <bool VEC, int U>
-__global__ __launch_bounds__(256) void kv_quant_load(QuantArgs a) {
-  const int L = (int)(blockIdx.x & 7) * a.chunk + (int)(blockIdx.x >> 3);
+__global__ __launch_bounds__(256) void kv_quant_load(QUANT_PARAMS) {
+  const int L = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
   const int lane16 = threadIdx.x & 15;
   const int row0 = L * 16 * U + (threadIdx.x >> 4);
   u32x2_t kc[U], vc[U];
@@ -97,20 +96,20 @@ __global__ __launch_bounds__(256) void kv_quant_load(QuantArgs a) {
   for (int u = 0; u < U; ++u) {
     const int row = row0 + 16 * u;
     ko[u] = nullptr;
-    if (row < a.rows) {
-      const int tok = (int)((uint32_t)row / (uint32_t)a.Hkv);
-      const int head = row - tok * a.Hkv;
-      const int64_t slot = a.slot[tok];
-      if (slot >= 0 && slot < a.n_slots) {
+    if (row < rows) {
+      const int tok = (int)((uint32_t)row / (uint32_t)Hkv);
+      const int head = row - tok * Hkv;
+      const int64_t slot = slots[tok];
+      if (slot >= 0 && slot < n_slots) {
         const int64_t e = (int64_t)head * kQuantD + lane16 * 8;
-        const int64_t rec = record_off((uint32_t)slot, a.Hkv, head);
+        const int64_t rec = record_off((uint32_t)slot, Hkv, head);
         const int r = (int)(slot & (kPageRows - 1));
-        ko[u] = a.k + (int64_t)tok * a.k_stride + e;
-        vo[u] = a.v + (int64_t)tok * a.v_stride + e;
-        kc[u] = *reinterpret_cast<const u32x2_t*>(a.kp + rec + r * kQuantD + lane16 * 8);
-        vc[u] = *reinterpret_cast<const u32x2_t*>(a.vp + rec + r * kQuantD + lane16 * 8);
-        kb[u] = a.kp[rec + kScaleOff + r];
-        vb[u] = a.vp[rec + kScaleOff + r];
+        ko[u] = k + (int64_t)tok * k_stride + e;
+        vo[u] = v + (int64_t)tok * v_stride + e;
+        kc[u] = *reinterpret_cast<const u32x2_t*>(kp + rec + r * kQuantD + lane16 * 8);
+        vc[u] = *reinterpret_cast<const u32x2_t*>(vp + rec + r * kQuantD + lane16 * 8);
+        kb[u] = kp[rec + kScaleOff + r];
+        vb[u] = vp[rec + kScaleOff + r];
       }
     }
   }
@@ -139,19 +138,15 @@ static int kv_quant(const char* name, uint16_t* k, int64_t ks, uint16_t* v, int6
   if ((int64_t)n_tok * Hkv > ((int64_t)1 << 30))
     return fail(DLLM_ERR_UNSUPPORTED, "%s: %d tokens of %d KV heads in one call", name, n_tok, Hkv);
   const bool vec = ks % 8 == 0 && vs % 8 == 0 && aligned16(k) && aligned16(v);
-  QuantArgs a = {};
-  a.k = k; a.v = v; a.kp = kp; a.vp = vp; a.slot = slot;
-  a.k_stride = ks; a.v_stride = vs;
-  a.n_slots = num_pages * kPageRows;
-  a.rows = n_tok * Hkv;
-  a.Hkv = Hkv;
+  const int rows = n_tok * Hkv;
   const int U = 1;
-  const int64_t blocks = ((int64_t)a.rows + 16 * U - 1) / (16 * U);
+  const int64_t blocks = ((int64_t)rows + 16 * U - 1) / (16 * U);
   // consecutive workgroups on one XCD: the scale bytes of a page's rows share lines
-  a.chunk = (int)((blocks + 7) / 8);
+  const int chunk = (int)((blocks + 7) / 8);
   auto kern = STORE ? (vec ? kv_quant_store<true, U> : kv_quant_store<false, U>)
                     : (vec ? kv_quant_load<true, U> : kv_quant_load<false, U>);
-  kern<<<dim3((unsigned)a.chunk * 8), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+  kern<<<dim3((unsigned)chunk * 8), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+      slot, k, v, rows, Hkv, chunk, ks, vs, kp, vp, num_pages * kPageRows);
   return check_launch(name);
 }
 
