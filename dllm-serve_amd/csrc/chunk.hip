@@ -1153,13 +1153,12 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   const int64_t all_t =
       std::min(n_seg * tiles, p.tile_form ? (total_cached + total_q + 2 * (key - 1) * n_seg) / key
                                           : (total_cached + (key - 1) * n_seg) / key);
-  // Keys are split where that shortens the longest workgroup: tile form, to half or less;
-  // rows form, to two thirds.  Every workgroup pays for its start and the joining (8 x 32
+  // Rows form: keys are split where that shortens the longest workgroup to two thirds.
+  // Every workgroup pays for its start and the joining (8 x 32
   // rows behind 608 - 1216, 32/32 heads, 256 workgroups: 20 us, split in two 30), and few
   // keys are not split: the joining takes 3 us, a turn of the rows form's wavefronts (four
   // tiles) 0.8: one token behind 511 rows 8.6 us whole, 8.8 in four, behind 1000 9.5 in eight.
-  // Tile form: the work dealt to two workgroups a CU, whose phases overlap.  Rows form,
-  // sequences of one length: as many parts as give every CU one workgroup (one token behind
+  // Sequences of one length: as many parts as give every CU one workgroup (one token behind
   // 131071, 28/4 heads: 256 workgroups 29.6 us, 384 34, 512 31).  Of different lengths:
   // 384 workgroups, half a part each lost to the last ones, of 12 tiles at least (32
   // single tokens, 28/4 heads: at most 256 workgroups 24.7 us, 384 21.4; 40 of them 51.6 and 39.5,
@@ -1168,14 +1167,22 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   const double work = (double)groups * (double)all_t / (double)n_seg;
   int64_t tps;
   if (p.tile_form) {
+    // The work dealt to two workgroups a CU, whose phases overlap, if that halves the longest
+    // and pays.  In us: a tile takes 1.7 in a workgroup that has its CU to itself, 2.4 in
+    // one of two, a part of 128 rows 0.027 for its way through memory, the joining 3.  (256
+    // workgroups of 20 tiles, 4 x 256 rows behind 1000, 32 heads: 44 us whole, 52 in two
+    // parts; 220 of 112, 1000 rows behind 6144, 28/4 heads: 176 whole, 148 in three.)
     tps = std::max<int64_t>((int64_t)(work / 512 + 0.999), 4);
+    const double parts = std::min((double)groups * (double)((tiles + tps - 1) / tps), work / (double)tps + 0.5 * (double)groups);
+    if (tps * 2 > tiles || tiles <= 8 || (groups <= 256 ? 1.7 : 2.4) * (double)tiles < 2.4 * (double)tps + 3 + 0.027 * parts)
+      tps = tiles;
   } else if (total_cached == n_seg * max_cached) {
     const int64_t parts = std::max<int64_t>(1, 256 / groups);
     tps = std::max<int64_t>((tiles + parts - 1) / parts, 4);
   } else {
     tps = groups < 768 ? std::max<int64_t>((int64_t)(work / (384 - 0.5 * (double)groups) + 0.999), 12) : tiles;
   }
-  if (p.tile_form ? tps * 2 > tiles || tiles <= 8 : tps * 3 > tiles * 2 || tiles <= 24) tps = tiles;
+  if (!p.tile_form && (tps * 3 > tiles * 2 || tiles <= 24)) tps = tiles;
   if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
   if (tps < 1) tps = 1;
   if (tps > 0x3fffffff) tps = 0x3fffffff;

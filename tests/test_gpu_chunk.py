@@ -111,6 +111,8 @@ SHAPES = [
     ([300], [0], 4, 1, 0),
     ([130], [64], 14, 1, 5),
     ([66], [4200], 16, 1, 1),
+    # parts of a row joined in several rounds
+    ([1], [33000], 2, 1, 1),
 ]
 
 
