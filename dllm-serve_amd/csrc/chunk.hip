@@ -332,8 +332,12 @@ __device__ __forceinline__ void v_rows(const uint8_t* vb_ptr, u32x2_t (&r)[16]) 
       : "memory");
 }
 
-template <int NB, bool FP8>
+// ONE: one M tile, so nothing else reads the keys and the loads are streaming ones (64
+// tokens behind 2000, 32 heads: 192 -> 171 us; with seven M tiles, 16 x 32 rows, 28/4
+// heads, they take 21.2, ordinary ones 19.8).
+template <int NB, bool FP8, bool ONE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(CHUNK_PARAMS) {
+  constexpr int AUX = ONE ? kStreamAux : 0;
   using T = RowsTile<FP8>;
   constexpr int BM = 16 * NB;
   constexpr int PARK = park_floats(NB);
@@ -412,8 +416,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
       for (int j = 0; j < T::kDma; ++j) {
         const uint32_t off = (uint32_t)(j * 1024) + row + (ch ^ (uint32_t)(j == 1 || j == 2 ? 64 : 0));
-        dma16<kStreamAux>(krs, stage + j * 1024, off);
-        dma16<kStreamAux>(vrs, stage + T::kV + j * 1024, off);
+        dma16<AUX>(krs, stage + j * 1024, off);
+        dma16<AUX>(vrs, stage + T::kV + j * 1024, off);
       }
       // lanes 0 .. 7: K's scale bytes, 8 .. 15: V's (the others repeat them)
       const uint8_t* sp = (lane & 8 ? a.vc : a.kc) + rec + kScaleOff + row0 + (lane & 7) * 4;
@@ -428,8 +432,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
       for (int j = 0; j < T::kDma; ++j) {  // lane l: row 4 j + l / 16, physical chunk l % 16
         const int row = 4 * j + g4;
-        dma16<kStreamAux>(krs, stage + j * 1024, (uint32_t)row * bf_row + (uint32_t)((col ^ (row & 15)) * 16));
-        dma16<kStreamAux>(vrs, stage + T::kV + j * 1024, (uint32_t)row * bf_row + (uint32_t)((col ^ (2 * (row & 7))) * 16));
+        dma16<AUX>(krs, stage + j * 1024, (uint32_t)row * bf_row + (uint32_t)((col ^ (row & 15)) * 16));
+        dma16<AUX>(vrs, stage + T::kV + j * 1024, (uint32_t)row * bf_row + (uint32_t)((col ^ (2 * (row & 7))) * 16));
       }
     }
   };
@@ -1317,12 +1321,15 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
   };
   if (p.tile_form)
     rc = launch(fp8 ? chunk_tile_kernel<true> : chunk_tile_kernel<false>, 2 * kTileStage);
-  else if (p.nb == 1)
-    rc = fp8 ? launch(chunk_rows_kernel<1, true>, rows_lds<1, true>())
-             : launch(chunk_rows_kernel<1, false>, rows_lds<1, false>());
+  else if (p.nb == 1)  // at most 16 rows
+    rc = fp8 ? launch(chunk_rows_kernel<1, true, true>, rows_lds<1, true>())
+             : launch(chunk_rows_kernel<1, false, true>, rows_lds<1, false>());
+  else if (p.mtiles == 1)
+    rc = fp8 ? launch(chunk_rows_kernel<2, true, true>, rows_lds<2, true>())
+             : launch(chunk_rows_kernel<2, false, true>, rows_lds<2, false>());
   else
-    rc = fp8 ? launch(chunk_rows_kernel<2, true>, rows_lds<2, true>())
-             : launch(chunk_rows_kernel<2, false>, rows_lds<2, false>());
+    rc = fp8 ? launch(chunk_rows_kernel<2, true, false>, rows_lds<2, true>())
+             : launch(chunk_rows_kernel<2, false, false>, rows_lds<2, false>());
   if (rc || p.max_split == 1) return rc;
   auto join = [&](auto one, auto eight) {
     const bool many = p.max_split > 8;
