@@ -422,9 +422,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       // lanes 0 .. 7: K's scale bytes, 8 .. 15: V's (the others repeat them)
       const uint8_t* sp = (lane & 8 ? a.vc : a.kc) + rec + kScaleOff + row0 + (lane & 7) * 4;
       // (in asm: after the builtin, which the compiler takes for an access that ends out of
-      // order, it waits for all that is in flight wherever it waits for anything)
+      // order, it waits for all that is in flight wherever it waits for anything.  A write of
+      // m0 is one wait state ahead of its use by such a load.)
       const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(stage + T::kScales);
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(sp) : "m0", "memory");
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(sp) : "m0", "memory");
     } else {
       const int64_t off0 = ((int64_t)max(pid, 0) * kPageRows + row0) * bf_row + hkv * HD * 2;
       const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * bf_row + HD * 2 : 0u;
@@ -1077,7 +1078,10 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
     float top = mx;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (p0 + i * G >= parts) pm[i] = -INFINITY;
+      if (p0 + i * G >= parts) {
+        pm[i] = -INFINITY;
+        pl[i] = 0.f;
+      }
       top = fmaxf(top, pm[i]);
     }
     const float mu = top == -INFINITY ? 0.f : top;
@@ -1086,13 +1090,14 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] *= w0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (pm[i] != -INFINITY) {
-        const float w = __builtin_amdgcn_exp2f(pm[i] - mu);
-        l += pl[i] * w;
+    for (int i = 0; i < 8; ++i) {
+      const float w = pm[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm[i] - mu);
+      l += pl[i] * w;  // a part of NaN scores alone has no maximum: its NaN stays in the sum
+      if (w != 0.f) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += x[i][e] * w;
       }
+    }
     mx = top;
     p0 += 8 * G;
     if (p0 >= parts) break;
@@ -1166,7 +1171,8 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   // 131071, 28/4 heads: 256 workgroups 29.6 us, 384 34, 512 31).  Of different lengths:
   // 384 workgroups, half a part each lost to the last ones, of 12 tiles at least (32
   // single tokens, 28/4 heads: at most 256 workgroups 24.7 us, 384 21.4; 40 of them 51.6 and 39.5,
-  // with 448 44.7; eight shorter ones 11.2, in parts of 8 tiles 12.9).
+  // with 448 44.7; eight shorter ones 11.2, in parts of 8 tiles 12.9), with many sequences 256, so that
+  // one long one among them is still split.
   const int64_t groups = all_m * Hkv;  // (M tile, KV head) pairs, each with its own parts
   const double work = (double)groups * (double)all_t / (double)n_seg;
   int64_t tps;
@@ -1184,7 +1190,7 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
     const int64_t parts = std::max<int64_t>(1, 256 / groups);
     tps = std::max<int64_t>((tiles + parts - 1) / parts, 4);
   } else {
-    tps = groups < 768 ? std::max<int64_t>((int64_t)(work / (384 - 0.5 * (double)groups) + 0.999), 12) : tiles;
+    tps = std::max<int64_t>((int64_t)(work / std::max(384 - 0.5 * (double)groups, 256.) + 0.999), 12);
   }
   if (!p.tile_form && (tps * 3 > tiles * 2 || tiles <= 24)) tps = tiles;
   if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);

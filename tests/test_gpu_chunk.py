@@ -391,3 +391,29 @@ def test_pieces_are_launched_longest_first(dev, bits, monkeypatch):
         assert torch.equal(chunk_attention(q, k, v, b.kc, b.vc, plan, SCALE), want)
     monkeypatch.setattr(_capi, "native", None)
     assert torch.equal(b.run(1), want)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("len_,cached,g", [(1, 1500, 4), (3, 33000, 2), (100, 1500, 2), (66, 4200, 16), (5, 20, 2)])
+def test_nan_rows_of_q(dev, bits, len_, cached, g):
+    """A NaN in q is a NaN in its row of o, however many parts the keys are in, and in no other."""
+    b = Batch(dev, [len_], [cached], g, 1, bits, seed=22)
+    want = b.run(1)
+    b.q[len_ - 1, g - 1, 5] = float("nan")
+    out = b.run(1).view(len_, g, 128)
+    assert out[len_ - 1, g - 1].isnan().all()
+    out[len_ - 1, g - 1] = want.view(len_, g, 128)[len_ - 1, g - 1]
+    assert torch.equal(out.view_as(want), want)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("len_,g", [(1, 4), (100, 2), (66, 16)])
+def test_nan_keys_of_one_part(dev, bits, len_, g):
+    """A whole page of NaN keys, all that some part sees: every row is NaN."""
+    b = Batch(dev, [len_], [4200], g, 1, bits, seed=23)
+    page = b.tables[0][5]
+    if bits == 8:
+        b.kc[page, :, :256 * 128] = 0x7F
+    else:
+        b.kc[page] = float("nan")
+    assert b.run(1).isnan().all()
