@@ -152,7 +152,8 @@ class ChunkPlan:
     needed are fine).  ``mask_block`` 0: the new rows see each other; b >= 1:
     a row sees the rows up to the end of its own block of b positions
     (1: causal), positions counted from the first cached row.  The tables are
-    uploaded with one asynchronous copy; nothing synchronises.
+    uploaded with one asynchronous copy; nothing synchronises.  A plan for a
+    captured graph is made before the capture.
 
     ``cached_lens`` and ``block_tables`` are in the order of the launch, which is
     the sequences' own unless they feed _SORT_ROWS rows together: then those with
@@ -176,6 +177,9 @@ class ChunkPlan:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            # a replay would copy from pinned memory that has long been given to something else
+            raise RuntimeError("make the ChunkPlan before the capture")
         self.n_seg = B = len(seqlens)
         self.total_rows, self.total_cached = sum(seqlens), sum(cached)
         self.max_q, self.max_cached = max(seqlens, default=0), max(cached, default=0)
@@ -250,8 +254,8 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
         for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
             if (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != dev or t.dim() != 4
                     or tuple(t.shape[1:]) != (_capi.PAGE_ROWS, Hkv, D)):
-                raise ValueError(f"{n} must be contiguous bf16 [num_pages, {_capi.PAGE_ROWS}, {Hkv}, {D}] or 8-bit pages "
-                                 f"on {dev}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+                raise ValueError(f"{n} must be contiguous bf16 [num_pages, {_capi.PAGE_ROWS}, {Hkv}, {D}] or 8-bit "
+                                 f"pages on {dev}; got {t.dtype} {tuple(t.shape)} on {t.device}")
         kind, pages = _capi.CACHE_BF16, min(k_cache.shape[0], v_cache.shape[0])
     if plan.max_page >= pages:
         raise ValueError(f"a block table names page {plan.max_page} of a cache of {pages}")
@@ -266,8 +270,9 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
             _capi.attn_chunk_paged_fwd_raw(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, plan._seg_ids, plan.n_seg,
                 plan.max_q, plan.max_cached, plan.total_rows, plan.total_cached, k_cache.data_ptr(),
-                v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens, plan.mask_block, Hq, Hkv, D, q_st, k_st, v_st, o.stride(0), float(softmax_scale),
-                None if ws is None else ws.data_ptr(), need, _capi._stream(dev))
+                v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens, plan.mask_block, Hq, Hkv, D, q_st, k_st,
+                v_st, o.stride(0), float(softmax_scale), None if ws is None else ws.data_ptr(), need,
+                _capi._stream(dev))
     return o
 
 
@@ -654,5 +659,6 @@ class Attention(nn.Module):
         ws = plan.workspace(("pages", Hq, Hkv, D), need)
         _capi.attn_chunk_paged_fwd_raw(qp, kp, vp, op, args["cu"], args["cached_ids"], *sizes, plan.rows_cached,
                                        plan.keeps_cached, kc, vc, _capi.CACHE_FP8, cache_slots // _capi.PAGE_ROWS,
-                                       table.data_ptr(), table.shape[1], lens.data_ptr(), 0, Hq, Hkv, D, q_st, k_st, v_st,
-                                       o_st, float(self.scale), None if ws is None else ws.data_ptr(), need, stream)
+                                       table.data_ptr(), table.shape[1], lens.data_ptr(), 0, Hq, Hkv, D, q_st, k_st,
+                                       v_st, o_st, float(self.scale), None if ws is None else ws.data_ptr(), need,
+                                       stream)

@@ -417,3 +417,15 @@ def test_nan_keys_of_one_part(dev, bits, len_, g):
     else:
         b.kc[page] = float("nan")
     assert b.run(1).isnan().all()
+
+
+def test_plans_are_made_before_a_capture(dev):
+    x = torch.zeros(4, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="before the capture"):
+            ChunkPlan([1], [0], [[]], dev)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (x == 1).all()
