@@ -429,3 +429,31 @@ def test_plans_are_made_before_a_capture(dev):
     graph.replay()
     torch.cuda.synchronize()
     assert (x == 1).all()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_pages_beyond_4_gib(dev, bits):
+    """The last pages of a cache whose byte offsets do not fit 32 bits: the same bits as from a small one."""
+    lens, cached = [1, 40], [300, 700]
+    small = [Batch(dev, lens, cached, g, 1, bits, seed=24) for g in _forms(40)]
+    b = small[0]
+    pages = 4 * 2**30 // (_capi.PAGE_BYTES if bits == 8 else 256 * 256) + 64
+    far = pages - b.pages
+    if bits == 8:
+        kc, vc = (torch.empty(pages, 1, _capi.PAGE_BYTES, dtype=torch.uint8, device=dev) for _ in range(2))
+    else:
+        kc, vc = (torch.empty(pages, 256, 1, 128, dtype=BF16, device=dev) for _ in range(2))
+    for s in small:
+        kc[far:], vc[far:] = s.kc, s.vc
+        plan = ChunkPlan(lens, cached, [[p + far for p in t] for t in s.tables], dev, mask_block=1)
+        out = chunk_attention(s.q.to(dev), s.k.to(dev), s.v.to(dev), kc, vc, plan, SCALE)
+        assert torch.equal(out, s.run(1))
+    k, v = b.k.to(dev), b.v.to(dev)
+    slots = torch.arange(41, dtype=torch.int32, device=dev) * 100 + far * 256
+    store_kvcache(k, v, kc, vc, slots)
+    store_kvcache(k, v, b.kc, b.vc, slots - far * 256)
+    # slots past the end are left out of both
+    back, want = ([torch.zeros_like(k) for _ in range(2)] for _ in range(2))
+    load_kvcache(*back, kc, vc, slots)
+    load_kvcache(*want, b.kc, b.vc, slots - far * 256)
+    assert all(torch.equal(x, y) for x, y in zip(back, want)) and back[0].any()
