@@ -11,7 +11,7 @@
 // head hkv * g + m % g; every K / V byte that is read serves all of them.
 //
 //   * chunk_rows_kernel (few M rows: single tokens, blocks): each of a workgroup's
-//     four wavefronts takes 32-key tiles of its own, by DMA into its own LDS.  No
+//     four or eight wavefronts takes 32-key tiles of its own, by DMA into its own LDS.  No
 //     wavefront waits for another until the states are merged at the end.
 //   * chunk_tile_kernel (many M rows: pieces of prompts): 64-key tiles of K and V in LDS,
 //     in bf16, shared by the workgroup's wavefronts of 32 M rows each; 8-bit rows are
@@ -207,9 +207,9 @@ struct RowsTile {
 // Floats of a wavefront's parked O (rows of 128 + 4, which spreads them over the
 // banks), and bytes of a workgroup's LDS: the stages, later the parked O, m and l.
 constexpr int park_floats(int nb) { return 16 * nb * 132; }
-template <int NB, bool FP8>
+template <int NB, bool FP8, int NW>
 constexpr int rows_lds() {
-  constexpr int stages = 4 * 2 * RowsTile<FP8>::kStage, park = (4 * park_floats(NB) + 8 * 16 * NB) * 4;
+  constexpr int stages = NW * 2 * RowsTile<FP8>::kStage, park = NW * (park_floats(NB) + 2 * 16 * NB) * 4;
   return stages > park ? stages : park;
 }
 
@@ -332,11 +332,11 @@ __device__ __forceinline__ void v_rows(const uint8_t* vb_ptr, u32x2_t (&r)[16]) 
       : "memory");
 }
 
-// ONE: one M tile, so nothing else reads the keys and the loads are streaming ones (64
+// NW: wavefronts.  ONE: one M tile, so nothing else reads the keys and the loads are streaming ones (64
 // tokens behind 2000, 32 heads: 192 -> 171 us; with seven M tiles, 16 x 32 rows, 28/4
 // heads, they take 21.2, ordinary ones 19.8).
-template <int NB, bool FP8, bool ONE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(CHUNK_PARAMS) {
+template <int NB, bool FP8, bool ONE, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_rows_kernel(CHUNK_PARAMS) {
   constexpr int AUX = ONE ? kStreamAux : 0;
   using T = RowsTile<FP8>;
   constexpr int BM = 16 * NB;
@@ -425,7 +425,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       // order, it waits for all that is in flight wherever it waits for anything.  A write of
       // m0 is one wait state ahead of its use by such a load.)
       const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(stage + T::kScales);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(sp) : "m0", "memory");
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                   :
+                   : "s"(to), "v"(sp)
+                   : "m0", "memory");
     } else {
       const int64_t off0 = ((int64_t)max(pid, 0) * kPageRows + row0) * bf_row + hkv * HD * 2;
       const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * bf_row + HD * 2 : 0u;
@@ -549,7 +552,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   // ---- new rows (the last split's), bf16 from k / v ------------------------------
   // Before the cached tiles: their loads are among the first, beside the first tile's DMA.
-  const int n = max(0, (t_end - t_begin - wave + 3) >> 2);  // this wavefront's cached tiles
+  const int n = max(0, (t_end - t_begin - wave + NW - 1) / NW);  // this wavefront's cached tiles
   const int first = t_begin + wave;
   bool fixed = false;
   const uint32_t vS = (uint32_t)(a.v_stride * 2), vb = (uint32_t)(sg.len - 1) * vS + HD * 2;
@@ -563,7 +566,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int last = min(m_base + BM, M) - 1;
     const int see = visible(sg, token_of(last, g), a.mask_block);
     const int new_tiles = (see + kTileKeys - 1) / kTileKeys;
-    for (int t = (wave - turn) & 3; t < new_tiles; t += 4) {
+    for (int t = (wave - turn) & (NW - 1); t < new_tiles; t += NW) {
       bf16x8_t kx[2][4];
       u32x4_t vx[2][4];
 #pragma unroll
@@ -623,10 +626,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   }
 
-  // ---- cached tiles: this wavefront takes every fourth, two in flight --------------
+  // ---- cached tiles: this wavefront takes every NW-th, two in flight ----------------
   if (n > 0) {
     wave_lds_fence();  // the new rows' V has been read
-    issue(my + T::kStage, first + 4, n > 1);  // no second tile: as many operations, all zeros
+    issue(my + T::kStage, first + NW, n > 1);  // no second tile: as many operations, all zeros
     // Q has landed, both tiles may be in flight.  (Where the compiler has to join paths with
     // different operations, it waits for the tiles as well.)
     vm_wait<2 * T::kOps>();
@@ -640,16 +643,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       else
         vm_wait<0>();
       uint8_t* const stage = my + (i & 1) * T::kStage;
-      compute_tile(stage, first + 4 * i);
+      compute_tile(stage, first + NW * i);
       wave_lds_fence();  // the tile's reads end before its stage is filled again
-      if (i + 2 < n) issue(stage, first + 4 * i + 8);
+      if (i + 2 < n) issue(stage, first + NW * (i + 2));
     }
   }
 
   if (fixed) {
 #pragma unroll 1
     for (int j = 0; j < sg.len; ++j) {
-      if ((((j / kTileKeys) + turn - wave) & 3) != 0) continue;  // a key of another wavefront
+      if ((((j / kTileKeys) + turn - wave) & (NW - 1)) != 0) continue;  // a key of another wavefront
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) {
         const u32x2_t w = __builtin_bit_cast(
@@ -667,8 +670,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   }
 
-  // ---- merge of the four wavefronts ------------------------------------------------
-  float* const ml = lds + 4 * PARK;
+  // ---- merge of the wavefronts -----------------------------------------------------
+  float* const ml = lds + NW * PARK;
   __syncthreads();  // the stages are free
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -682,18 +685,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       *reinterpret_cast<f32x4_t*>(lds + wave * PARK + (16 * b + col) * 132 + 16 * dt + 4 * g4) = st.o[b][dt];
   }
   __syncthreads();
-  constexpr int TPR = 256 / BM;   // threads of a row
-  constexpr int DPT = HD / TPR;   // d positions of a thread
+  constexpr int TPR = 64 * NW / BM;  // threads of a row
+  constexpr int DPT = HD / TPR;      // d positions of a thread
   const int row = tid / TPR, d0 = (tid % TPR) * 4;  // d0 + 4 TPR j
   const int m = m_base + row;
   if (m >= M) return;
   float mx = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[(w * 2) * BM + row]);
+  for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ml[(w * 2) * BM + row]);
   const float mu = mx == -INFINITY ? 0.f : mx;
-  float f[4], lsum = 0.f;
+  float f[NW], lsum = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     const float mw = ml[(w * 2) * BM + row];
     f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mu);
     lsum += ml[(w * 2 + 1) * BM + row] * f[w];
@@ -705,7 +708,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int d = d0 + 4 * TPR * j;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       if (f[w] == 0.f) continue;  // a wavefront without keys
       const f32x4_t x = *reinterpret_cast<const f32x4_t*>(lds + w * PARK + row * 132 + d);
 #pragma unroll
@@ -864,7 +867,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int kk = 0; kk < 8; ++kk) qf[kk] = as_bf16x8(bload(qrs, ok ? qoff + (uint32_t)kk * 32u : qbytes, 0u));
   }
   // of this wavefront's rows: the least and the most that any sees
-  const int lim_lo = __builtin_amdgcn_readfirstlane(visible(sg, min(token_of(m_base + wave * 32, g), sg.len - 1), a.mask_block));
+  const int lim_lo = __builtin_amdgcn_readfirstlane(
+      visible(sg, min(token_of(m_base + wave * 32, g), sg.len - 1), a.mask_block));
   const int lim_hi =
       __builtin_amdgcn_readfirstlane(visible(sg, token_of(min(m_base + wave * 32 + 32, M) - 1, g), a.mask_block));
   const bool live = m_base + wave * 32 < M;
@@ -1183,9 +1187,10 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
     // workgroups of 20 tiles, 4 x 256 rows behind 1000, 32 heads: 44 us whole, 52 in two
     // parts; 220 of 112, 1000 rows behind 6144, 28/4 heads: 176 whole, 148 in three.)
     tps = std::max<int64_t>((int64_t)(work / 512 + 0.999), 4);
-    const double parts = std::min((double)groups * (double)((tiles + tps - 1) / tps), work / (double)tps + 0.5 * (double)groups);
-    if (tps * 2 > tiles || tiles <= 8 || (groups <= 256 ? 1.7 : 2.4) * (double)tiles < 2.4 * (double)tps + 3 + 0.027 * parts)
-      tps = tiles;
+    const double parts = std::min((double)groups * (double)((tiles + tps - 1) / tps),
+                                  work / (double)tps + 0.5 * (double)groups);
+    const double whole = (groups <= 256 ? 1.7 : 2.4) * (double)tiles;
+    if (tps * 2 > tiles || tiles <= 8 || whole < 2.4 * (double)tps + 3 + 0.027 * parts) tps = tiles;
   } else if (total_cached == n_seg * max_cached) {
     const int64_t parts = std::max<int64_t>(1, 256 / groups);
     tps = std::max<int64_t>((tiles + parts - 1) / parts, 4);
@@ -1255,7 +1260,8 @@ extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached
 
 extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,
                                          const int32_t* cu, const int32_t* seg_ids, int n_seg, int max_q, int max_cached,
-                                         int64_t total_q, int64_t total_cached, const void* k_cache, const void* v_cache, int cache_type, int num_pages,
+                                         int64_t total_q, int64_t total_cached, const void* k_cache,
+                                         const void* v_cache, int cache_type, int num_pages,
                                          const int32_t* page_table, int max_pages, const int32_t* cached_len,
                                          int mask_block, int Hq, int Hkv, int D, int64_t q_stride, int64_t k_stride,
                                          int64_t v_stride, int64_t o_stride, float softmax_scale, void* workspace,
@@ -1288,7 +1294,8 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
     if (!aligned16(k_cache) || !aligned16(v_cache))
       return fail(DLLM_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", name);
   }
-  if ((int64_t)n_seg * max_pages >= ((int64_t)1 << 31) || max_pages >= (1 << 26)) return fail(DLLM_ERR_INVALID_ARG, "%s: page table too large", name);
+  if ((int64_t)n_seg * max_pages >= ((int64_t)1 << 31) || max_pages >= (1 << 26))
+    return fail(DLLM_ERR_INVALID_ARG, "%s: page table too large", name);
   ChunkArgs a = {};
   a.q = q; a.k = k; a.v = v; a.o = o;
   a.kc = reinterpret_cast<const uint8_t*>(k_cache);
@@ -1314,33 +1321,43 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
   int chunk;
   const int grid = chunk_grid(p, &chunk);
   const int chunk_pages = chunk + 32 * (max_cached > 0 && num_pages > 0 ? max_pages : 0);
-  auto start = [&](auto kern, dim3 blocks, int lds_bytes) {
-    kern<<<blocks, dim3(256), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
+  auto start = [&](auto kern, dim3 blocks, int threads, int lds_bytes) {
+    kern<<<blocks, dim3((unsigned)threads), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
         cu, seg_ids, cached_len, page_table, chunk_pages, (int)p.logical, p.mtiles, p.max_split, p.tiles_per_split, Hkv, a);
     return check_launch(name);
   };
   const bool fp8 = cache_type == DLLM_CACHE_FP8;
-  auto launch = [&](auto kern, int lds_bytes) -> int {
+  auto launch = [&](auto kern, int lds_bytes, int threads = 256) -> int {
     int e = set_lds(kern, lds_bytes, name);
     if (e) return e;
-    return start(kern, dim3((unsigned)grid), lds_bytes);
+    return start(kern, dim3((unsigned)grid), threads, lds_bytes);
   };
+  // Few workgroups of some length: eight wavefronts each, which halves the turns (and takes a
+  // CU's LDS, so 8-bit rows only).  One token behind 511 rows, 32 heads, 8.5 -> 7.4 us, behind
+  // 767 10.1 -> 8.5, 128 rows behind 4000 29.9 -> 26.9; not where a workgroup a CU streams from
+  // memory (4 tokens behind 2000 18.6, 18.8), nor for 32 rows of few keys, whose merge is
+  // longer (32 behind 300 10.0, 10.4).
+  const bool eight = fp8 && p.logical <= (p.mtiles > 1 ? 256 : 192) && p.tiles_per_split > (p.nb == 1 ? 4 : 12);
   if (p.tile_form)
     rc = launch(fp8 ? chunk_tile_kernel<true> : chunk_tile_kernel<false>, 2 * kTileStage);
+  else if (eight)
+    rc = p.nb == 1 ? launch(chunk_rows_kernel<1, true, true, 8>, rows_lds<1, true, 8>(), 512)
+         : p.mtiles == 1 ? launch(chunk_rows_kernel<2, true, true, 8>, rows_lds<2, true, 8>(), 512)
+                         : launch(chunk_rows_kernel<2, true, false, 8>, rows_lds<2, true, 8>(), 512);
   else if (p.nb == 1)  // at most 16 rows
-    rc = fp8 ? launch(chunk_rows_kernel<1, true, true>, rows_lds<1, true>())
-             : launch(chunk_rows_kernel<1, false, true>, rows_lds<1, false>());
+    rc = fp8 ? launch(chunk_rows_kernel<1, true, true, 4>, rows_lds<1, true, 4>())
+             : launch(chunk_rows_kernel<1, false, true, 4>, rows_lds<1, false, 4>());
   else if (p.mtiles == 1)
-    rc = fp8 ? launch(chunk_rows_kernel<2, true, true>, rows_lds<2, true>())
-             : launch(chunk_rows_kernel<2, false, true>, rows_lds<2, false>());
+    rc = fp8 ? launch(chunk_rows_kernel<2, true, true, 4>, rows_lds<2, true, 4>())
+             : launch(chunk_rows_kernel<2, false, true, 4>, rows_lds<2, false, 4>());
   else
-    rc = fp8 ? launch(chunk_rows_kernel<2, true, false>, rows_lds<2, true>())
-             : launch(chunk_rows_kernel<2, false, false>, rows_lds<2, false>());
+    rc = fp8 ? launch(chunk_rows_kernel<2, true, false, 4>, rows_lds<2, true, 4>())
+             : launch(chunk_rows_kernel<2, false, false, 4>, rows_lds<2, false, 4>());
   if (rc || p.max_split == 1) return rc;
   auto join = [&](auto one, auto eight) {
     const bool many = p.max_split > 8;
     const int64_t rows = (int64_t)max_q * a.g;
-    return start(many ? eight : one, dim3((unsigned)(many ? rows : (rows + 7) / 8), (unsigned)Hkv, (unsigned)n_seg), 0);
+    return start(many ? eight : one, dim3((unsigned)(many ? rows : (rows + 7) / 8), (unsigned)Hkv, (unsigned)n_seg), 256, 0);
   };
   if (p.tile_form) return join(chunk_combine_kernel<kTileRows, true, 1>, chunk_combine_kernel<kTileRows, true, 8>);
   return p.nb == 1 ? join(chunk_combine_kernel<16, false, 1>, chunk_combine_kernel<16, false, 8>)

@@ -113,6 +113,9 @@ SHAPES = [
     ([66], [4200], 16, 1, 1),
     # parts of a row joined in several rounds
     ([1], [33000], 2, 1, 1),
+    # one block of 17 to 32 rows, whole and in parts
+    ([17], [500], 2, 2, 1),
+    ([8, 6], [2000, 1500], 4, 1, 4),
 ]
 
 
@@ -159,9 +162,10 @@ def test_large_scores(dev, bits, g):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("cached", [70, 600])
 @pytest.mark.parametrize("L,g", [(5, 1), (40, 1), (140, 1), (70, 15), (130, 9)])
-def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L, g):
-    b = Batch(dev, [L], [70], 2 * g, 2, bits, seed=6)
+def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L, g, cached):
+    b = Batch(dev, [L], [cached], 2 * g, 2, bits, seed=6)
     b.v[L - 1, 0, 3] = float("nan")
     b.v[L - 2, 1, 9] = float("inf")
     b.k[L - 1, 1, 0] = float("nan")
@@ -171,7 +175,7 @@ def test_nan_and_infinity_reach_only_the_rows_that_see_them(dev, bits, L, g):
     assert torch.isfinite(out[ref_rows]).all()
     x = [_np(t) for t in (b.q, b.k, b.v)]
     ref, spread, reach = chunk.attend(*x, b.cache_rows(b.kc, 0), b.cache_rows(b.vc, 0), SCALE, 1)
-    check(out[ref_rows], ref[ref_rows], spread[ref_rows], reach[ref_rows], L + 70)
+    check(out[ref_rows], ref[ref_rows], spread[ref_rows], reach[ref_rows], L + cached)
     o = _np(out).reshape(ref.shape)
     assert np.isnan(o[L - 1]).all(axis=-1)[g:].all()   # a NaN score
     assert (o[L - 2, g:, 9] == np.inf).all() and np.isnan(o[L - 1, g:, 9]).all()
