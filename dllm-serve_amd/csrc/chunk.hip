@@ -1167,10 +1167,10 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
       std::min(n_seg * tiles, p.tile_form ? (total_cached + total_q + 2 * (key - 1) * n_seg) / key
                                           : (total_cached + (key - 1) * n_seg) / key);
   // Rows form: keys are split where that shortens the longest workgroup to two thirds.
-  // Every workgroup pays for its start and the joining (8 x 32
-  // rows behind 608 - 1216, 32/32 heads, 256 workgroups: 20 us, split in two 30), and few
-  // keys are not split: the joining takes 3 us, a turn of the rows form's wavefronts (four
-  // tiles) 0.8: one token behind 511 rows 8.6 us whole, 8.8 in four, behind 1000 9.5 in eight.
+  // Every workgroup pays for its start and the joining (8 x 32 rows behind 608 - 1216,
+  // 32/32 heads, 256 workgroups: 20 us, split in two 30), and few keys are not split: the
+  // joining takes 3 us, a turn of the wavefronts 0.8 (one token, 32 heads, whole / in parts:
+  // behind 511 7.4 / 8.8, behind 767 8.4 / 9.3, behind 900 10.0 / 8.3).
   // Sequences of one length: as many parts as give every CU one workgroup (one token behind
   // 131071, 28/4 heads: 256 workgroups 29.6 us, 384 34, 512 31).  Of different lengths:
   // 384 workgroups, half a part each lost to the last ones, of 12 tiles at least (32
