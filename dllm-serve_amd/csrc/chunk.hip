@@ -187,7 +187,13 @@ __device__ __forceinline__ float row_sum4(float x) {
 // the conversion; V^T, whose operand holds eight keys of one d
 // (ds_read_b64_tr_b8: in a group of 16 lanes lane 2k + h supplies bytes 8 h .. 8 h + 7
 // of row k of an 8 x 16 block and lane n receives column n), without: the powers of two
-// are multiplied onto P instead, which commutes with its rounding.
+// are multiplied onto P instead, which commutes with its rounding (a V row of 2^127 may
+// overflow there where only its larger elements would in f32).
+//
+// Bound by memory where workgroups fill the card (one token behind 131071, 28/4 heads: 23.8
+// us, 5.7 TB/s; 16 ragged tokens over bf16 pages, 32 heads: 133 us, 6.0 TB/s), by what a
+// CU takes in where there is one a CU (8 x 32 rows behind 608 - 1216, 32 heads, 18 us), by
+// the chain start - lengths - first tile - turns - merge where there are few keys.
 //
 // Chunks of 16 bytes are XOR-swizzled inside a row, so that the lanes of a read phase
 // fall on different banks:
@@ -740,6 +746,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // pieces, 28/4 heads, 147 against 139, 5 ragged ones, 32 heads, 212 against 199).
 // The bf16 form also runs into what a CU takes in, 32 KB a tile and workgroup; V reads
 // in one block that leaves the next tile's loads in flight were no faster.
+//
+// Bound by the matrix pipe and what its two wavefronts a SIMD do not overlap, and by
+// power: 2048 rows behind 6144, 32 heads, 8-bit, 275 us back to back with changing inputs, 875
+// TFLOP/s, the pipe busy 43 % of the time (bf16 50 %); 2 x 4096 bidirectional rows in bf16 1006.
 constexpr int kTileRows = 128;
 constexpr int kTileStage = 2 * kBigTile * 256;
 template <bool FP8>
@@ -1041,8 +1051,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // Joins the parts of every (segment, KV head, M row) whose keys were split.  G groups of
 // 32 threads (four d each) share a row's parts, each taking every G-th, so that a row
-// of many parts is one round of loads rather than a long chain (28 rows of 128 parts:
-// 39 us with one group, 9 with eight).
+// of many parts is one round of loads rather than a long chain (28 rows of 128 parts: 39 us
+// with one group, 3.8 with eight).  Bound by its launch and that round: 3 - 4 us (32 x
+// 28 rows of up to 8 parts 3.9).
 template <int BM, bool TILE, int G>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(CHUNK_PARAMS) {
   static_assert(G == 1 || G == 8, "a workgroup holds eight rows or one");
