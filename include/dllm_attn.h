@@ -247,9 +247,9 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * n = cached_len[s].  A row whose page is outside the cache (or whose page index is >=
  * max_pages) is left out of the softmax.
  * max_q and max_cached must bound L and n of every segment: longer segments are
- * cut there.  total_q and total_cached must bound their sums (0: not known), which
- * lets the work be dealt evenly when the segments differ; beyond them rows are left
- * unwritten.  D must be 128, Hq a multiple of Hkv, softmax_scale positive; pointers are
+ * cut there.  total_q and total_cached are their sums (0: not known); they only decide
+ * how the keys are dealt to workgroups, and so must be the same for the workspace's
+ * size.  D must be 128, Hq a multiple of Hkv, softmax_scale positive; pointers are
  * 16-byte aligned, token strides multiples of 8 elements, and a segment's new rows span
  * at most 4 GiB of q, k or v.  workspace: dllm_attn_chunk_workspace_size(...) bytes
  * (0 where one workgroup takes all keys of a row), any contents; calls that may
