@@ -172,13 +172,24 @@ PyObject* quant_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // chunk(q, k, v, k_cache, v_cache, plan: bytes, scale) -> output or None.
+// `plan` is this description and then the streams that are behind the tables' upload:
+// on any other the Python form runs, which makes it wait.
 struct ChunkTables {
   int64_t device, rows, n_seg, max_q, max_cached, total_cached, max_pages, max_page, mask_block, cu, lens, tables, seg_ids;
 };
+bool behind_upload(PyObject* plan, void* stream) {
+  const char* at = PyBytes_AS_STRING(plan) + sizeof(ChunkTables);
+  const char* const end = PyBytes_AS_STRING(plan) + PyBytes_GET_SIZE(plan);
+  for (int64_t s; at < end; at += sizeof(s)) {
+    std::memcpy(&s, at, sizeof(s));
+    if (s == (int64_t)reinterpret_cast<intptr_t>(stream)) return true;
+  }
+  return false;
+}
 
 PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7 || !PyBytes_CheckExact(a[5]) || PyBytes_GET_SIZE(a[5]) != (Py_ssize_t)sizeof(ChunkTables) ||
-      !PyFloat_CheckExact(a[6]))
+  if (n != 7 || !PyBytes_CheckExact(a[5]) || PyBytes_GET_SIZE(a[5]) < (Py_ssize_t)sizeof(ChunkTables) ||
+      PyBytes_GET_SIZE(a[5]) % (Py_ssize_t)sizeof(int64_t) || !PyFloat_CheckExact(a[6]))
     Py_RETURN_NONE;
   return guarded([&]() -> PyObject* {
     ChunkTables p;
@@ -193,6 +204,8 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int64_t Hq = heads[0], Hkv = heads[1];
     if (heads[2] != Hkv || Hq % Hkv || p.rows == 0 || c10::hip::current_device() != p.device) Py_RETURN_NONE;
+    void* const st = stream_of((int)p.device);
+    if (!behind_upload(a[5], st)) Py_RETURN_NONE;
     const at::Tensor *kc = pages_of(a[3], Hkv, (int)p.device), *vc = pages_of(a[4], Hkv, (int)p.device);
     const int kind = kc ? DLLM_CACHE_FP8 : DLLM_CACHE_BF16;
     if (!kc) {
@@ -212,7 +225,6 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor ws;
     if (nb) ws = at::empty({(int64_t)nb}, t[0]->options().dtype(at::kByte));
     const float scale = (float)PyFloat_AS_DOUBLE(a[6]);
-    void* st = stream_of((int)p.device);
     auto dev_i32 = [](int64_t x) { return reinterpret_cast<const int32_t*>(x); };
     const int rc = no_gil([&] {
       return dllm_attn_chunk_paged_fwd(ptr<dllm_bf16>(*t[0]), ptr<dllm_bf16>(*t[1]), ptr<dllm_bf16>(*t[2]),

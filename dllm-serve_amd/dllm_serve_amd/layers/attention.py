@@ -152,8 +152,12 @@ class ChunkPlan:
     needed are fine).  ``mask_block`` 0: the new rows see each other; b >= 1:
     a row sees the rows up to the end of its own block of b positions
     (1: causal), positions counted from the first cached row.  The tables are
-    uploaded with one asynchronous copy; nothing synchronises.  A plan for a
-    captured graph is made before the capture.
+    uploaded with one asynchronous copy on the stream that is current; nothing
+    synchronises the host.  The first call on any other stream makes that stream
+    wait for the upload, and a plan may be dropped while calls are in flight.  A plan
+    for a captured graph is made before the capture, has to have arrived by then
+    (torch.cuda.graph synchronises) and to live as long as the graph, which holds its
+    addresses.
 
     ``cached_lens`` and ``block_tables`` are in the order of the launch, which is
     the sequences' own unless they feed _SORT_ROWS rows together: then those with
@@ -201,15 +205,38 @@ class ChunkPlan:
         host = torch.from_numpy(flat.astype(np.int32))
         if self.device.type == "cuda":
             host = host.pin_memory()
-        dev = host.to(self.device, non_blocking=True)
+        self._tables = dev = host.to(self.device, non_blocking=True)
+        self._ready, self._streams = None, ()  # the upload's event, the streams that are behind it
+        if self.device.type == "cuda":
+            stream = torch.cuda.current_stream(self.device)
+            self._ready = torch.cuda.Event()
+            self._ready.record(stream)
+            self._streams = (stream.cuda_stream,)
         self.cu, self.cached_lens, self.block_tables = dev[:B + 1], dev[B + 1:2 * B + 1], dev[3 * B + 1:]
         self._seg_ids = None if order == sorted(order) else dev[2 * B + 1:].data_ptr()
         self._args = (self.cu.data_ptr(), self.cached_lens.data_ptr(), self.block_tables.data_ptr())
-        # the same for the native form (csrc/native.cpp, ChunkTables)
-        self._packed = struct.pack(
-            "=13q", -1 if self.device.index is None else self.device.index, self.total_rows, B, self.max_q,
-            self.max_cached, self.total_cached, W, self.max_page, self.mask_block, *self._args,
-            self._seg_ids or 0)
+        self._packed = self._pack()
+
+    _STREAMS = 16  # streams remembered; one that was forgotten waits once more
+
+    def _pack(self) -> bytes:
+        """The plan for the native form (csrc/native.cpp, ChunkTables), the streams behind it."""
+        return struct.pack(
+            f"={13 + len(self._streams)}q", -1 if self.device.index is None else self.device.index, self.total_rows,
+            self.n_seg, self.max_q, self.max_cached, self.total_cached, self.max_pages, self.max_page,
+            self.mask_block, *self._args, self._seg_ids or 0, *self._streams)
+
+    def _join(self) -> None:
+        """Puts the device's current stream behind the upload, and the tables' memory
+        behind what that stream will have read of it when the plan is dropped.  (A stream
+        that is being captured cannot wait for an event from outside its graph.)"""
+        stream = torch.cuda.current_stream(self.device)
+        if stream.cuda_stream in self._streams or torch.cuda.is_current_stream_capturing():
+            return
+        stream.wait_event(self._ready)
+        self._tables.record_stream(stream)
+        self._streams = (self._streams + (stream.cuda_stream,))[-self._STREAMS:]
+        self._packed = self._pack()
 
 
 def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -260,6 +287,7 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
     if plan.max_page >= pages:
         raise ValueError(f"a block table names page {plan.max_page} of a cache of {pages}")
     with _on_device(dev):
+        plan._join()
         o = torch.empty(nq, Hq * D, dtype=torch.bfloat16, device=dev)
         need = _capi.chunk_workspace_size(plan.n_seg, plan.max_q, plan.max_cached, Hq, Hkv, D, plan.total_rows,
                                           plan.total_cached)
