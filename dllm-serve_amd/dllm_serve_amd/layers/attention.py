@@ -181,9 +181,7 @@ class ChunkPlan:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            # a replay would copy from pinned memory that has long been given to something else
-            raise RuntimeError("make the ChunkPlan before the capture")
+        _not_captured("make the ChunkPlan", self.device)
         self.n_seg = B = len(seqlens)
         self.total_rows, self.total_cached = sum(seqlens), sum(cached)
         self.max_q, self.max_cached = max(seqlens, default=0), max(cached, default=0)
@@ -386,11 +384,21 @@ class StepLayout:
                 tuple(self.cfgs[i] for i in self.jobs_idx))
 
 
+def _not_captured(what: str, device: torch.device) -> None:
+    """Refuses an upload of tables inside a capture: the graph's replays would copy from
+    pinned memory that has long been given to something else."""
+    if device.type == "cuda":
+        with _on_device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what} before the capture")
+
+
 class StepPlan:
     """Launch tables of one diffusion forward (shared by all layers).
 
     ``StepPlan(context, device, ...)`` builds them from host integers of
-    ``context.seqs`` and uploads them with one asynchronous copy;
+    ``context.seqs`` and uploads them with one asynchronous copy (not inside
+    a capture: a forward of the same Context has to come before it);
     ``StepPlan.from_device`` wraps tables the device-side builder wrote."""
 
     _SCALARS = ("n_seq", "total_rows", "any_skipped", "n_dense", "max_q_dense", "n_job", "max_kc", "max_keep",
@@ -399,6 +407,7 @@ class StepPlan:
 
     def __init__(self, context, device: torch.device, num_kv_heads: int = 0, head_dim: int = 0, num_heads: int = 0,
                  layout: StepLayout | None = None):
+        _not_captured("run the step's forward once, which builds its plan,", device)
         seqs = context.seqs
         lay = layout if layout is not None else StepLayout(seqs)
         self._take(lay, device)
@@ -503,6 +512,8 @@ class StepPlan:
             if t is None:
                 raise ValueError("8-bit pages need the sequences' block tables (seq.block_table)")
             if not isinstance(t, torch.Tensor):
+                _not_captured("run the step's forward over 8-bit pages once, which uploads its page table,",
+                              self.device)
                 width = max(1, -(-self.max_keep_cached // _capi.PAGE_ROWS))
                 host = torch.full((self.n_cached, width), -1, dtype=torch.int32)
                 for r, pages in enumerate(t):

@@ -1,0 +1,87 @@
+"""A step whose tables the host builds has run before it is captured: inside a capture
+the upload would be replayed from pinned memory that has been given to something else."""
+import pytest
+import torch
+
+from dllm_serve_amd.engine.kv_cache import quantized_pages
+from dllm_serve_amd.engine.sequence import PageAllocator, Sequence, prepare_step
+from dllm_serve_amd.layers.attention import Attention
+from dllm_serve_amd.sparse.state import SparseConfig
+from dllm_serve_amd.utils.context import reset_context
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _step_of_reuse(dev):
+    cfg = SparseConfig(enabled=True, default_block_len=32, retention_ratio=0.9, pool_kernel=3, delay_step=1,
+                       head_select=True)
+    seqs = [Sequence([1] * n, 64, 126336, cfg, device=dev) for n in (200, 400)]
+    alloc = PageAllocator([5, 2, 7, 0, 3])
+    for s in seqs:
+        alloc.allocate(s)
+        s.advance()
+        s.advance()
+    g = torch.Generator().manual_seed(51)
+    x = [torch.randn(64, h * 128, generator=g).to(BF16).to(dev) for h in (8, 2, 2)]
+    return seqs, x
+
+
+def _layer(dev, quantised):
+    attn = Attention(8, 128, 128 ** -0.5, 2, causal=False)
+    if quantised:
+        attn.k_cache, attn.v_cache = quantized_pages(8, 2, device=dev), quantized_pages(8, 2, device=dev)
+    else:
+        attn.k_cache, attn.v_cache = torch.zeros(2, 8, 256, 2, 128, dtype=BF16, device=dev)
+    return attn
+
+
+def test_uploads_inside_a_capture_are_refused(dev):
+    seqs, x = _step_of_reuse(dev)
+    bf16, pages = _layer(dev, False), _layer(dev, True)
+    y = torch.zeros(4, device=dev)
+
+    def capture(layer, match):
+        graph = torch.cuda.CUDAGraph()
+        y.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            y.add_(1)
+            with pytest.raises(RuntimeError, match=match):
+                layer(*x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (y == 1).all()
+
+    prepare_step(seqs, dev)
+    for layer in (bf16, pages):
+        capture(layer, "before the capture")
+    # the plan is there, its page table is not
+    bf16(*x)
+    capture(pages, "page table, before the capture")
+    reset_context()
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_after_one_forward_the_step_is_captured(dev, quantised):
+    seqs, x = _step_of_reuse(dev)
+    layer = _layer(dev, quantised)
+    if quantised:
+        for t in (layer.k_cache, layer.v_cache):
+            t.copy_(torch.randint(0, 120, t.shape, dtype=torch.uint8, device=dev))
+    else:
+        for t in (layer.k_cache, layer.v_cache):
+            t.normal_()
+    prepare_step(seqs, dev)
+    want = layer(*x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(*x)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(layer(*x), want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    reset_context()
