@@ -460,10 +460,8 @@ class StepPlan:
         self.cached_ids = dev[o:o + max(1, len(cached))]; o += max(1, len(cached))
         self.slot_off = dev[o:o + slot_off.size]; o += slot_off.size
         self.jobs = dev[o:o + jobs.size]
-        tables = [getattr(seqs[i], "block_table", None) for i in cached]
-        if all(t is not None for t in tables):
-            self._keeps = [keeps[i] for i in cached]
-            self._block_tables = [list(t)[:-(-n // _capi.PAGE_ROWS)] for n, t in zip(self._keeps, tables)]
+        # what page_tables() needs, which only 8-bit pages call
+        self._cached_seqs = [(seqs[i], keeps[i]) for i in cached]
 
     def _take(self, lay: StepLayout, device) -> None:
         self.device = device
@@ -473,7 +471,7 @@ class StepPlan:
         self._args = {}
         self._packed = {}
         self.last_idx = None
-        self._block_tables = None
+        self._cached_seqs = self._block_tables = None
         self._pages = None
 
     @classmethod
@@ -510,16 +508,18 @@ class StepPlan:
         if self._pages is None:
             t = self._block_tables
             if t is None:
-                raise ValueError("8-bit pages need the sequences' block tables (seq.block_table)")
-            if not isinstance(t, torch.Tensor):
+                tables = [getattr(seq, "block_table", None) for seq, _ in self._cached_seqs or []]
+                if self._cached_seqs is None or any(pages is None for pages in tables):
+                    raise ValueError("8-bit pages need the sequences' block tables (seq.block_table)")
                 _not_captured("run the step's forward over 8-bit pages once, which uploads its page table,",
                               self.device)
                 width = max(1, -(-self.max_keep_cached // _capi.PAGE_ROWS))
                 host = torch.full((self.n_cached, width), -1, dtype=torch.int32)
-                for r, pages in enumerate(t):
-                    if len(pages) < -(-self._keeps[r] // _capi.PAGE_ROWS):
-                        raise ValueError(f"cached sequence {r}: {self._keeps[r]} rows in {len(pages)} pages")
-                    host[r, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+                for r, (pages, (_, keep)) in enumerate(zip(tables, self._cached_seqs)):
+                    need = -(-keep // _capi.PAGE_ROWS)
+                    if len(pages) < need:
+                        raise ValueError(f"cached sequence {r}: {keep} rows in {len(pages)} pages")
+                    host[r, :need] = torch.tensor(pages[:need], dtype=torch.int32)
                 if self.device.type == "cuda":
                     host = host.pin_memory()
                 t = host.to(self.device, non_blocking=True)
