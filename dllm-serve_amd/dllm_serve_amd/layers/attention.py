@@ -461,7 +461,7 @@ class StepPlan:
         self.slot_off = dev[o:o + slot_off.size]; o += slot_off.size
         self.jobs = dev[o:o + jobs.size]
         # what page_tables() needs, which only 8-bit pages call
-        self._cached_seqs = [(seqs[i], keeps[i]) for i in cached]
+        self._cached_seqs = [(seqs[i], keeps[i], slot_mapping[i]) for i in cached]
 
     def _take(self, lay: StepLayout, device) -> None:
         self.device = device
@@ -503,30 +503,49 @@ class StepPlan:
     def page_tables(self):
         """(page table [n_cached, max_pages], cached lengths [n_cached]) of the
         state-2 sequences on the device, int32: what attention over 8-bit
-        pages reads instead of the slot lists.  Their rows are the pages' rows in
-        order, as the slot lists of prepare_step and dllm_step_build name them."""
+        pages reads instead of the slot lists.
+
+        A host-built plan's pages are those of context.slot_mapping, every 256th
+        slot's.  The lists must name whole pages, the last one from row 0 on, in any
+        order inside a page; lists and CPU tensors are checked, device tensors are
+        not (that would wait for the GPU)."""
         if self._pages is None:
             t = self._block_tables
             if t is None:
-                tables = [getattr(seq, "block_table", None) for seq, _ in self._cached_seqs or []]
-                if self._cached_seqs is None or any(pages is None for pages in tables):
-                    raise ValueError("8-bit pages need the sequences' block tables (seq.block_table)")
-                _not_captured("run the step's forward over 8-bit pages once, which uploads its page table,",
-                              self.device)
-                width = max(1, -(-self.max_keep_cached // _capi.PAGE_ROWS))
-                host = torch.full((self.n_cached, width), -1, dtype=torch.int32)
-                for r, (pages, (_, keep)) in enumerate(zip(tables, self._cached_seqs)):
-                    need = -(-keep // _capi.PAGE_ROWS)
-                    if len(pages) < need:
-                        raise ValueError(f"cached sequence {r}: {keep} rows in {len(pages)} pages")
-                    host[r, :need] = torch.tensor(pages[:need], dtype=torch.int32)
-                if self.device.type == "cuda":
-                    host = host.pin_memory()
-                t = host.to(self.device, non_blocking=True)
+                t = self._pages_of_slots()
             elif not self.cached_identity:
                 t = t.index_select(0, self.cached_ids)
             self._pages = t, self.slot_off[1:] - self.slot_off[:-1]
         return self._pages
+
+    def _pages_of_slots(self) -> torch.Tensor:
+        if self._cached_seqs is None:
+            raise ValueError("8-bit pages need the sequences' block tables on the device")
+        _not_captured("run the step's forward over 8-bit pages once, which uploads its page table,", self.device)
+        R = _capi.PAGE_ROWS
+        width = max(1, -(-self.max_keep_cached // R))
+        at = torch.zeros(self.n_cached, width, dtype=torch.int64)  # past a sequence's pages: not read
+        base = 0
+        for r, (seq, keep, slots) in enumerate(self._cached_seqs):
+            need = -(-keep // R)
+            pages = getattr(seq, "block_table", None)
+            if pages is not None and len(pages) < need:
+                raise ValueError(f"cached sequence {r}: {keep} rows in {len(pages)} pages")
+            if not (isinstance(slots, torch.Tensor) and slots.is_cuda):
+                a = np.asarray(slots, dtype=np.int64).reshape(-1)
+                for j in range(0, keep, R):
+                    run = np.sort(a[j:j + R])
+                    if run[0] % R or not np.array_equal(run, run[0] + np.arange(run.size)):
+                        raise ValueError(f"cached sequence {r}: slots {j} .. {j + run.size - 1} of its slot_mapping are not "
+                                         f"the rows of one cache page from row 0 on, which 8-bit pages are read by")
+            at[r, :need] = base + R * torch.arange(need)
+            base += keep
+        if base == 0:
+            return torch.full((self.n_cached, width), -1, dtype=torch.int32, device=self.device)
+        if self.device.type == "cuda":
+            at = at.pin_memory()
+        at = at.to(self.device, non_blocking=True)
+        return (self.slots.index_select(0, at.view(-1)) >> 8).view(self.n_cached, width)
 
     def launch_args(self, Hq: int, Hkv: int, D: int) -> dict:
         """Device addresses of the step's tables and the K3b workspace for

@@ -7,7 +7,7 @@ from dllm_serve_amd.engine.kv_cache import quantized_pages
 from dllm_serve_amd.engine.sequence import PageAllocator, Sequence, prepare_step
 from dllm_serve_amd.layers.attention import Attention
 from dllm_serve_amd.sparse.state import SparseConfig
-from dllm_serve_amd.utils.context import reset_context
+from dllm_serve_amd.utils.context import get_context, reset_context
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -84,4 +84,27 @@ def test_after_one_forward_the_step_is_captured(dev, quantised):
         assert torch.equal(layer(*x), want)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+    reset_context()
+
+
+def test_pages_follow_the_slot_mapping(dev):
+    """8-bit pages that the block table does not name: state 2 reads the rows of the slot
+    mapping, as it does with a bf16 cache."""
+    seqs, x = _step_of_reuse(dev)
+    layer = _layer(dev, True)
+    for t in (layer.k_cache, layer.v_cache):
+        t.copy_(torch.randint(0, 120, t.shape, dtype=torch.uint8, device=dev))
+    prepare_step(seqs, dev)
+    want = layer(*x)
+    moved = [4, 6, 1]  # the sequences' pages 5 | 2, 7 elsewhere
+    for t in (layer.k_cache, layer.v_cache):
+        t[moved] = t[[5, 2, 7]]
+        t[[5, 2, 7]] = 0
+    reset_context()
+    prepare_step(seqs, dev)
+    ctx = get_context()
+    to = dict(zip([5, 2, 7], moved))
+    ctx.slot_mapping = [torch.tensor([to[s // 256] * 256 + s % 256 for s in m.tolist()], dtype=torch.int32, device=dev)
+                        for m in ctx.slot_mapping]
+    assert torch.equal(layer(*x), want)
     reset_context()

@@ -59,13 +59,60 @@ def test_page_tables():
     reset_context()
 
 
-def test_page_tables_refuse():
+def test_page_tables_refuse_too_few_pages():
     seqs = _reuse_step()
     plan = StepPlan(get_context(), CPU)
     seqs[2].block_table = list(seqs[2].block_table)[:2]
     with pytest.raises(ValueError, match="rows in 2 pages"):
         plan.page_tables()
-    del seqs[1].block_table
+    reset_context()
+
+
+def test_pages_are_those_of_the_slot_mapping():
+    """Other pages than the block table's, rows of a page in another order, no block table."""
+    seqs = _reuse_step()
+    ctx = get_context()
+    rows = [s.current_sparse_token for s in seqs]
+    pages = [[20, 11], [12, 30], [14, 13, 21, 40]]
+    want = [p[:-(-n // 256)] for p, n in zip(pages, rows)]
+    maps = [[p[r // 256] * 256 + r % 256 for r in range(n)] for p, n in zip(pages, rows)]
+    maps[1] = torch.tensor(maps[1], dtype=torch.int32)
+    maps[2][:256] = maps[2][:256][::-1]
+    del seqs[0].block_table
+    ctx.slot_mapping = maps
+    table, lens = StepPlan(ctx, CPU).page_tables()
+    assert lens.tolist() == rows
+    assert [row[:len(w)] for row, w in zip(table.tolist(), want)] == want
+    reset_context()
+
+
+@pytest.mark.parametrize("change", ["starts in a page", "gap", "two pages", "row twice", "outside"])
+def test_mappings_that_pages_cannot_be_read_by(change):
+    seqs = _reuse_step((400,))
+    ctx = get_context()
+    n = seqs[0].current_sparse_token
+    assert 256 < n < 500
+    m = [5 * 256 + r if r < 256 else 7 * 256 + r - 256 for r in range(n)]
+    if change == "starts in a page":
+        m = [x + 1 for x in m]
+    elif change == "gap":
+        m[-1] += 1
+    elif change == "two pages":
+        m[10], m[300] = m[300], m[10]
+    elif change == "row twice":
+        m[10] = m[11]
+    else:
+        m[0] = -1
+    ctx.slot_mapping = [m]
+    with pytest.raises(ValueError, match="one cache page"):
+        StepPlan(ctx, CPU).page_tables()
+    reset_context()
+
+
+def test_a_plan_of_device_tables_needs_block_tables():
+    seqs = _reuse_step()
+    plan = StepPlan(get_context(), CPU)
+    plan._cached_seqs = None  # as StepPlan.from_device leaves it
     with pytest.raises(ValueError, match="block tables"):
         plan.page_tables()
     reset_context()
