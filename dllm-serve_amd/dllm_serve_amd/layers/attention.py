@@ -547,24 +547,31 @@ class StepPlan:
         at = at.to(self.device, non_blocking=True)
         return (self.slots.index_select(0, at.view(-1)) >> 8).view(self.n_cached, width)
 
-    def launch_args(self, Hq: int, Hkv: int, D: int) -> dict:
-        """Device addresses of the step's tables and the K3b workspace for
-        one head shape, computed once per step for all layers.  The workspace
-        is keyed by the head shape and held in the returned dict, so the
-        address cached here stays valid while the plan lives, whatever other
+    def launch_args(self, Hq: int, Hkv: int, D: int, pages: bool = False) -> dict:
+        """Device addresses of the step's tables and the workspace of its
+        attention over cached rows (K3b, or with ``pages`` the one over 8-bit
+        pages) for one head shape, computed once per step for all layers.  The
+        workspace is keyed by the head shape and held in the returned dict, so
+        the address cached here stays valid while the plan lives, whatever other
         head shapes later ask for."""
-        key = (Hq, Hkv, D)
+        key = (Hq, Hkv, D, "pages") if pages else (Hq, Hkv, D)
         a = self._args.get(key)
         if a is None:
-            ws = self.workspace(("cached",) + key, _capi.block_cached_workspace_size(
-                self.n_cached, self.max_q_cached, self.max_keys_cached, Hq, Hkv, D)) if self.n_cached else None
+            need = 0
+            if self.n_cached and pages:
+                need = _capi.chunk_workspace_size(self.n_cached, self.max_q_cached, self.max_keep_cached, Hq, Hkv, D,
+                                                  self.rows_cached, self.keeps_cached)
+            elif self.n_cached:
+                need = _capi.block_cached_workspace_size(self.n_cached, self.max_q_cached, self.max_keys_cached, Hq,
+                                                         Hkv, D)
+            ws = self.workspace(("cached",) + key, need)
             a = dict(cu=self.cu.data_ptr(), slots=self.slots.data_ptr(), slot_off=self.slot_off.data_ptr(),
                      dense_ids=None if self.dense_identity else self.dense_ids.data_ptr(),
                      cached_ids=None if self.cached_identity else self.cached_ids.data_ptr(),
                      ws=None if ws is None else ws.data_ptr(), ws_bytes=0 if ws is None else ws.numel(),
                      ws_tensor=ws)
             self._args[key] = a
-            if not (self.any_skipped or self.n_job) and self.device.type == "cuda":
+            if not (pages or self.any_skipped or self.n_job) and self.device.type == "cuda":
                 # the step's launches for the native form (csrc/native.cpp, PlanArgs)
                 dev = self.device.index if self.device.index is not None else torch.cuda.current_device()
                 self._packed[key] = struct.pack(
@@ -632,15 +639,17 @@ class Attention(nn.Module):
         cache that passed keeps passing while the same tensors keep their
         addresses and sizes."""
         kc, vc = self.k_cache, self.v_cache
-        if kc.dtype == torch.uint8:
-            if _check_pages(kc, vc, device) != self.num_kv_heads or self.head_dim != 128:
-                raise ValueError(f"8-bit pages of {kc.shape[1]} KV heads of 128, the layer has {self.num_kv_heads} of "
-                                 f"{self.head_dim}")
-            return kc.data_ptr(), vc.data_ptr(), min(kc.shape[0], vc.shape[0]) * _capi.PAGE_ROWS
         key = (kc.data_ptr(), vc.data_ptr(), kc.numel(), vc.numel(), device)
         ok = self._cache_ok
         if ok is not None and ok[0]() is kc and ok[1]() is vc and ok[2:7] == key:
             return ok[7]
+        if kc.dtype == torch.uint8:
+            if _check_pages(kc, vc, device) != self.num_kv_heads or self.head_dim != 128:
+                raise ValueError(f"8-bit pages of {kc.shape[1]} KV heads of 128, the layer has {self.num_kv_heads} of "
+                                 f"{self.head_dim}")
+            res = (kc.data_ptr(), vc.data_ptr(), min(kc.shape[0], vc.shape[0]) * _capi.PAGE_ROWS)
+            self._cache_ok = (weakref.ref(kc), weakref.ref(vc)) + key + (res,)
+            return res
         for t, n in ((kc, "k_cache"), (vc, "v_cache")):
             if (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != device or t.dim() < 2
                     or tuple(t.shape[-2:]) != (self.num_kv_heads, self.head_dim)):
@@ -666,7 +675,7 @@ class Attention(nn.Module):
         if nq != plan.total_rows or nk != plan.total_rows or nv != plan.total_rows:
             raise ValueError(f"q/k/v have {nq}/{nk}/{nv} rows, the step's sequences feed {plan.total_rows}")
         first = (Hq, Hkv, D) not in plan._args
-        args = plan.launch_args(Hq, Hkv, D)
+        args = plan.launch_args(Hq, Hkv, D, bool(plan.n_cached) and self.k_cache.dtype == torch.uint8)
         if first:  # the step's first layer of this shape: its launch arguments exist only now
             o = self._native_attention(plan, q, k, v)
             if o is not None:
@@ -712,11 +721,8 @@ class Attention(nn.Module):
         """The state-2 sequences' blocks against their cached rows in 8-bit pages and against themselves."""
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
         table, lens = plan.page_tables()
-        sizes = (plan.n_cached, plan.max_q_cached, plan.max_keep_cached)
-        need = _capi.chunk_workspace_size(*sizes, Hq, Hkv, D, plan.rows_cached, plan.keeps_cached)
-        ws = plan.workspace(("pages", Hq, Hkv, D), need)
-        _capi.attn_chunk_paged_fwd_raw(qp, kp, vp, op, args["cu"], args["cached_ids"], *sizes, plan.rows_cached,
-                                       plan.keeps_cached, kc, vc, _capi.CACHE_FP8, cache_slots // _capi.PAGE_ROWS,
-                                       table.data_ptr(), table.shape[1], lens.data_ptr(), 0, Hq, Hkv, D, q_st, k_st,
-                                       v_st, o_st, float(self.scale), None if ws is None else ws.data_ptr(), need,
-                                       stream)
+        _capi.attn_chunk_paged_fwd_raw(qp, kp, vp, op, args["cu"], args["cached_ids"], plan.n_cached,
+                                       plan.max_q_cached, plan.max_keep_cached, plan.rows_cached, plan.keeps_cached,
+                                       kc, vc, _capi.CACHE_FP8, cache_slots // _capi.PAGE_ROWS, table.data_ptr(),
+                                       table.shape[1], lens.data_ptr(), 0, Hq, Hkv, D, q_st, k_st, v_st, o_st,
+                                       float(self.scale), args["ws"], args["ws_bytes"], stream)

@@ -108,3 +108,24 @@ def test_pages_follow_the_slot_mapping(dev):
                         for m in ctx.slot_mapping]
     assert torch.equal(layer(*x), want)
     reset_context()
+
+
+def test_a_step_over_pages_takes_one_workspace(dev):
+    seqs, x = _step_of_reuse(dev)
+    layer = _layer(dev, True)
+    prepare_step(seqs, dev)
+    want = layer(*x)
+    plan = get_context()._dllm_plan
+    assert list(plan._args) == [(8, 2, 128, "pages")]
+    other = _layer(dev, True)       # another layer with the checked caches of the first
+    other.k_cache, other.v_cache = layer.k_cache, layer.v_cache
+    assert torch.equal(other(*x), want) and len(plan._args) == 1
+    # a bf16 layer in the same step has its own
+    _layer(dev, False)(*x)
+    assert set(plan._args) == {(8, 2, 128, "pages"), (8, 2, 128)}
+    assert torch.equal(layer(*x), want)
+    # caches that are rebound are checked again
+    layer.k_cache = torch.zeros(8, 2, 100, dtype=torch.uint8, device=dev)
+    with pytest.raises(ValueError, match="k_cache"):
+        layer(*x)
+    reset_context()

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from dllm_serve_amd import _capi
 from dllm_serve_amd.engine.sequence import PageAllocator, Sequence, prepare_step
 from dllm_serve_amd.layers.attention import StepPlan
 from dllm_serve_amd.sparse.state import SparseConfig
@@ -115,4 +116,22 @@ def test_a_plan_of_device_tables_needs_block_tables():
     plan._cached_seqs = None  # as StepPlan.from_device leaves it
     with pytest.raises(ValueError, match="block tables"):
         plan.page_tables()
+    reset_context()
+
+
+def test_workspace_of_the_attention_that_runs():
+    """Over 8-bit pages the other attention's workspace is not allocated."""
+    _reuse_step((200, 400, 1500))
+    plan = StepPlan(get_context(), CPU)
+    sizes = {p: _capi.chunk_workspace_size(3, plan.max_q_cached, plan.max_keep_cached, 2, 2, 128, plan.rows_cached,
+                                           plan.keeps_cached)
+             if p else _capi.block_cached_workspace_size(3, plan.max_q_cached, plan.max_keys_cached, 2, 2, 128)
+             for p in (True, False)}
+    assert sizes[True] > 0 and sizes[False] > 0
+    a = plan.launch_args(2, 2, 128, True)
+    assert a["ws_bytes"] == sizes[True] and a is plan.launch_args(2, 2, 128, True)
+    assert [t.numel() for t in plan._ws.values()] == [sizes[True]]
+    assert plan.launch_args(2, 2, 128)["ws_bytes"] == sizes[False]
+    assert sorted(t.numel() for t in plan._ws.values()) == sorted(sizes.values())
+    assert plan.launch_args(2, 2, 128, True) is a
     reset_context()
