@@ -44,6 +44,8 @@ struct ChunkArgs {
 constexpr int kTileKeys = 32;   // keys of a wavefront's tile (chunk_rows_kernel)
 constexpr int kBigTile = 64;    // keys of a workgroup's tile (chunk_tile_kernel)
 constexpr int kMaxSplitTiles = 62 * kPageRows / kTileKeys;  // chunk_rows_kernel: at most 63 pages, one a lane
+constexpr int64_t kMaxParts = (int64_t)1 << 30;             // bytes of parts (workspace) in a launch
+constexpr int64_t kMaxBlocks = (int64_t)1 << 22;            // workgroups of a launch: 2^32 threads is HIP's limit
 
 // A segment: new rows' first row and count, cached rows.
 struct Segment {
@@ -1154,7 +1156,8 @@ struct ChunkPlan {
   int bm;                        // M rows of a workgroup
   int max_split, tiles_per_split;
   int mtiles;                    // of the largest segment
-  int64_t logical;               // workgroups
+  int run;                       // segments of a launch
+  int64_t logical;               // its workgroups
 };
 // total_q / total_cached: the segments' sums, or an upper bound of them.
 static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached, int Hq,
@@ -1211,10 +1214,27 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   if (!p.tile_form && (tps * 3 > tiles * 2 || tiles <= 24)) tps = tiles;
   if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
   if (tps < 1) tps = 1;
+  // Every segment of a launch has room for the parts that the one with the most rows and
+  // the one with the most keys have together: a piece of a prompt among many single tokens
+  // would ask for tens of gigabytes (2048 rows behind 131072 and 63 tokens behind 500,
+  // 28/4 heads: 65).  So the segments are launched in runs, one after the other, that
+  // use the same workspace; a run that fills it has over sixteen thousand workgroups.
+  const int64_t part = Hkv * (int64_t)p.mtiles * p.bm * (HD + 2) * (int64_t)sizeof(float);  // of all rows of a segment
+  const int64_t most = std::max<int64_t>(1, kMaxParts / part);
+  if ((tiles + tps - 1) / tps > most) {
+    tps = (tiles + most - 1) / most;
+    if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
+  }
   if (tps > 0x3fffffff) tps = 0x3fffffff;
   p.tiles_per_split = (int)tps;
   p.max_split = (int)std::max<int64_t>(1, (tiles + tps - 1) / tps);
-  p.logical = n_seg * Hkv * p.mtiles * p.max_split;
+  const int64_t blocks = Hkv * (int64_t)p.mtiles * p.max_split;  // of a segment
+  int64_t run = std::min(n_seg, kMaxBlocks / blocks);
+  if (p.max_split > 1) run = std::min(run, kMaxParts / (part * p.max_split));
+  run = std::max<int64_t>(run, 1);
+  const int64_t runs = (n_seg + run - 1) / run;
+  p.run = (int)((n_seg + runs - 1) / runs);
+  p.logical = p.run * blocks;
   return p;
 }
 static size_t chunk_ws(const ChunkPlan& p) {
@@ -1243,13 +1263,13 @@ extern "C" size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_c
                              chunk_total(total_cached, n_seg, max_cached), Hq, Hkv));
 }
 
-static int chunk_grid(const ChunkPlan& p, int* chunk) {
+static int chunk_grid(int64_t logical, int mtiles, int* chunk) {
   // The M tiles of a (segment, KV head) read the same keys: next to each other on one XCD,
   // but no more than four, which would give one XCD the longest work (8 ragged
   // pieces, 28/4 heads: chunks of 16 156 us, 4 140; 8192 new rows, 32 heads, 662 and 678).
-  *chunk = std::min(p.mtiles, 4);
+  *chunk = std::min(mtiles, 4);
   const int64_t grain = 8 * (int64_t)*chunk;
-  return (int)((p.logical + grain - 1) / grain * grain);
+  return (int)((logical + grain - 1) / grain * grain);
 }
 
 extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached,
@@ -1261,7 +1281,7 @@ extern "C" int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached
   if (n_seg > 0 && max_q > 0) {
     p = chunk_plan(n_seg, max_q, max_cached, chunk_total(total_q, n_seg, max_q),
                    chunk_total(total_cached, n_seg, max_cached), Hq, Hkv);
-    blocks = p.logical > (1 << 28) ? 0 : chunk_grid(p, &chunk);
+    blocks = p.logical > kMaxBlocks ? 0 : chunk_grid(p.logical, p.mtiles, &chunk);
   }
   if (rows) *rows = p.bm;
   if (n_split) *n_split = p.max_split;
@@ -1319,7 +1339,7 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
   a.scale_log2 = softmax_scale * kLog2e;
   const ChunkPlan p = chunk_plan(n_seg, max_q, max_cached, chunk_total(total_q, n_seg, max_q),
                                  chunk_total(total_cached, n_seg, max_cached), Hq, Hkv);
-  if (p.logical > (int64_t)1 << 28 || n_seg > 65535 || Hkv > 65535)
+  if (p.logical > kMaxBlocks || n_seg > 65535 || Hkv > 65535)
     return fail(DLLM_ERR_INVALID_ARG, "%s: problem too large", name);
   const size_t need = chunk_ws(p);
   if (need) {
@@ -1330,47 +1350,62 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
     a.ws = reinterpret_cast<float*>(workspace);
   }
   int chunk;
-  const int grid = chunk_grid(p, &chunk);
-  const int chunk_pages = chunk + 32 * (max_cached > 0 && num_pages > 0 ? max_pages : 0);
-  auto start = [&](auto kern, dim3 blocks, int threads, int lds_bytes) {
-    kern<<<blocks, dim3((unsigned)threads), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
-        cu, seg_ids, cached_len, page_table, chunk_pages, (int)p.logical, p.mtiles, p.max_split, p.tiles_per_split, Hkv, a);
-    return check_launch(name);
-  };
+  const int chunk_pages_row = max_cached > 0 && num_pages > 0 ? max_pages : 0;
   const bool fp8 = cache_type == DLLM_CACHE_FP8;
-  auto launch = [&](auto kern, int lds_bytes, int threads = 256) -> int {
-    int e = set_lds(kern, lds_bytes, name);
-    if (e) return e;
-    return start(kern, dim3((unsigned)grid), threads, lds_bytes);
-  };
   // Few workgroups of some length: eight wavefronts each, which halves the turns (and takes a
   // CU's LDS, so 8-bit rows only).  One token behind 511 rows, 32 heads, 8.5 -> 7.4 us, behind
   // 767 10.1 -> 8.5, 128 rows behind 4000 29.9 -> 26.9; not where a workgroup a CU streams from
   // memory (4 tokens behind 2000 18.6, 18.8), nor for 32 rows of few keys, whose merge is
   // longer (32 behind 300 10.0, 10.4).
   const bool eight = fp8 && p.logical <= (p.mtiles > 1 ? 256 : 192) && p.tiles_per_split > (p.nb == 1 ? 4 : 12);
-  if (p.tile_form)
-    rc = launch(fp8 ? chunk_tile_kernel<true> : chunk_tile_kernel<false>, 2 * kTileStage);
-  else if (eight)
-    rc = p.nb == 1 ? launch(chunk_rows_kernel<1, true, true, 8>, rows_lds<1, true, 8>(), 512)
-         : p.mtiles == 1 ? launch(chunk_rows_kernel<2, true, true, 8>, rows_lds<2, true, 8>(), 512)
-                         : launch(chunk_rows_kernel<2, true, false, 8>, rows_lds<2, true, 8>(), 512);
-  else if (p.nb == 1)  // at most 16 rows
-    rc = fp8 ? launch(chunk_rows_kernel<1, true, true, 4>, rows_lds<1, true, 4>())
-             : launch(chunk_rows_kernel<1, false, true, 4>, rows_lds<1, false, 4>());
-  else if (p.mtiles == 1)
-    rc = fp8 ? launch(chunk_rows_kernel<2, true, true, 4>, rows_lds<2, true, 4>())
-             : launch(chunk_rows_kernel<2, false, true, 4>, rows_lds<2, false, 4>());
-  else
-    rc = fp8 ? launch(chunk_rows_kernel<2, true, false, 4>, rows_lds<2, true, 4>())
-             : launch(chunk_rows_kernel<2, false, false, 4>, rows_lds<2, false, 4>());
-  if (rc || p.max_split == 1) return rc;
-  auto join = [&](auto one, auto eight) {
-    const bool many = p.max_split > 8;
-    const int64_t rows = (int64_t)max_q * a.g;
-    return start(many ? eight : one, dim3((unsigned)(many ? rows : (rows + 7) / 8), (unsigned)Hkv, (unsigned)n_seg), 256, 0);
-  };
-  if (p.tile_form) return join(chunk_combine_kernel<kTileRows, true, 1>, chunk_combine_kernel<kTileRows, true, 8>);
-  return p.nb == 1 ? join(chunk_combine_kernel<16, false, 1>, chunk_combine_kernel<16, false, 8>)
-                   : join(chunk_combine_kernel<32, false, 1>, chunk_combine_kernel<32, false, 8>);
+  for (int s0 = 0; s0 < n_seg; s0 += p.run) {
+    const int segs = std::min(p.run, n_seg - s0);
+    const int logical = (int)(p.logical / p.run * segs);
+    const int grid = chunk_grid(logical, p.mtiles, &chunk);
+    const int chunk_pages = chunk + 32 * chunk_pages_row;
+    auto start = [&](auto kern, dim3 blocks, int threads, int lds_bytes) {
+      kern<<<blocks, dim3((unsigned)threads), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
+          seg_ids ? cu : cu + s0, seg_ids ? seg_ids + s0 : nullptr, cached_len + s0,
+          page_table + (int64_t)s0 * chunk_pages_row, chunk_pages, logical, p.mtiles, p.max_split, p.tiles_per_split, Hkv,
+          a);
+      return check_launch(name);
+    };
+    auto launch = [&](auto kern, int lds_bytes, int threads = 256) -> int {
+      int e = set_lds(kern, lds_bytes, name);
+      if (e) return e;
+      return start(kern, dim3((unsigned)grid), threads, lds_bytes);
+    };
+    if (p.tile_form)
+      rc = launch(fp8 ? chunk_tile_kernel<true> : chunk_tile_kernel<false>, 2 * kTileStage);
+    else if (eight)
+      rc = p.nb == 1 ? launch(chunk_rows_kernel<1, true, true, 8>, rows_lds<1, true, 8>(), 512)
+           : p.mtiles == 1 ? launch(chunk_rows_kernel<2, true, true, 8>, rows_lds<2, true, 8>(), 512)
+                           : launch(chunk_rows_kernel<2, true, false, 8>, rows_lds<2, true, 8>(), 512);
+    else if (p.nb == 1)  // at most 16 rows
+      rc = fp8 ? launch(chunk_rows_kernel<1, true, true, 4>, rows_lds<1, true, 4>())
+               : launch(chunk_rows_kernel<1, false, true, 4>, rows_lds<1, false, 4>());
+    else if (p.mtiles == 1)
+      rc = fp8 ? launch(chunk_rows_kernel<2, true, true, 4>, rows_lds<2, true, 4>())
+               : launch(chunk_rows_kernel<2, false, true, 4>, rows_lds<2, false, 4>());
+    else
+      rc = fp8 ? launch(chunk_rows_kernel<2, true, false, 4>, rows_lds<2, true, 4>())
+               : launch(chunk_rows_kernel<2, false, false, 4>, rows_lds<2, false, 4>());
+    if (rc || p.max_split == 1) {
+      if (rc) return rc;
+      continue;
+    }
+    auto join = [&](auto one, auto eight) {
+      const bool many = p.max_split > 8;
+      const int64_t rows = (int64_t)max_q * a.g;
+      return start(many ? eight : one, dim3((unsigned)(many ? rows : (rows + 7) / 8), (unsigned)Hkv, (unsigned)segs), 256,
+                   0);
+    };
+    if (p.tile_form)
+      rc = join(chunk_combine_kernel<kTileRows, true, 1>, chunk_combine_kernel<kTileRows, true, 8>);
+    else
+      rc = p.nb == 1 ? join(chunk_combine_kernel<16, false, 1>, chunk_combine_kernel<16, false, 8>)
+                     : join(chunk_combine_kernel<32, false, 1>, chunk_combine_kernel<32, false, 8>);
+    if (rc) return rc;
+  }
+  return DLLM_OK;
 }

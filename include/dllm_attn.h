@@ -253,14 +253,16 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * 16-byte aligned, token strides multiples of 8 elements, and a segment's new rows span
  * at most 4 GiB of q, k or v.  workspace: dllm_attn_chunk_workspace_size(...) bytes
  * (0 where one workgroup takes all keys of a row), any contents; calls that may
- * overlap need workspaces of their own.
+ * overlap need workspaces of their own.  It is 1 GiB at most, or what one segment
+ * with a KV head's rows in parts of 15872 keys takes where that is more: a call whose
+ * segments would need more launches them in several runs.
  */
 #define DLLM_CACHE_BF16 0
 #define DLLM_CACHE_FP8 1
 size_t dllm_attn_chunk_workspace_size(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached,
                                       int Hq, int Hkv, int D);
 /* Launch shape for these sizes, without launching: M rows (tokens x Hq / Hkv) of a
- * workgroup, workgroups along the keys, grid.  Any output pointer may be null. */
+ * workgroup, workgroups along the keys, grid of a run.  Any output pointer may be null. */
 int dllm_attn_chunk_launch_shape(int n_seg, int max_q, int max_cached, int64_t total_q, int64_t total_cached, int Hq,
                                  int Hkv, int D, int* rows, int* n_split, int* grid);
 int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k, const dllm_bf16* v, dllm_bf16* o,

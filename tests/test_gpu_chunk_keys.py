@@ -1,0 +1,166 @@
+"""chunk_attention with keys that decide the output one by one, so that a key, tile, part
+or page that is left out, read from elsewhere, joined twice or seen too early shows,
+however many keys there are.
+
+Every key is a code of random signs, 6 c.  A row of q is the sum of two keys' codes: the
+two have one and the same score, 6 (128 + c_a c_b) / sqrt(128), and every other key's is 6 c_u
+(c_a + c_b) / sqrt(128), whose standard deviation is 6 sqrt(256 + 2 c_a c_b) / sqrt(128).  With
+partners of c_a c_b >= -10 and 2^32 pairs of a row and a key (6.3 standard deviations) the
+others lie 10 below at least, and 37 on the average, so together they weigh below 1e-3 of
+a value of at most 6.  The output is (V_a + V_b) / 2, up to the rounding of the two
+probabilities to bf16 (2^-8 each, in the product and in the sum, which may be made against
+different maxima) and of the result (2^-8)."""
+import pytest
+import torch
+
+from dllm_serve_amd import _capi
+from dllm_serve_amd.engine.kv_cache import quantized_pages
+from dllm_serve_amd.layers.attention import ChunkPlan, chunk_attention, load_kvcache, store_kvcache
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+SCALE = 128 ** -0.5
+
+
+class Marked:
+    """Sequences whose keys are codes.  With `share` they have the same pages."""
+
+    def __init__(self, dev, lens, cached, Hq, Hkv, bits, seed, share=False, mask_block=1):
+        self.g = torch.Generator(device=dev).manual_seed(seed)
+        self.dev, self.lens, self.cached, self.Hq, self.Hkv, self.mask_block = dev, lens, cached, Hq, Hkv, mask_block
+        need = [-(-c // 256) for c in cached]
+        pages = (max(need) if share else sum(need)) + 2
+        perm = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        self.tables = [perm[:n] if share else perm[sum(need[:b]):sum(need[:b + 1])] for b, n in enumerate(need)]
+        rows = pages * 256
+        self.n = sum(lens)
+        signs = torch.randint(0, 2, (rows + self.n, Hkv, 128), generator=self.g, device=dev, dtype=torch.int8)
+        self.codes = (2 * signs - 1).to(BF16)
+        values = torch.randn(rows + self.n, Hkv, 128, generator=self.g, device=dev).to(BF16)
+        keys = self.codes * 6
+        self.k, self.v = keys[rows:].contiguous(), values[rows:].contiguous()
+        if bits == 8:
+            self.kc, self.vc = quantized_pages(pages, Hkv, device=dev), quantized_pages(pages, Hkv, device=dev)
+            slots = torch.arange(rows, dtype=torch.int32, device=dev)
+            store_kvcache(keys[:rows], values[:rows], self.kc, self.vc, slots)
+            held = torch.empty_like(keys[:rows])
+            load_kvcache(held, values[:rows], self.kc, self.vc, slots)
+            assert torch.equal(held, keys[:rows])
+        else:
+            self.kc, self.vc = (t[:rows].contiguous().view(pages, 256, Hkv, 128) for t in (keys, values))
+        self.values = values
+        self.new0 = rows
+        # per row of q: its sequence's page table, cached rows, new rows and those it sees
+        width = max(1, max(need))
+        tab = torch.zeros(len(lens), width, dtype=torch.int64)
+        for b, t in enumerate(self.tables):
+            tab[b, :len(t)] = torch.tensor(t, dtype=torch.int64)
+        self.tab = tab.to(dev)
+        per_row = [(b, cached[b], sum(lens[:b]), L, self.sees(cached[b], L, t)) for b, L in enumerate(lens) for t in range(L)]
+        self.row = torch.tensor(per_row, dtype=torch.int64).t().to(dev)  # [5, rows]
+        self.plan = ChunkPlan(lens, cached, self.tables, dev, mask_block=mask_block)
+
+    def sees(self, n, L, t):
+        b = self.mask_block
+        return L if b == 0 else min(L, ((n + t) // b + 1) * b - n)
+
+    def shape(self):
+        p = self.plan
+        return _capi.chunk_launch_shape(p.n_seg, p.max_q, p.max_cached, self.Hq, self.Hkv, 128, p.total_rows, p.total_cached)
+
+    def at(self, key):
+        """Rows of codes / values of keys [rows, Hq] (counted over cached, then new rows)."""
+        b, n, r0, _, _ = (x[:, None] for x in self.row)
+        old = key.clamp(max=self.tab.shape[1] * 256 - 1)
+        slot = self.tab[b.expand_as(key), old // 256] * 256 + old % 256
+        return torch.where(key < n, slot, self.new0 + r0 + key - n)
+
+    def of(self, rows, key):
+        head = torch.arange(self.Hq, device=self.dev) // (self.Hq // self.Hkv)
+        return rows[self.at(key), head[None, :].expand_as(key)].float()
+
+    def rand(self, high):
+        """Integers below high [rows, Hq] (at least 1)."""
+        return (torch.rand(high.shape, generator=self.g, device=self.dev) * high).long().clamp(max=high - 1)
+
+    def partner(self, a, pick):
+        """Of eight picks, those whose code is nearest to that of key a."""
+        ca, best, dot = self.of(self.codes, a), None, None
+        for _ in range(8):
+            b = pick()
+            d = (ca * self.of(self.codes, b)).sum(-1)
+            best = b if best is None else torch.where(d > dot, b, best)
+            dot = d if dot is None else torch.maximum(d, dot)
+        return best
+
+    def check(self, a, b, weight_b=0.5):
+        q = (self.of(self.codes, a) + self.of(self.codes, b)).to(BF16)
+        o = chunk_attention(q, self.k, self.v, self.kc, self.vc, self.plan, SCALE).view(self.n, self.Hq, 128).float()
+        va, vb = self.of(self.values, a), self.of(self.values, b)
+        if not weight_b:
+            vb = va
+        ref = 0.5 * (va + vb)
+        tol = 2.0 ** -8 * ref.abs() + 1.05 * 2.0 ** -8 * (va.abs() + vb.abs()) + 6e-3
+        bad = ~((o - ref).abs() <= tol)
+        if bad.any():
+            r, h, d = bad.nonzero()[0].tolist()
+            raise AssertionError(f"row {r} head {h} d {d}: {o[r, h, d]} for {ref[r, h, d]}, keys {a[r, h]} and {b[r, h]}; "
+                                 f"{int(bad.any(-1).sum())} rows differ")
+
+    def seen(self):
+        return (self.row[1] + self.row[4])[:, None].expand(-1, self.Hq)
+
+    def pair(self, a):
+        """Row r's two keys: a and another one that it sees."""
+        n = self.seen()
+        self.check(a, self.partner(a, lambda: (a + 1 + self.rand((n - 1).clamp(min=1))) % n))
+
+    def all_of(self, keys):
+        """Every key of `keys` (of each KV head) decides some row."""
+        keys, per = torch.as_tensor(keys, dtype=torch.int64, device=self.dev), self.n * (self.Hq // self.Hkv)
+        g = self.Hq // self.Hkv
+        r = torch.arange(self.n, device=self.dev)[:, None] * g + torch.arange(self.Hq, device=self.dev)[None, :] % g
+        for i in range(0, len(keys), per):
+            self.pair(torch.minimum(keys[(i + r) % len(keys)], self.seen() - 1))
+
+    def anywhere(self, times):
+        for _ in range(times):
+            self.pair(self.rand(self.seen()))
+
+    def hidden(self, times):
+        """A new row that row r does not see, and one that it sees: the latter alone counts."""
+        _, n, _, L, see = (x[:, None].expand(-1, self.Hq) for x in self.row)
+        for _ in range(times):
+            b = n + torch.where(see < L, see + self.rand((L - see).clamp(min=1)), self.rand(L))
+            a = self.partner(b, lambda: self.rand(n + see))
+            # rows that see all of their sequence's rows are an ordinary pair
+            sees_b = (b - n < see)[..., None]
+            va, vb = self.of(self.values, a), self.of(self.values, b)
+            q = (self.of(self.codes, a) + self.of(self.codes, b)).to(BF16)
+            o = chunk_attention(q, self.k, self.v, self.kc, self.vc, self.plan, SCALE).view(self.n, self.Hq, 128).float()
+            ref = torch.where(sees_b, 0.5 * (va + vb), va)
+            tol = 2.0 ** -8 * ref.abs() + 1.05 * 2.0 ** -8 * (va.abs() + vb.abs()) + 6e-3
+            assert ((o - ref).abs() <= tol).all()
+
+
+# ---- runs of segments ----------------------------------------------------------------
+# Batches whose parts need more than the workspace's limit are launched in several runs.
+
+RUNS = [
+    # one long sequence among single tokens: rows form, parts set by the page ids of a split
+    ([1] * 1100, [300, 5] * 200 + [16200] + [40, 0, 256] * 233, 64, 64, 16),
+    # a piece of a prompt among single tokens: tile form
+    ([1] * 20 + [520] + [1] * 44, [300] * 10 + [0] * 10 + [20000] + [700] * 44, 28, 4, 128),
+]
+
+
+@pytest.mark.parametrize("lens,cached,Hq,Hkv,rows", RUNS)
+def test_segments_in_runs(dev, lens, cached, Hq, Hkv, rows):
+    b = Marked(dev, lens, cached, Hq, Hkv, 8, seed=61, share=True)
+    shape, p = b.shape(), b.plan
+    ws = _capi.chunk_workspace_size(p.n_seg, p.max_q, p.max_cached, Hq, Hkv, 128, p.total_rows, p.total_cached)
+    a_segment = Hkv * -(-p.max_q * Hq // Hkv // rows) * shape["n_split"]
+    assert shape["rows"] == rows and 0 < ws <= 1 << 30 and shape["n_split"] > 1
+    assert p.n_seg * a_segment > ws // (rows * 520) >= a_segment  # several runs, one segment or more each
+    b.anywhere(12)
+    b.hidden(4)
