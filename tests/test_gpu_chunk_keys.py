@@ -164,3 +164,54 @@ def test_segments_in_runs(dev, lens, cached, Hq, Hkv, rows):
     assert p.n_seg * a_segment > ws // (rows * 520) >= a_segment  # several runs, one segment or more each
     b.anywhere(12)
     b.hidden(4)
+
+
+# ---- every tile, page, part and round ---------------------------------------------------
+
+def _borders(n, L):
+    """First and last key of every run of 32 cached rows (tiles, pages, parts and rounds of
+    parts begin and end there) and of every 32 new rows."""
+    out = [x for i in range(0, n, 32) for x in (i, min(i + 31, n - 1))]
+    return out + [n + x for i in range(0, L, 32) for x in (i, min(i + 31, L - 1))]
+
+
+CASES = [
+    # lens, cached, Hq, Hkv, mask_block, shared pages, rows of a workgroup, parts
+    # parts of a row joined in three rounds, and the same of two rows of 16
+    ([1], [33000], 16, 1, 1, False, 16, range(100, 200)),
+    ([2], [33000], 16, 1, 1, False, 32, range(100, 200)),
+    ([1], [131071], 8, 1, 1, False, 16, range(200, 300)),
+    # parts as long as a workgroup's page ids reach (15872 rows): whole, one row more, three
+    ([1] * 16, [31744] * 16, 16, 16, 1, True, 16, [2]),
+    ([1] * 16, [31745] * 16, 16, 16, 1, True, 16, [3]),
+    ([20] * 16, [33000] * 16, 16, 16, 4, True, 32, [3]),
+    # one part, page ids fetched again every 64 pages
+    ([100] * 16, [17000] * 16, 32, 32, 1, True, 128, [1]),
+    ([70] * 16, [33100] * 16, 32, 32, 0, True, 128, [1]),
+    # parts of new and cached tiles, of cached pages that begin inside a part
+    ([66], [4200], 16, 1, 1, False, 128, range(10, 100)),
+    ([600, 530], [40000, 1000], 8, 2, 32, False, 128, range(2, 200)),
+    ([300], [2500], 8, 1, 0, False, 128, range(2, 100)),
+    # few keys, ragged, several M tiles, eight wavefronts and four
+    ([1], [900], 4, 4, 1, False, 16, range(2, 20)),
+    ([1], [511], 32, 32, 1, False, 16, [1]),
+    ([1, 3, 1], [1, 700, 4000], 14, 2, 1, False, 32, range(2, 100)),
+    ([1] * 32, [512 + 97 * i for i in range(32)], 28, 4, 1, False, 16, range(2, 20)),
+    ([32] * 4, [608, 1216, 90, 0], 4, 4, 0, False, 32, range(1, 20)),
+    ([32] * 16, [384 + 56 * i for i in range(16)], 28, 4, 0, False, 32, [1]),
+    ([9, 40], [255, 257], 14, 2, 4, False, 32, [1]),
+    ([260, 70], [511, 0], 4, 4, 33, False, 32, range(1, 20)),
+]
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("lens,cached,Hq,Hkv,mask_block,share,rows,parts", CASES)
+def test_every_key_counts_once(dev, lens, cached, Hq, Hkv, mask_block, share, rows, parts, bits):
+    b = Marked(dev, lens, cached, Hq, Hkv, bits, seed=62 + len(lens) + max(cached), share=share, mask_block=mask_block)
+    shape = b.shape()
+    assert shape["rows"] == rows and shape["n_split"] in parts, shape
+    longest = max(range(len(lens)), key=lambda i: cached[i])
+    b.all_of(_borders(cached[longest], lens[longest]))
+    b.anywhere(6)
+    if mask_block:
+        b.hidden(4)
