@@ -86,7 +86,8 @@ __device__ __forceinline__ int splits_of(const ChunkArgs& a, int max_split, int 
   const int32_t *__restrict__ cu, const int32_t *__restrict__ seg_ids, const int32_t *__restrict__ lens,       \
       const int32_t *__restrict__ table, int chunk_pages, int logical_blocks, int mtiles, int max_split,       \
       int tiles_per_split, int Hkv, ChunkArgs a
-// chunk_pages: the XCD interleave's chunk (1 .. 4) + 32 x the page table's row length.
+// chunk_pages: the XCD interleave's chunk (1 .. 4) + 16 x whether the splits turn (work_of) +
+// 32 x the page table's row length.
 
 // A workgroup's work: one M tile and split of one (segment, KV head), M tiles fastest.
 // Every segment has max_split splits; those past its end stop at once.
@@ -104,17 +105,33 @@ __device__ __forceinline__ int take(uint32_t& r, int n) {
   r = q;
   return (int)(x - q * (uint32_t)n);
 }
-__device__ __forceinline__ Work work_of(int L, int mtiles, int max_split, int Hkv) {
+// Workgroup L runs on XCD L % 8 and there on shader engine L / 8 % 4.  Of sequences with
+// very different lengths most have only their first splits: with max_split a multiple of
+// 32 those of all sequences would meet on one engine.  `turn`: split 0 of group (segment, KV
+// head) i stands i / P places later, modulo max_split, P groups being what it takes for
+// i * max_split to come back to the same engine.  (16 x 8 rows behind 100 - 8000, 28/4
+// heads, 16 parts: 52.9 -> 30.6 us; 8 tokens behind 64 - 4000, 32 heads, 4 parts 34.2 -> 23.7.  Where
+// all splits exist it is 1 - 3 % slower: one token behind 131071 27.2 and 27.7.)
+__device__ __forceinline__ Work work_of(int L, int mtiles, int max_split, int Hkv, bool turn) {
   Work w;
   uint32_t r = (uint32_t)L;
   w.mt = take(r, mtiles);
   w.split = take(r, max_split);
+  if (turn) {
+    uint32_t t = r >> (5 - min(5, __builtin_ctz((uint32_t)max_split)));
+    w.split -= take(t, max_split);
+    if (w.split < 0) w.split += max_split;
+  }
   w.hkv = take(r, Hkv);
   w.s = (int)r;
   return w;
 }
+// The place of a workgroup's part: M tiles fastest, then splits, KV heads, segments.
+__device__ __forceinline__ int part_of(const Work& w, int mtiles, int max_split, int Hkv) {
+  return ((w.s * Hkv + w.hkv) * max_split + w.split) * mtiles + w.mt;
+}
 __device__ __forceinline__ int block_of(int chunk_pages) {
-  const int chunk = chunk_pages & 31;
+  const int chunk = chunk_pages & 15;
   return chunk == 1 ? (int)blockIdx.x : xcd_remap(blockIdx.x, chunk);
 }
 // Token of M row m (m >= 0).
@@ -353,7 +370,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int L = block_of(chunk_pages);
   if (L >= logical_blocks) return;
   const int max_pages = chunk_pages >> 5;
-  const Work wk = work_of(L, mtiles, max_split, Hkv);
+  const Work wk = work_of(L, mtiles, max_split, Hkv, chunk_pages & 16);
   const int s = wk.s, hkv = wk.hkv, split = wk.split;
   const int lane = threadIdx.x & 63;
   const int t_begin = split * tiles_per_split;
@@ -711,6 +728,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   }
   const int tok = token_of(m, g), head = hkv * g + (m - tok * g);
   const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+  const int part = part_of(wk, mtiles, max_split, Hkv);
 #pragma unroll
   for (int j = 0; j < DPT / 4; ++j) {
     const int d = d0 + 4 * TPR * j;
@@ -726,11 +744,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       const u32x2_t w2 = {cvt_pk_bf16(acc[0] * inv, acc[1] * inv), cvt_pk_bf16(acc[2] * inv, acc[3] * inv)};
       *reinterpret_cast<u32x2_t*>(a.o + (int64_t)(sg.row0 + tok) * a.o_stride + head * HD + d) = w2;
     } else {
-      *reinterpret_cast<f32x4_t*>(part_o<BM>(a, L, row) + d) = acc;
+      *reinterpret_cast<f32x4_t*>(part_o<BM>(a, part, row) + d) = acc;
     }
   }
   if (ns > 1 && d0 == 0) {
-    float* const pml = part_ml<BM>(a, logical_blocks, L, row);
+    float* const pml = part_ml<BM>(a, logical_blocks, part, row);
     pml[0] = mx;
     pml[1] = lsum;
   }
@@ -765,7 +783,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int L = block_of(chunk_pages);
   if (L >= logical_blocks) return;
   const int max_pages = chunk_pages >> 5;
-  const Work wk = work_of(L, mtiles, max_split, Hkv);
+  const Work wk = work_of(L, mtiles, max_split, Hkv, false);
   const int s = wk.s, hkv = wk.hkv;
   const Segment sg = segment(a, cu, seg_ids, lens, s);
   const int g = a.g;
@@ -1155,6 +1173,7 @@ struct ChunkPlan {
   int nb;                        // chunk_rows_kernel: 16-row blocks
   int bm;                        // M rows of a workgroup
   int max_split, tiles_per_split;
+  bool turn;                     // rows form: the splits turn (work_of)
   int mtiles;                    // of the largest segment
   int run;                       // segments of a launch
   int64_t logical;               // its workgroups
@@ -1185,12 +1204,19 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
   // 32/32 heads, 256 workgroups: 20 us, split in two 30), and few keys are not split: the
   // joining takes 3 us, a turn of the wavefronts 0.8 (one token, 32 heads, whole / in parts:
   // behind 511 7.4 / 8.8, behind 767 8.4 / 9.3, behind 900 10.0 / 8.3).
-  // Sequences of one length: as many parts as give every CU one workgroup (one token behind
-  // 131071, 28/4 heads: 256 workgroups 29.6 us, 384 34, 512 31).  Of different lengths:
-  // 384 workgroups, half a part each lost to the last ones, of 12 tiles at least (32
-  // single tokens, 28/4 heads: at most 256 workgroups 24.7 us, 384 21.4; 40 of them 51.6 and 39.5,
-  // with 448 44.7; eight shorter ones 11.2, in parts of 8 tiles 12.9), with many sequences 256, so that
-  // one long one among them is still split.
+  // As many parts as give every CU one workgroup where the sequences fill 0.7 or more of
+  // the keys that they would all have at the longest one's length (one token behind 131071,
+  // 28/4 heads: 256 workgroups 29.6 us, 384 34, 512 31; tokens, 28/4 heads, these parts / those of
+  // the rule below: 16 behind 4000 18.2 / 20.3, behind 1600 - 4000 16.1 / 16.8, 12 behind 1200 -
+  // 3000 12.8 / 13.1, 4 behind 3200 - 8000 12.4 / 13.9).  Three parts where whole ones would leave a third
+  // of the CUs idle (5 tokens, 32 heads, bf16: behind 3565 54.1 whole, 53.1 in three, behind 1070 - 3565
+  // 50.3 and 43.7; with several M tiles, 11 x 16 rows behind 3909, 28/4 heads, 30.5 and 37.8).
+  // Where they fill 0.6 or less, parts of the longer ones even the card out: 384 workgroups, half
+  // a part each lost to the last ones, 256 with many sequences, of 12 tiles at least, and none
+  // of over half the longest (the same two: 32 tokens behind 512 - 4096 21.6 / 19.7, 32 behind 64 - 8192
+  // 33 / 22.4, 64 behind 100 - 8000 53 / 37, 8 behind 64 - 4000, 32 heads, 30 / 24, one behind 15000 among
+  // 256 behind 500 99 / 42; 8 behind 150 - 1500, 32 heads, whole 15.8, in two 18.3).  In between, the part
+  // length goes over from the one to the other.
   const int64_t groups = all_m * Hkv;  // (M tile, KV head) pairs, each with its own parts
   const double work = (double)groups * (double)all_t / (double)n_seg;
   int64_t tps;
@@ -1205,13 +1231,17 @@ static ChunkPlan chunk_plan(int64_t n_seg, int max_q, int max_cached, int64_t to
                                   work / (double)tps + 0.5 * (double)groups);
     const double whole = (groups <= 256 ? 1.7 : 2.4) * (double)tiles;
     if (tps * 2 > tiles || tiles <= 8 || whole < 2.4 * (double)tps + 3 + 0.027 * parts) tps = tiles;
-  } else if (total_cached == n_seg * max_cached) {
-    const int64_t parts = std::max<int64_t>(1, 256 / groups);
-    tps = std::max<int64_t>((tiles + parts - 1) / parts, 4);
   } else {
-    tps = std::max<int64_t>((int64_t)(work / std::max(384 - 0.5 * (double)groups, 256.) + 0.999), 12);
+    const double fill = tiles ? (double)all_t / ((double)n_seg * (double)tiles) : 1;
+    int64_t parts = std::max<int64_t>(1, 256 / groups);
+    if (parts == 1 && p.mtiles == 1 && groups * 3 <= 512 && tiles >= 96) parts = 3;
+    const double even = (double)std::max<int64_t>((tiles + parts - 1) / parts, 4);
+    const double uneven = std::max(work / std::max(384 - 0.5 * (double)groups, 256.), 12.);
+    const double to_even = std::min(std::max((fill - 0.6) * 10, 0.), 1.);
+    tps = (int64_t)(uneven + to_even * (even - uneven) + 0.999);
+    p.turn = to_even < 1;
+    if ((double)tps > (double)tiles * (3 + to_even) / 6 || tiles <= (groups > 128 ? 32 : 24)) tps = tiles;
   }
-  if (!p.tile_form && (tps * 3 > tiles * 2 || tiles <= 24)) tps = tiles;
   if (!p.tile_form) tps = std::min<int64_t>((tps + 3) / 4 * 4, kMaxSplitTiles);
   if (tps < 1) tps = 1;
   // Every segment of a launch has room for the parts that the one with the most rows and
@@ -1362,7 +1392,7 @@ extern "C" int dllm_attn_chunk_paged_fwd(const dllm_bf16* q, const dllm_bf16* k,
     const int segs = std::min(p.run, n_seg - s0);
     const int logical = (int)(p.logical / p.run * segs);
     const int grid = chunk_grid(logical, p.mtiles, &chunk);
-    const int chunk_pages = chunk + 32 * chunk_pages_row;
+    const int chunk_pages = chunk + (p.turn && p.max_split > 1 ? 16 : 0) + 32 * chunk_pages_row;
     auto start = [&](auto kern, dim3 blocks, int threads, int lds_bytes) {
       kern<<<blocks, dim3((unsigned)threads), lds_bytes, reinterpret_cast<hipStream_t>(stream)>>>(
           seg_ids ? cu : cu + s0, seg_ids ? seg_ids + s0 : nullptr, cached_len + s0,
