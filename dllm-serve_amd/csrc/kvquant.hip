@@ -44,83 +44,55 @@ __device__ __forceinline__ void st_row8(uint16_t* p, u32x4_t x) {
   }
 }
 
-// U rows of sixteen lanes in flight; a workgroup takes 16 U consecutive (token,
-// head) rows.
-template <bool VEC, int U>
+// Sixteen lanes a row; a workgroup takes 16 consecutive (token, head) rows.
+template <bool VEC>
 __global__ __launch_bounds__(256) void kv_quant_store(QUANT_PARAMS) {
   const int L = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
   const int lane16 = threadIdx.x & 15;
-  const int row0 = L * 16 * U + (threadIdx.x >> 4);
-  u32x4_t kx[U], vx[U];
-  int64_t slot[U];
-  int head[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int row = row0 + 16 * u;
-    slot[u] = -1;
-    head[u] = 0;
-    kx[u] = vx[u] = u32x4_t{0, 0, 0, 0};
-    if (row < rows) {
-      const int tok = (int)((uint32_t)row / (uint32_t)Hkv);
-      head[u] = row - tok * Hkv;
-      const int64_t e = (int64_t)head[u] * kQuantD + lane16 * 8;
-      slot[u] = slots[tok];
-      kx[u] = ld_row8<VEC>(k + (int64_t)tok * k_stride + e);
-      vx[u] = ld_row8<VEC>(v + (int64_t)tok * v_stride + e);
-    }
+  const int row = L * 16 + (threadIdx.x >> 4);
+  int64_t slot = -1;
+  int head = 0;
+  u32x4_t kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
+  if (row < rows) {
+    const int tok = (int)((uint32_t)row / (uint32_t)Hkv);
+    head = row - tok * Hkv;
+    const int64_t e = (int64_t)head * kQuantD + lane16 * 8;
+    slot = slots[tok];
+    kx = ld_row8<VEC>(k + (int64_t)tok * k_stride + e);
+    vx = ld_row8<VEC>(v + (int64_t)tok * v_stride + e);
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    uint32_t kb, vb;
-    const u32x2_t kc = quant_row16(kx[u], kb);
-    const u32x2_t vc = quant_row16(vx[u], vb);
-    if (slot[u] < 0 || slot[u] >= n_slots) continue;
-    const int64_t rec = record_off((uint32_t)slot[u], Hkv, head[u]);
-    const int r = (int)(slot[u] & (kPageRows - 1));
-    *reinterpret_cast<u32x2_t*>(kp + rec + r * kQuantD + lane16 * 8) = kc;
-    *reinterpret_cast<u32x2_t*>(vp + rec + r * kQuantD + lane16 * 8) = vc;
-    if (lane16 == 0) {
-      kp[rec + kScaleOff + r] = (uint8_t)kb;
-      vp[rec + kScaleOff + r] = (uint8_t)vb;
-    }
+  uint32_t kb, vb;
+  const u32x2_t kc = quant_row16(kx, kb);  // every lane is here
+  const u32x2_t vc = quant_row16(vx, vb);
+  if (slot < 0 || slot >= n_slots) return;
+  const int64_t rec = record_off((uint32_t)slot, Hkv, head);
+  const int r = (int)(slot & (kPageRows - 1));
+  *reinterpret_cast<u32x2_t*>(kp + rec + r * kQuantD + lane16 * 8) = kc;
+  *reinterpret_cast<u32x2_t*>(vp + rec + r * kQuantD + lane16 * 8) = vc;
+  if (lane16 == 0) {
+    kp[rec + kScaleOff + r] = (uint8_t)kb;
+    vp[rec + kScaleOff + r] = (uint8_t)vb;
   }
 }
 
-template <bool VEC, int U>
+template <bool VEC>
 __global__ __launch_bounds__(256) void kv_quant_load(QUANT_PARAMS) {
   const int L = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
   const int lane16 = threadIdx.x & 15;
-  const int row0 = L * 16 * U + (threadIdx.x >> 4);
-  u32x2_t kc[U], vc[U];
-  uint32_t kb[U], vb[U];
-  uint16_t *ko[U], *vo[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int row = row0 + 16 * u;
-    ko[u] = nullptr;
-    if (row < rows) {
-      const int tok = (int)((uint32_t)row / (uint32_t)Hkv);
-      const int head = row - tok * Hkv;
-      const int64_t slot = slots[tok];
-      if (slot >= 0 && slot < n_slots) {
-        const int64_t e = (int64_t)head * kQuantD + lane16 * 8;
-        const int64_t rec = record_off((uint32_t)slot, Hkv, head);
-        const int r = (int)(slot & (kPageRows - 1));
-        ko[u] = k + (int64_t)tok * k_stride + e;
-        vo[u] = v + (int64_t)tok * v_stride + e;
-        kc[u] = *reinterpret_cast<const u32x2_t*>(kp + rec + r * kQuantD + lane16 * 8);
-        vc[u] = *reinterpret_cast<const u32x2_t*>(vp + rec + r * kQuantD + lane16 * 8);
-        kb[u] = kp[rec + kScaleOff + r];
-        vb[u] = vp[rec + kScaleOff + r];
-      }
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (ko[u]) {
-      st_row8<VEC>(ko[u], dequant8(kc[u], scale_of(kb[u])));
-      st_row8<VEC>(vo[u], dequant8(vc[u], scale_of(vb[u])));
-    }
+  const int row = L * 16 + (threadIdx.x >> 4);
+  if (row >= rows) return;
+  const int tok = (int)((uint32_t)row / (uint32_t)Hkv);
+  const int head = row - tok * Hkv;
+  const int64_t slot = slots[tok];
+  if (slot < 0 || slot >= n_slots) return;
+  const int64_t e = (int64_t)head * kQuantD + lane16 * 8;
+  const int64_t rec = record_off((uint32_t)slot, Hkv, head);
+  const int r = (int)(slot & (kPageRows - 1));
+  const u32x2_t kc = *reinterpret_cast<const u32x2_t*>(kp + rec + r * kQuantD + lane16 * 8);
+  const u32x2_t vc = *reinterpret_cast<const u32x2_t*>(vp + rec + r * kQuantD + lane16 * 8);
+  const uint32_t kb = kp[rec + kScaleOff + r], vb = vp[rec + kScaleOff + r];
+  st_row8<VEC>(k + (int64_t)tok * k_stride + e, dequant8(kc, scale_of(kb)));
+  st_row8<VEC>(v + (int64_t)tok * v_stride + e, dequant8(vc, scale_of(vb)));
 }
 
 template <bool STORE>
@@ -141,12 +113,11 @@ static int kv_quant(const char* name, uint16_t* k, int64_t ks, uint16_t* v, int6
     return fail(DLLM_ERR_UNSUPPORTED, "%s: %d tokens of %d KV heads in one call", name, n_tok, Hkv);
   const bool vec = ks % 8 == 0 && vs % 8 == 0 && aligned16(k) && aligned16(v);
   const int rows = n_tok * Hkv;
-  const int U = 1;
-  const int64_t blocks = ((int64_t)rows + 16 * U - 1) / (16 * U);
+  const int64_t blocks = ((int64_t)rows + 15) / 16;
   // consecutive workgroups on one XCD: the scale bytes of a page's rows share lines
   const int chunk = (int)((blocks + 7) / 8);
-  auto kern = STORE ? (vec ? kv_quant_store<true, U> : kv_quant_store<false, U>)
-                    : (vec ? kv_quant_load<true, U> : kv_quant_load<false, U>);
+  auto kern = STORE ? (vec ? kv_quant_store<true> : kv_quant_store<false>)
+                    : (vec ? kv_quant_load<true> : kv_quant_load<false>);
   kern<<<dim3((unsigned)chunk * 8), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       slot, k, v, rows, Hkv, chunk, ks, vs, kp, vp, num_pages * kPageRows);
   return check_launch(name);

@@ -616,10 +616,6 @@ __device__ __forceinline__ uint16_t raw_bits(const SelArgs& a, const Job& jb, in
   return (uint16_t)f64_to_bf16_bits_2step(t);
 }
 
-// The copy of the selected rows of ranks [r0, r1) -- their KV-head-h pieces
-// -- into their cache slots by the whole workgroup: item i = (rank r0 + i / 16,
-// 16-byte chunk i % 16), eight items per thread in flight.  cand(r) gives the
-// candidate of rank r.
 // One 16-byte piece (chunk chk of KV head h's 128 values) of a row of K and V to 8-bit
 // pages; the sixteen lanes of a row share its slot.  Every lane of the wavefront is
 // active; a slot outside the cache stores nothing.
@@ -638,6 +634,10 @@ __device__ __forceinline__ void store_quant(const SelArgs& a, int h, int chk, in
   }
 }
 
+// The copy of the selected rows of ranks [r0, r1) -- their KV-head-h pieces
+// -- into their cache slots by the whole workgroup: item i = (rank r0 + i / 16,
+// 16-byte chunk i % 16), eight items per thread in flight.  cand(r) gives the
+// candidate of rank r.
 template <bool QUANT, typename CandFn>
 __device__ __forceinline__ void copy_selected(const SelArgs& a, const Job& jb, int h, int r0, int r1, CandFn cand) {
   const int64_t row_elems = (int64_t)a.Hkv * SHD;
