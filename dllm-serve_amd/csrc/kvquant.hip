@@ -109,7 +109,8 @@ static int kv_quant(const char* name, uint16_t* k, int64_t ks, uint16_t* v, int6
     return fail(DLLM_ERR_INVALID_ARG, "%s: token stride (%lld, %lld) smaller than a token row of %lld", name,
                 (long long)ks, (long long)vs, (long long)Hkv * D);
   if (!aligned16(kp) || !aligned16(vp)) return fail(DLLM_ERR_INVALID_ARG, "%s: pages must be 16-byte aligned", name);
-  if ((int64_t)n_tok * Hkv > ((int64_t)1 << 30))
+  // sixteen threads a row, and HIP launches fewer than 2^32
+  if ((int64_t)n_tok * Hkv >= ((int64_t)1 << 28) - 128)
     return fail(DLLM_ERR_UNSUPPORTED, "%s: %d tokens of %d KV heads in one call", name, n_tok, Hkv);
   const bool vec = ks % 8 == 0 && vs % 8 == 0 && aligned16(k) && aligned16(v);
   const int rows = n_tok * Hkv;

@@ -212,7 +212,7 @@ int dllm_attn_block_cached_fwd_noalloc(const dllm_bf16* q, const dllm_bf16* k, c
  * dllm_load_kvcache from them: key / value are [n_tok][Hkv][D] with the given token
  * strides; a slot outside the cache is skipped, or leaves its row untouched.  The
  * slots of one store must differ: a row written twice by one call holds parts of
- * both.
+ * both.  One call takes fewer than 2^28 - 128 rows (n_tok * Hkv).
  */
 size_t dllm_quant_page_bytes(int D);
 int dllm_store_kvcache_fp8(const dllm_bf16* key, int64_t key_stride_tok, const dllm_bf16* value,
