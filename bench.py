@@ -1108,22 +1108,26 @@ def profile_denoise_run(dev):
 
 
 TRAFFIC_SUMMARY = os.path.join(ROOT, "profiles", "attn_dense_kernel_llada_c2_8x384_counters.md")
-KERNEL_SOURCE = os.path.join(ROOT, "dllm-serve_amd", "csrc", "attn.hip")
+# what the headline kernel is compiled from, in this order
+KERNEL_SOURCES = [os.path.join(ROOT, "dllm-serve_amd", "csrc", n) for n in ("attn.hip", "attn_tile.h", "common.h")]
 
 
 def kernel_source_sha256() -> str:
-    """First 16 hex digits of the SHA-256 of the attention kernels' source file."""
+    """First 16 hex digits of the SHA-256 of the attention kernels' source files, one after the other."""
     import hashlib
-    with open(KERNEL_SOURCE, "rb") as f:
-        return hashlib.sha256(f.read()).hexdigest()[:16]
+    h = hashlib.sha256()
+    for path in KERNEL_SOURCES:
+        with open(path, "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()[:16]
 
 
 def measured_traffic(kernel: str):
     """HBM bytes per launch of `kernel` from the committed rocprofv3 FETCH_SIZE /
     WRITE_SIZE summary (counters scaled by a plain 256 MiB copy), and where that
     figure was recorded: the summary's `recorded_on:` line names the commit and
-    the SHA-256 of `attn.hip` of the build the counters ran on, which is compared
-    with the source this run loads.  Returns (bytes or None, provenance dict)."""
+    the SHA-256 of the sources of the build the counters ran on, which is compared
+    with those of this run.  Returns (bytes or None, provenance dict)."""
     prov = {"summary": os.path.relpath(TRAFFIC_SUMMARY, ROOT), "commit": None,
             "kernel_source_sha256": None, "current_kernel_source_sha256": kernel_source_sha256()}
     try:
@@ -1142,7 +1146,7 @@ def measured_traffic(kernel: str):
                 key, _, val = part.strip().partition(" ")
                 if key == "commit":
                     prov["commit"] = val.strip()
-                elif key == "attn.hip_sha256":
+                elif key == "source_sha256":
                     prov["kernel_source_sha256"] = val.strip()
     prov["source_matches"] = prov["kernel_source_sha256"] == prov["current_kernel_source_sha256"]
     return traffic, prov
