@@ -151,7 +151,9 @@ class ChunkPlan:
     256-row cache pages ``block_tables[b]`` (host integers; more pages than
     needed are fine).  ``mask_block`` 0: the new rows see each other; b >= 1:
     a row sees the rows up to the end of its own block of b positions
-    (1: causal), positions counted from the first cached row.  The tables are
+    (1: causal), positions counted from the first cached row: behind a cache that
+    holds a selection of the rows, n cached rows do not end at position n, and
+    only 0 and 1 mean what they say.  The tables are
     uploaded with one asynchronous copy on the stream that is current; nothing
     synchronises the host.  The first call on any other stream makes that stream
     wait for the upload, and a plan may be dropped while calls are in flight.  A plan
@@ -399,7 +401,9 @@ class StepPlan:
     ``StepPlan(context, device, ...)`` builds them from host integers of
     ``context.seqs`` and uploads them with one asynchronous copy (not inside
     a capture: a forward of the same Context has to come before it);
-    ``StepPlan.from_device`` wraps tables the device-side builder wrote."""
+    ``StepPlan.from_device`` wraps tables the device-side builder wrote.
+    Its layers and the graphs captured from it share its workspaces: they run
+    one after another."""
 
     _SCALARS = ("n_seq", "total_rows", "any_skipped", "n_dense", "max_q_dense", "n_job", "max_kc", "max_keep",
                 "max_blk", "n_cached", "max_q_cached", "max_keys_cached", "max_keep_cached", "rows_cached",

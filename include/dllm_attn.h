@@ -229,8 +229,10 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * (cache_type: DLLM_CACHE_FP8 as above, or DLLM_CACHE_BF16, [rows][Hkv][D] as
  * dllm_store_kvcache writes it), and masks among the new tokens.
  *
- * Segment s (id = seg_ids ? seg_ids[s] : s) has new rows [cu[id], cu[id+1]) of q, k, v
- * (L of them) and n cached rows.  Its new row t stands at position n + t and sees
+ * Segment s (id = seg_ids ? seg_ids[s] : s; no id twice) has new rows [cu[id],
+ * cu[id+1]) of q, k, v (L of them) and n cached rows.  Its new row t stands at position n +
+ * t (where the cache holds a selection of a sequence's rows that is not its place in
+ * the sequence, and blocks of more than one position do not begin where they should) and sees
  * every cached row and the new rows j < vis(t):
  *   mask_block = 0      vis(t) = L                               (bidirectional)
  *   mask_block = b > 0  vis(t) = min(L, ((n + t) / b + 1) * b - n)  (causal between
