@@ -82,14 +82,29 @@ struct PlanArgs {
   int64_t n_dense, max_q_dense, cu, dense_ids;
   int64_t n_cached, max_q_cached, max_keys_cached, cached_ids, slots, slot_off, ws, ws_bytes;
 };
+// Behind it where the cached rows are in 8-bit pages.
+struct PageArgs {
+  int64_t max_keep, rows, keeps, table, max_pages, lens;
+};
+
+// An 8-bit cache (uint8 [pages, heads, bytes of a page]), or null.
+const at::Tensor* pages_of(PyObject* o, int64_t heads, int device) {
+  const at::Tensor* t = plain(o, at::kByte);
+  if (!t || t->get_device() != device || t->dim() != 3 || t->size(1) != heads ||
+      t->size(2) != (int64_t)dllm_quant_page_bytes(128) || !t->is_contiguous())
+    return nullptr;
+  return t;
+}
 
 PyObject* attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7 || !PyBytes_CheckExact(a[5]) || PyBytes_GET_SIZE(a[5]) != (Py_ssize_t)sizeof(PlanArgs) ||
-      !PyFloat_CheckExact(a[6]))
-    Py_RETURN_NONE;
+  if (n != 7 || !PyBytes_CheckExact(a[5]) || !PyFloat_CheckExact(a[6])) Py_RETURN_NONE;
+  const bool paged = PyBytes_GET_SIZE(a[5]) == (Py_ssize_t)(sizeof(PlanArgs) + sizeof(PageArgs));
+  if (!paged && PyBytes_GET_SIZE(a[5]) != (Py_ssize_t)sizeof(PlanArgs)) Py_RETURN_NONE;
   return guarded([&]() -> PyObject* {
     PlanArgs p;
+    PageArgs pg = {};
     std::memcpy(&p, PyBytes_AS_STRING(a[5]), sizeof(p));
+    if (paged) std::memcpy(&pg, PyBytes_AS_STRING(a[5]) + sizeof(p), sizeof(pg));
     const at::Tensor *q = plain(a[0], at::kBFloat16), *k = plain(a[1], at::kBFloat16), *v = plain(a[2], at::kBFloat16);
     if (!q || !k || !v || q->get_device() != p.device || k->get_device() != p.device || v->get_device() != p.device ||
         !token_rows(*q, p.Hq, p.D) || !token_rows(*k, p.Hkv, p.D) || !token_rows(*v, p.Hkv, p.D) ||
@@ -97,7 +112,12 @@ PyObject* attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Py_RETURN_NONE;
     const at::Tensor *kc = nullptr, *vc = nullptr;
     int64_t cache_slots = 0;
-    if (p.n_cached) {
+    if (paged) {
+      kc = pages_of(a[3], p.Hkv, (int)p.device);
+      vc = pages_of(a[4], p.Hkv, (int)p.device);
+      if (!kc || !vc || kc->numel() == 0 || vc->numel() == 0 || p.D != 128) Py_RETURN_NONE;
+      if (std::min(kc->size(0), vc->size(0)) > INT32_MAX) Py_RETURN_NONE;
+    } else if (p.n_cached) {
       kc = plain(a[3], at::kBFloat16);
       vc = plain(a[4], at::kBFloat16);
       for (const at::Tensor* t : {kc, vc})
@@ -118,7 +138,16 @@ PyObject* attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                  dev_i32(p.cu), dev_i32(p.cu), dev_i32(p.dense_ids), (int)p.n_dense,
                                  (int)p.max_q_dense, (int)p.max_q_dense, (int)p.Hq, (int)p.Hkv, (int)p.D, q->stride(0),
                                  k->stride(0), v->stride(0), o.stride(0), scale, st);
-      if (r == DLLM_OK && p.n_cached) {
+      if (r == DLLM_OK && paged) {
+        what = "dllm_attn_chunk_paged_fwd";
+        r = dllm_attn_chunk_paged_fwd(ptr<dllm_bf16>(*q), ptr<dllm_bf16>(*k), ptr<dllm_bf16>(*v), ptr<dllm_bf16>(o),
+                                      dev_i32(p.cu), dev_i32(p.cached_ids), (int)p.n_cached, (int)p.max_q_cached,
+                                      (int)pg.max_keep, pg.rows, pg.keeps, kc->data_ptr(), vc->data_ptr(), DLLM_CACHE_FP8,
+                                      (int)std::min(kc->size(0), vc->size(0)), dev_i32(pg.table), (int)pg.max_pages,
+                                      dev_i32(pg.lens), 0, (int)p.Hq, (int)p.Hkv, (int)p.D, q->stride(0), k->stride(0),
+                                      v->stride(0), o.stride(0), scale, reinterpret_cast<void*>(p.ws), (size_t)p.ws_bytes,
+                                      st);
+      } else if (r == DLLM_OK && p.n_cached) {
         what = "dllm_attn_block_cached_fwd";
         r = dllm_attn_block_cached_fwd(ptr<dllm_bf16>(*q), ptr<dllm_bf16>(*k), ptr<dllm_bf16>(*v), ptr<dllm_bf16>(o),
                                        dev_i32(p.cu), dev_i32(p.cached_ids), (int)p.n_cached, (int)p.max_q_cached,
@@ -132,15 +161,6 @@ PyObject* attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (rc != DLLM_OK) return refused(what, rc);
     return THPVariable_Wrap(o.dim() == 2 ? std::move(o) : o.view({-1, p.Hq * p.D}));
   });
-}
-
-// An 8-bit cache (uint8 [pages, heads, bytes of a page]), or null.
-const at::Tensor* pages_of(PyObject* o, int64_t heads, int device) {
-  const at::Tensor* t = plain(o, at::kByte);
-  if (!t || t->get_device() != device || t->dim() != 3 || t->size(1) != heads ||
-      t->size(2) != (int64_t)dllm_quant_page_bytes(128) || !t->is_contiguous())
-    return nullptr;
-  return t;
 }
 
 // quant_copy(key, value, k_cache, v_cache, slot_mapping, store) -> True or None

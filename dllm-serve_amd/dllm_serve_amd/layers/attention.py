@@ -574,14 +574,19 @@ class StepPlan:
                      cached_ids=None if self.cached_identity else self.cached_ids.data_ptr(),
                      ws=None if ws is None else ws.data_ptr(), ws_bytes=0 if ws is None else ws.numel(),
                      ws_tensor=ws)
-            self._args[key] = a
-            if not (pages or self.any_skipped or self.n_job) and self.device.type == "cuda":
-                # the step's launches for the native form (csrc/native.cpp, PlanArgs)
+            if not (self.any_skipped or self.n_job) and self.device.type == "cuda":
+                # the step's launches for the native form (csrc/native.cpp, PlanArgs and PageArgs)
                 dev = self.device.index if self.device.index is not None else torch.cuda.current_device()
-                self._packed[key] = struct.pack(
+                packed = struct.pack(
                     "=17q", dev, self.total_rows, Hq, Hkv, D, self.n_dense, self.max_q_dense, a["cu"],
                     a["dense_ids"] or 0, self.n_cached, self.max_q_cached, self.max_keys_cached, a["cached_ids"] or 0,
                     a["slots"], a["slot_off"], a["ws"] or 0, a["ws_bytes"])
+                if pages:
+                    table, lens = self.page_tables()
+                    packed += struct.pack("=6q", self.max_keep_cached, self.rows_cached, self.keeps_cached,
+                                          table.data_ptr(), table.shape[1], lens.data_ptr())
+                self._packed[key] = packed
+            self._args[key] = a
         return a
 
 
@@ -624,7 +629,8 @@ class Attention(nn.Module):
 
     def _native_attention(self, plan, q, k, v):
         """The step's attention through the native form, or None (see csrc/native.cpp)."""
-        packed = plan._packed.get((self.num_heads, self.num_kv_heads, self.head_dim))
+        key = (self.num_heads, self.num_kv_heads, self.head_dim)
+        packed = plan._packed.get(key) or plan._packed.get(key + ("pages",))
         if packed is None or _capi.native is None:
             return None
         return _capi.native.attn(q, k, v, self.k_cache, self.v_cache, packed, float(self.scale))
@@ -678,8 +684,9 @@ class Attention(nn.Module):
         plan = self._plan(context, dev)
         if nq != plan.total_rows or nk != plan.total_rows or nv != plan.total_rows:
             raise ValueError(f"q/k/v have {nq}/{nk}/{nv} rows, the step's sequences feed {plan.total_rows}")
-        first = (Hq, Hkv, D) not in plan._args
+        known = len(plan._args)
         args = plan.launch_args(Hq, Hkv, D, bool(plan.n_cached) and self.k_cache.dtype == torch.uint8)
+        first = len(plan._args) > known
         if first:  # the step's first layer of this shape: its launch arguments exist only now
             o = self._native_attention(plan, q, k, v)
             if o is not None:

@@ -3,6 +3,7 @@ the upload would be replayed from pinned memory that has been given to something
 import pytest
 import torch
 
+from dllm_serve_amd import _capi
 from dllm_serve_amd.engine.kv_cache import quantized_pages
 from dllm_serve_amd.engine.sequence import PageAllocator, Sequence, prepare_step
 from dllm_serve_amd.layers.attention import Attention
@@ -128,4 +129,50 @@ def test_a_step_over_pages_takes_one_workspace(dev):
     layer.k_cache = torch.zeros(8, 2, 100, dtype=torch.uint8, device=dev)
     with pytest.raises(ValueError, match="k_cache"):
         layer(*x)
+    reset_context()
+
+
+@pytest.mark.parametrize("with_dense", [False, True])
+def test_state_2_over_pages_is_one_native_call(dev, with_dense, monkeypatch):
+    """The same bits as the Python form; other layouts and caches are left to it."""
+    seqs, x = _step_of_reuse(dev)
+    if with_dense:  # a sequence without a cache in the same step
+        seqs.insert(1, Sequence([3] * 90, 38, 126336, None, device=dev))
+        g = torch.Generator().manual_seed(52)
+        x = [torch.randn(192, h * 128, generator=g).to(BF16).to(dev) for h in (8, 2, 2)]
+    layer = _layer(dev, True)
+    for t in (layer.k_cache, layer.v_cache):
+        t.copy_(torch.randint(0, 120, t.shape, dtype=torch.uint8, device=dev))
+    prepare_step(seqs, dev)
+    with monkeypatch.context() as m:
+        m.setattr(_capi, "native", None)
+        want = layer(*x)
+    reset_context()
+    prepare_step(seqs, dev)
+    assert torch.equal(layer(*x), want)       # builds the plan
+    plan = get_context()._dllm_plan
+    with monkeypatch.context() as m:
+        def python_form(*a):
+            raise AssertionError("the Python form ran")
+        m.setattr(Attention, "_mixed_sparse_dense_attention", python_form)
+        assert torch.equal(layer(*x), want)
+        three = [t.view(t.shape[0], -1, 128) for t in x]
+        assert torch.equal(layer(*three), want)
+        # in a graph too
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(*x)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    packed = plan._packed[(8, 2, 128, "pages")]
+    call = lambda kc, vc: _capi.native.attn(*x, kc, vc, packed, float(layer.scale))  # noqa: E731
+    assert torch.equal(call(layer.k_cache, layer.v_cache), want)
+    bf16 = torch.zeros(8, 256, 2, 128, dtype=BF16, device=dev)
+    for kc, vc in ((bf16, bf16), (layer.k_cache, bf16), (layer.k_cache[:, :1], layer.v_cache), (layer.k_cache, None),
+                   (layer.k_cache[:0], layer.v_cache[:0]), (layer.k_cache.cpu(), layer.v_cache.cpu())):
+        assert call(kc, vc) is None
     reset_context()
