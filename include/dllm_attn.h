@@ -255,9 +255,9 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * 16-byte aligned, token strides multiples of 8 elements, and a segment's new rows span
  * at most 4 GiB of q, k or v.  workspace: dllm_attn_chunk_workspace_size(...) bytes
  * (0 where one workgroup takes all keys of a row), any contents; calls that may
- * overlap need workspaces of their own.  It is 1 GiB at most, or what one segment
- * with a KV head's rows in parts of 15872 keys takes where that is more: a call whose
- * segments would need more launches them in several runs.
+ * overlap need workspaces of their own.  It is 1 GiB at most, or what one segment's rows
+ * in parts of 15872 keys take where that is more: a call whose segments would need
+ * more launches them in several runs.
  */
 #define DLLM_CACHE_BF16 0
 #define DLLM_CACHE_FP8 1
