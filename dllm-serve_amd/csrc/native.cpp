@@ -192,13 +192,21 @@ PyObject* quant_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // chunk(q, k, v, k_cache, v_cache, plan: bytes, scale) -> output or None.
-// `plan` is this description and then the streams that are behind the tables' upload:
-// on any other the Python form runs, which makes it wait.
+// `plan` is this description, n_groups launches and then the streams that are behind the
+// tables' upload: on any other the Python form runs, which makes it wait.
 struct ChunkTables {
-  int64_t device, rows, n_seg, max_q, max_cached, total_cached, max_pages, max_page, mask_block, cu, lens, tables, seg_ids;
+  int64_t device, rows, n_groups, max_pages, max_page, mask_block, cu, lens, tables, seg_ids;
 };
-bool behind_upload(PyObject* plan, void* stream) {
-  const char* at = PyBytes_AS_STRING(plan) + sizeof(ChunkTables);
+struct ChunkGroup {
+  int64_t first, n_seg, max_q, max_cached, total_q, total_cached;
+};
+ChunkGroup chunk_group(PyObject* plan, int64_t i) {
+  ChunkGroup g;
+  std::memcpy(&g, PyBytes_AS_STRING(plan) + sizeof(ChunkTables) + i * sizeof(g), sizeof(g));
+  return g;
+}
+bool behind_upload(PyObject* plan, int64_t n_groups, void* stream) {
+  const char* at = PyBytes_AS_STRING(plan) + sizeof(ChunkTables) + n_groups * sizeof(ChunkGroup);
   const char* const end = PyBytes_AS_STRING(plan) + PyBytes_GET_SIZE(plan);
   for (int64_t s; at < end; at += sizeof(s)) {
     std::memcpy(&s, at, sizeof(s));
@@ -225,7 +233,8 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t Hq = heads[0], Hkv = heads[1];
     if (heads[2] != Hkv || Hq % Hkv || p.rows == 0 || c10::hip::current_device() != p.device) Py_RETURN_NONE;
     void* const st = stream_of((int)p.device);
-    if (!behind_upload(a[5], st)) Py_RETURN_NONE;
+    const int64_t room = (PyBytes_GET_SIZE(a[5]) - (int64_t)sizeof(p)) / (int64_t)sizeof(ChunkGroup);
+    if (p.n_groups < 0 || p.n_groups > room || !behind_upload(a[5], p.n_groups, st)) Py_RETURN_NONE;
     const at::Tensor *kc = pages_of(a[3], Hkv, (int)p.device), *vc = pages_of(a[4], Hkv, (int)p.device);
     const int kind = kc ? DLLM_CACHE_FP8 : DLLM_CACHE_BF16;
     if (!kc) {
@@ -240,19 +249,29 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t pages = std::min(kc->size(0), vc->size(0));
     if (p.max_page >= pages || pages > INT32_MAX) Py_RETURN_NONE;
     at::Tensor o = at::empty({p.rows, Hq * 128}, t[0]->options());
-    const size_t nb = dllm_attn_chunk_workspace_size((int)p.n_seg, (int)p.max_q, (int)p.max_cached, p.rows,
-                                                     p.total_cached, (int)Hq, (int)Hkv, 128);
+    size_t nb = 0;  // the launches follow one another, so they share it
+    for (int64_t i = 0; i < p.n_groups; ++i) {
+      const ChunkGroup g = chunk_group(a[5], i);
+      nb = std::max(nb, dllm_attn_chunk_workspace_size((int)g.n_seg, (int)g.max_q, (int)g.max_cached, g.total_q,
+                                                       g.total_cached, (int)Hq, (int)Hkv, 128));
+    }
     at::Tensor ws;
     if (nb) ws = at::empty({(int64_t)nb}, t[0]->options().dtype(at::kByte));
     const float scale = (float)PyFloat_AS_DOUBLE(a[6]);
     auto dev_i32 = [](int64_t x) { return reinterpret_cast<const int32_t*>(x); };
     const int rc = no_gil([&] {
-      return dllm_attn_chunk_paged_fwd(ptr<dllm_bf16>(*t[0]), ptr<dllm_bf16>(*t[1]), ptr<dllm_bf16>(*t[2]),
-                                       ptr<dllm_bf16>(o), dev_i32(p.cu), dev_i32(p.seg_ids), (int)p.n_seg, (int)p.max_q,
-                                       (int)p.max_cached, p.rows, p.total_cached, kc->data_ptr(), vc->data_ptr(), kind,
-                                       (int)pages, dev_i32(p.tables), (int)p.max_pages, dev_i32(p.lens),
-                                       (int)p.mask_block, (int)Hq, (int)Hkv, 128, t[0]->stride(0), t[1]->stride(0),
-                                       t[2]->stride(0), o.stride(0), scale, nb ? ws.data_ptr() : nullptr, nb, st);
+      int r = DLLM_OK;
+      for (int64_t i = 0; i < p.n_groups && r == DLLM_OK; ++i) {
+        const ChunkGroup g = chunk_group(a[5], i);
+        r = dllm_attn_chunk_paged_fwd(
+            ptr<dllm_bf16>(*t[0]), ptr<dllm_bf16>(*t[1]), ptr<dllm_bf16>(*t[2]), ptr<dllm_bf16>(o),
+            dev_i32(p.cu) + (p.seg_ids ? 0 : g.first), p.seg_ids ? dev_i32(p.seg_ids) + g.first : nullptr, (int)g.n_seg,
+            (int)g.max_q, (int)g.max_cached, g.total_q, g.total_cached, kc->data_ptr(), vc->data_ptr(), kind, (int)pages,
+            dev_i32(p.tables) + g.first * p.max_pages, (int)p.max_pages, dev_i32(p.lens) + g.first, (int)p.mask_block,
+            (int)Hq, (int)Hkv, 128, t[0]->stride(0), t[1]->stride(0), t[2]->stride(0), o.stride(0), scale,
+            nb ? ws.data_ptr() : nullptr, nb, st);
+      }
+      return r;
     });
     if (rc != DLLM_OK) return refused("dllm_attn_chunk_paged_fwd", rc);
     return THPVariable_Wrap(std::move(o));

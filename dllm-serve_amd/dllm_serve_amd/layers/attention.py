@@ -161,9 +161,12 @@ class ChunkPlan:
     (torch.cuda.graph synchronises) and to live as long as the graph, which holds its
     addresses.
 
-    ``cached_lens`` and ``block_tables`` are in the order of the launch, which is
+    ``cached_lens`` and ``block_tables`` are in the order of the launches, which is
     the sequences' own unless they feed _SORT_ROWS rows together: then those with
-    the most keys come first, so that no long workgroup starts when the others end."""
+    the most keys come first, so that no long workgroup starts when the others end.
+
+    A launch takes the form, grid and workspace of its longest new rows, so short
+    sequences among long ones go into one of their own (``groups``)."""
 
     # The order costs a dependent load at the start of every workgroup, which only
     # pieces of prompts are long enough not to feel.
@@ -190,9 +193,14 @@ class ChunkPlan:
         self.max_pages = W = max(need, default=0)
         self.max_page = max((p for t, n in zip(tables, need) for p in t[:n]), default=-1)
         self.mask_block = int(mask_block)
-        order = list(range(B))
-        if self.total_rows >= self._SORT_ROWS:
-            order.sort(key=lambda b: -(seqlens[b] + cached[b]))  # stable
+        order, self.groups = [], []
+        for members in self._cut(seqlens, cached):
+            if self.total_rows >= self._SORT_ROWS:
+                members.sort(key=lambda b: -(seqlens[b] + cached[b]))  # stable
+            # first sequence in the order, sequences, longest new rows and cache, sums of both
+            q, c = [seqlens[b] for b in members], [cached[b] for b in members]
+            self.groups.append((len(order), len(members), max(q), max(c), sum(q), sum(c)))
+            order += members
         flat = np.full(3 * B + 1 + B * W, -1, dtype=np.int64)
         flat[0] = 0
         flat[1:B + 1] = np.cumsum(seqlens)
@@ -217,14 +225,37 @@ class ChunkPlan:
         self._args = (self.cu.data_ptr(), self.cached_lens.data_ptr(), self.block_tables.data_ptr())
         self._packed = self._pack()
 
+    @staticmethod
+    def _cut(seqlens, cached) -> list:
+        """The sequences (indices, in order) of every launch.
+
+        Those with under a sixteenth of the longest one's new rows are launched apart where
+        there are two or more and they would waste enough: their number times the rows
+        of the longest times the keys that there may be, 2^20 or more.  One launch / two, in us,
+        28/4 heads, beside single tokens behind 2000: 2048 rows behind 6000 and 31 of them 1470 / 260,
+        2 301 / 251, 512 behind 3000 and 16 189 / 59, 256 behind 500 and 2 62 / 31, 64 behind 1000 and 8 26 / 25,
+        but 4 20 / 23; 256 rows and two tokens, all behind 100, 18 / 24."""
+        out, rest = [], list(range(len(seqlens)))
+        while rest:
+            most = max(seqlens[b] for b in rest)
+            short = [b for b in rest if seqlens[b] * 16 < most]
+            n = sum(seqlens[b] > 0 for b in short)
+            if n < 2 or n * most * (most + max(cached[b] for b in rest)) < 1 << 20:
+                short = []
+            apart = set(short)
+            out.append([b for b in rest if b not in apart])
+            rest = short
+        return out
+
     _STREAMS = 16  # streams remembered; one that was forgotten waits once more
 
     def _pack(self) -> bytes:
-        """The plan for the native form (csrc/native.cpp, ChunkTables), the streams behind it."""
+        """The plan for the native form (csrc/native.cpp, ChunkTables), its launches, the streams behind it."""
+        groups = [x for g in self.groups for x in g]
         return struct.pack(
-            f"={13 + len(self._streams)}q", -1 if self.device.index is None else self.device.index, self.total_rows,
-            self.n_seg, self.max_q, self.max_cached, self.total_cached, self.max_pages, self.max_page,
-            self.mask_block, *self._args, self._seg_ids or 0, *self._streams)
+            f"={10 + len(groups) + len(self._streams)}q", -1 if self.device.index is None else self.device.index,
+            self.total_rows, len(self.groups), self.max_pages, self.max_page, self.mask_block, *self._args,
+            self._seg_ids or 0, *groups, *self._streams)
 
     def _join(self) -> None:
         """Puts the device's current stream behind the upload, and the tables' memory
@@ -289,18 +320,18 @@ def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
     with _on_device(dev):
         plan._join()
         o = torch.empty(nq, Hq * D, dtype=torch.bfloat16, device=dev)
-        need = _capi.chunk_workspace_size(plan.n_seg, plan.max_q, plan.max_cached, Hq, Hkv, D, plan.total_rows,
-                                          plan.total_cached)
+        need = max((_capi.chunk_workspace_size(n, mq, mc, Hq, Hkv, D, tq, tc) for _, n, mq, mc, tq, tc in plan.groups),
+                   default=0)
         # from the allocator at every call: a plan may be used on several streams and in several graphs
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        if nq:
-            cu, lens, tables = plan._args
+        cu, lens, tables = plan._args
+        for first, n, mq, mc, tq, tc in plan.groups if nq else ():
             _capi.attn_chunk_paged_fwd_raw(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu, plan._seg_ids, plan.n_seg,
-                plan.max_q, plan.max_cached, plan.total_rows, plan.total_cached, k_cache.data_ptr(),
-                v_cache.data_ptr(), kind, pages, tables, plan.max_pages, lens, plan.mask_block, Hq, Hkv, D, q_st, k_st,
-                v_st, o.stride(0), float(softmax_scale), None if ws is None else ws.data_ptr(), need,
-                _capi._stream(dev))
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu if plan._seg_ids else cu + 4 * first,
+                plan._seg_ids + 4 * first if plan._seg_ids else None, n, mq, mc, tq, tc, k_cache.data_ptr(),
+                v_cache.data_ptr(), kind, pages, tables + 4 * first * plan.max_pages, plan.max_pages, lens + 4 * first,
+                plan.mask_block, Hq, Hkv, D, q_st, k_st, v_st, o.stride(0), float(softmax_scale),
+                None if ws is None else ws.data_ptr(), need, _capi._stream(dev))
     return o
 
 

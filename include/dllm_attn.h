@@ -257,7 +257,8 @@ int dllm_load_kvcache_fp8(dllm_bf16* key, int64_t key_stride_tok, dllm_bf16* val
  * (0 where one workgroup takes all keys of a row), any contents; calls that may
  * overlap need workspaces of their own.  It is 1 GiB at most, or what one segment's rows
  * in parts of 15872 keys take where that is more: a call whose segments would need
- * more launches them in several runs.
+ * more launches them in several runs.  A call takes the form and grid of its longest new
+ * rows: single tokens among pieces of prompts are many times faster in a call of their own.
  */
 #define DLLM_CACHE_BF16 0
 #define DLLM_CACHE_FP8 1

@@ -31,7 +31,7 @@ class _Tables:
 
 
 def _streams_of(plan):
-    return struct.unpack(f"={len(plan._packed) // 8}q", plan._packed)[13:]
+    return struct.unpack(f"={len(plan._packed) // 8}q", plan._packed)[10 + 6 * len(plan.groups):]
 
 
 def test_other_streams_wait_once(monkeypatch):

@@ -59,6 +59,10 @@ class Marked:
         per_row = [(b, cached[b], sum(lens[:b]), L, self.sees(cached[b], L, t)) for b, L in enumerate(lens) for t in range(L)]
         self.row = torch.tensor(per_row, dtype=torch.int64).t().to(dev)  # [5, rows]
         self.plan = ChunkPlan(lens, cached, self.tables, dev, mask_block=mask_block)
+        self.bits = bits
+
+    def attend(self, q):
+        return chunk_attention(q, self.k, self.v, self.kc, self.vc, self.plan, SCALE).view(self.n, self.Hq, 128).float()
 
     def sees(self, n, L, t):
         b = self.mask_block
@@ -93,12 +97,10 @@ class Marked:
             dot = d if dot is None else torch.maximum(d, dot)
         return best
 
-    def check(self, a, b, weight_b=0.5):
+    def check(self, a, b):
         q = (self.of(self.codes, a) + self.of(self.codes, b)).to(BF16)
-        o = chunk_attention(q, self.k, self.v, self.kc, self.vc, self.plan, SCALE).view(self.n, self.Hq, 128).float()
+        o = self.attend(q)
         va, vb = self.of(self.values, a), self.of(self.values, b)
-        if not weight_b:
-            vb = va
         ref = 0.5 * (va + vb)
         tol = 2.0 ** -8 * ref.abs() + 1.05 * 2.0 ** -8 * (va.abs() + vb.abs()) + 6e-3
         bad = ~((o - ref).abs() <= tol)
@@ -137,7 +139,7 @@ class Marked:
             sees_b = (b - n < see)[..., None]
             va, vb = self.of(self.values, a), self.of(self.values, b)
             q = (self.of(self.codes, a) + self.of(self.codes, b)).to(BF16)
-            o = chunk_attention(q, self.k, self.v, self.kc, self.vc, self.plan, SCALE).view(self.n, self.Hq, 128).float()
+            o = self.attend(q)
             ref = torch.where(sees_b, 0.5 * (va + vb), va)
             tol = 2.0 ** -8 * ref.abs() + 1.05 * 2.0 ** -8 * (va.abs() + vb.abs()) + 6e-3
             assert ((o - ref).abs() <= tol).all()
@@ -154,9 +156,26 @@ RUNS = [
 ]
 
 
+class OneCall(Marked):
+    """All sequences in one call of the C entry point, where a plan may launch some apart."""
+
+    def attend(self, q):
+        p, (cu, lens, tables) = self.plan, self.plan._args
+        o = torch.full((self.n, self.Hq * 128), float("nan"), dtype=BF16, device=self.dev)
+        need = _capi.chunk_workspace_size(p.n_seg, p.max_q, p.max_cached, self.Hq, self.Hkv, 128, p.total_rows, p.total_cached)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=self.dev)
+        rows = (self.Hq * 128, self.Hkv * 128, self.Hkv * 128, self.Hq * 128)
+        _capi.attn_chunk_paged_fwd_raw(
+            q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), o.data_ptr(), cu, p._seg_ids, p.n_seg, p.max_q,
+            p.max_cached, p.total_rows, p.total_cached, self.kc.data_ptr(), self.vc.data_ptr(),
+            _capi.CACHE_FP8 if self.bits == 8 else _capi.CACHE_BF16, self.kc.shape[0], tables, p.max_pages, lens,
+            self.mask_block, self.Hq, self.Hkv, 128, *rows, SCALE, ws.data_ptr(), need, _capi._stream(self.dev))
+        return o.view(self.n, self.Hq, 128).float()
+
+
 @pytest.mark.parametrize("lens,cached,Hq,Hkv,rows", RUNS)
 def test_segments_in_runs(dev, lens, cached, Hq, Hkv, rows):
-    b = Marked(dev, lens, cached, Hq, Hkv, 8, seed=61, share=True)
+    b = OneCall(dev, lens, cached, Hq, Hkv, 8, seed=61, share=True)
     shape, p = b.shape(), b.plan
     ws = _capi.chunk_workspace_size(p.n_seg, p.max_q, p.max_cached, Hq, Hkv, 128, p.total_rows, p.total_cached)
     a_segment = Hkv * -(-p.max_q * Hq // Hkv // rows) * shape["n_split"]
@@ -215,3 +234,45 @@ def test_every_key_counts_once(dev, lens, cached, Hq, Hkv, mask_block, share, ro
     b.anywhere(6)
     if mask_block:
         b.hidden(4)
+
+
+# ---- long and short new rows in one plan ---------------------------------------------------
+
+MIXED = [
+    # lens, cached, Hq, Hkv, mask_block, sequences of every launch
+    ([1] * 20 + [520] + [1] * 44, [300] * 10 + [0] * 10 + [2000] + [700] * 44, 28, 4, 1, [1, 64]),
+    # three launches, sequences without new rows, another order
+    ([1, 0, 700, 2, 40, 1, 600, 0, 33] + [1] * 20, [50, 9, 800, 31, 0, 2000, 0, 0, 7] + [90 + i for i in range(20)], 8, 2, 4,
+     [2, 2, 25]),
+    # too few rows for an order of their own
+    ([64] + [1] * 10, [500] + [1900] * 10, 14, 2, 1, [1, 10]),
+    ([3, 400, 0, 1], [10, 20, 30, 5], 4, 2, 0, [4]),
+]
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("lens,cached,Hq,Hkv,mask_block,groups", MIXED)
+def test_short_among_long(dev, lens, cached, Hq, Hkv, mask_block, groups, bits, monkeypatch):
+    b = Marked(dev, lens, cached, Hq, Hkv, bits, seed=64, mask_block=mask_block)
+    assert [g[1] for g in b.plan.groups] == groups
+    b.anywhere(12)
+    if mask_block:
+        b.hidden(4)
+    # the Python form, a graph and, launched at once, the C entry point
+    q = torch.randn(b.n, Hq, 128, generator=b.g, device=dev).to(BF16)
+    want = chunk_attention(q, b.k, b.v, b.kc, b.vc, b.plan, SCALE)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chunk_attention(q, b.k, b.v, b.kc, b.vc, b.plan, SCALE)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(chunk_attention(q, b.k, b.v, b.kc, b.vc, b.plan, SCALE), want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    with monkeypatch.context() as m:
+        m.setattr(_capi, "native", None)
+        assert torch.equal(chunk_attention(q, b.k, b.v, b.kc, b.vc, b.plan, SCALE), want)
+    once = OneCall(dev, lens, cached, Hq, Hkv, bits, seed=64, mask_block=mask_block)
+    once.anywhere(4)
