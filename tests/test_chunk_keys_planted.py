@@ -1,4 +1,4 @@
-"""The checker of test_gpu_chunk_keys on the CPU: it passes the formula, and fails it with one
+"""The checks of test_gpu_chunk_keys on the CPU: they pass the formula, and fail it with one
 mistake planted at a time."""
 import pytest
 import torch
